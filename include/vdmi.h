@@ -648,6 +648,56 @@ int vdmi_sla_train_rows_bwd(const void* qkv, const void* qt, const void* dout, c
  * VDMI_SLA_ROWS_MFMA=0 in the environment does the same.  No counterpart in the reference. */
 void vdmi_sla_rows_mfma_enable(int on);
 
+/* ------------------------------------------------------------------------------------------
+ * Attention over time with a decay per head (no counterpart in the reference, whose temporal attention is a softmax over
+ * all frames and keeps no state): per head, with lambda = exp(log_decay[head]), log_decay <= 0, and m = scale,
+ *     S_t = lambda S_(t-1) + k_t v_t^T   (d x d, float),      o_t = m q_t S_t.
+ * Rows of heads by strides (in elements, multiples of 8, pointers 16-byte aligned, the d features of a head contiguous):
+ * element (b, i, t, h) of a vdmi_rows4 starts at p + b*.b + i*.i + t*.n + h*.h, for b < b, i < inner, t < n, h < heads
+ * (sequences are the pairs (b, i): with inner = h*w and .i the row pitch the frames of every site).  d = 32, 64 or 128;
+ * dtype VDMI_DT_BF16 or VDMI_DT_F16 in either library build.
+ * lengths: int32 [b*inner] or NULL - tokens from there on are not read, their rows of o (of dq, dk, dv) are zeros and
+ * the state is the one after the last token.  state_in / state_out: float [b*inner][heads][d][d], the state before the
+ * first and after the last token, either may be NULL (zeros / not wanted) and state_in may be state_out.
+ * Backward: from q, k, v, dout and dstate_in (gradient of the last state; NULL = zeros) the gradients dq, dk, dv and
+ * dstate_out (of the first state; NULL = not wanted; state_in as in the forward, state_out unused).  log_decay and scale
+ * are constants.  A token that is not finite makes the outputs from it on not finite and may make earlier ones of its own
+ * sequence so; other sequences are unaffected.
+ * Sequences of up to 32 tokens without states share 32-row tiles (one launch forward, one backward).  Others are scanned;
+ * few long ones in segments, which takes `workspace` (vdmi_decay_attn_workspace_bytes() bytes, 16-byte aligned, contents
+ * irrelevant; the same for both directions, 0 where none is needed).
+ * ------------------------------------------------------------------------------------------ */
+enum vdmi_dtype { VDMI_DT_BF16 = 0, VDMI_DT_F16 = 1, VDMI_DT_F32 = 2 };
+
+typedef struct vdmi_rows4 {
+    void* p;
+    int64_t b, i, n, h;
+} vdmi_rows4;
+
+typedef struct vdmi_decay_args {
+    int32_t dtype, b, inner, n, heads, d;
+    float scale;
+    int32_t reserved;
+    vdmi_rows4 q, k, v, o;            /* forward: o is written */
+    vdmi_rows4 dout, dq, dk, dv;      /* backward */
+    const float* log_decay;           /* [heads] */
+    const int32_t* lengths;
+    const float* state_in;
+    float* state_out;
+    const float* dstate_in;
+    float* dstate_out;
+    void* workspace;
+    int64_t workspace_bytes;
+} vdmi_decay_args;
+
+size_t vdmi_decay_attn_workspace_bytes(const vdmi_decay_args* a);                          /* HOST */
+int vdmi_decay_attn_fwd(const vdmi_decay_args* a, vdmi_stream stream);
+int vdmi_decay_attn_bwd(const vdmi_decay_args* a, vdmi_stream stream);
+/* One more token of every sequence: `state` (float [seqs][heads][d][d], 16-byte aligned) is updated in place, o written.
+ * strides: int64 [8], host memory - (sequence, head) strides in elements of q, k, v, o. */
+int vdmi_decay_attn_step(const void* q, const void* k, const void* v, void* o, const int64_t* strides, const float* log_decay,
+                         float* state, int dtype, int64_t seqs, int heads, int d, float scale, vdmi_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -82,6 +82,25 @@ class PackJob(C.Structure):
                 ("bkc", C.c_int), ("transposed", C.c_int)]
 
 
+DT_BF16, DT_F16, DT_F32 = 0, 1, 2          # enum vdmi_dtype
+
+
+class Rows4(C.Structure):
+    """include/vdmi.h: vdmi_rows4"""
+    _fields_ = [("p", C.c_void_p), ("b", C.c_int64), ("i", C.c_int64), ("n", C.c_int64), ("h", C.c_int64)]
+
+
+class DecayArgs(C.Structure):
+    """include/vdmi.h: vdmi_decay_args"""
+    _fields_ = [("dtype", C.c_int32), ("b", C.c_int32), ("inner", C.c_int32), ("n", C.c_int32), ("heads", C.c_int32),
+                ("d", C.c_int32), ("scale", C.c_float), ("reserved", C.c_int32),
+                ("q", Rows4), ("k", Rows4), ("v", Rows4), ("o", Rows4),
+                ("dout", Rows4), ("dq", Rows4), ("dk", Rows4), ("dv", Rows4),
+                ("log_decay", C.c_void_p), ("lengths", C.c_void_p), ("state_in", C.c_void_p), ("state_out", C.c_void_p),
+                ("dstate_in", C.c_void_p), ("dstate_out", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64)]
+
+
 class VdmiError(RuntimeError):
     pass
 
@@ -210,6 +229,11 @@ _SIGNATURES = {
     "vdmi_sla_train_rows_fwd": (C.c_int, [C.c_void_p] * 4 + [C.c_int] * 3 + [C.c_float, C.c_void_p]),
     "vdmi_sla_train_rows_bwd": (C.c_int, [C.c_void_p] * 6 + [C.c_int] * 3 + [C.c_float, C.c_void_p]),
     "vdmi_sla_rows_mfma_enable": (None, [C.c_int]),
+    "vdmi_decay_attn_workspace_bytes": (C.c_size_t, [C.POINTER(DecayArgs)]),
+    "vdmi_decay_attn_fwd": (C.c_int, [C.POINTER(DecayArgs), C.c_void_p]),
+    "vdmi_decay_attn_bwd": (C.c_int, [C.POINTER(DecayArgs), C.c_void_p]),
+    "vdmi_decay_attn_step": (C.c_int, [C.c_void_p] * 4 + [C.POINTER(C.c_int64)] + [C.c_void_p] * 2 +
+                             [C.c_int, C.c_int64, C.c_int, C.c_int, C.c_float, C.c_void_p]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -1,0 +1,58 @@
+// Shared by the block operators (decay.hip, blocknorm.hip, rows8.hip), which take the element type per call: both library
+// builds carry bfloat16, IEEE half and float forms of them, so the storage-type switch of vdmi_common.h is undone here.
+#pragma once
+#include "vdmi_common.h"
+#ifdef VDMI_F16
+#undef __bf16
+#undef __builtin_amdgcn_mfma_f32_32x32x16_bf16
+#endif
+
+template <typename T>
+struct Pack;
+template <>
+struct Pack<__bf16> {
+    typedef __attribute__((ext_vector_type(8))) __bf16 x8;
+    static constexpr unsigned EXP = 0x7f80u;       // exponent field: all ones in infinities and NaN
+};
+template <>
+struct Pack<_Float16> {
+    typedef __attribute__((ext_vector_type(8))) _Float16 x8;
+    static constexpr unsigned EXP = 0x7c00u;
+};
+template <typename T>
+using x8_t = typename Pack<T>::x8;
+
+__device__ __forceinline__ f32x16 mfma16(const Pack<__bf16>::x8& a, const Pack<__bf16>::x8& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma16(const Pack<_Float16>::x8& a, const Pack<_Float16>::x8& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.f;
+    return z;
+}
+
+// registers 8 s .. 8 s + 7 of an accumulator as a 16-bit operand: 8 contraction values in accumulator-row order
+template <typename T>
+__device__ __forceinline__ x8_t<T> acc_operand(const f32x16& a, int s) {
+    x8_t<T> f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (T)a[8 * s + j];
+    return f;
+}
+
+typedef short vdmi_s4 __attribute__((ext_vector_type(4)));
+
+// ds_read_b64_tr_b16: the 16 lanes of a group supply four rows x four 8-byte pieces, and each lane receives one column's
+// four values.  Here: contraction values from the four rows at `base` and the four rows `step` bytes further on.
+template <typename T>
+__device__ __forceinline__ x8_t<T> tr_operand(const char* base, int step) {
+    typedef __attribute__((address_space(3))) vdmi_s4* lds_s4;
+    const vdmi_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base));
+    const vdmi_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + step));
+    return __builtin_bit_cast(x8_t<T>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
