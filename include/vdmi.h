@@ -698,6 +698,59 @@ int vdmi_decay_attn_bwd(const vdmi_decay_args* a, vdmi_stream stream);
 int vdmi_decay_attn_step(const void* q, const void* k, const void* v, void* o, const int64_t* strides, const float* log_decay,
                          float* state, int dtype, int64_t seqs, int heads, int d, float scale, vdmi_stream stream);
 
+/* ------------------------------------------------------------------------------------------
+ * The norms before and after a block with its gate and residual scale (the reference's nearest relatives are PreNorm,
+ * Residual and the scale / shift of Block, vdp.py:331-408, 421-427):
+ *     sum = alpha x + gate * P(h) * post_weight           (h NULL: sum = x, and post_weight, gate must be NULL)
+ *     out = sum                                           (forward: non-NULL exactly where h is)
+ *     y   = N(sum) * weight * (1 + scale) + shift         (may be NULL)
+ * over rows of c columns (1 .. 8192), row r of x at x + r * ldx elements, and so on.  kind (of N) and post_kind (of P):
+ * VDMI_NORM_RMS t / sqrt(mean t^2 + eps), VDMI_NORM_LAYER (t - mean) / sqrt(var + eps), post_kind also VDMI_NORM_NONE
+ * (P(h) = h).  weight, post_weight: float [c] or NULL (ones).  gate (NULL: ones), scale, shift (NULL: zeros): float, one row
+ * of c for all rows (stride 0) or one per sample of rows_per_sample consecutive rows (stride c).  Any pitch and element
+ * alignment; multiples of 8 elements at 16-byte aligned addresses take the wide-load form.
+ * Backward: from x, h and the gradients dout (of out, or of sum where h is NULL and it is used elsewhere) and dy, either
+ * NULL for zeros, the gradients dx, dh and, summed over the rows in a fixed order, of the parameters (each NULL where not
+ * wanted; dgate, dscale, dshift have the layout of gate, scale, shift; at most 65535 samples where any is wanted).
+ * workspace: vdmi_block_norm_bwd_workspace_bytes() bytes, 16-byte aligned, contents irrelevant.
+ * ------------------------------------------------------------------------------------------ */
+enum vdmi_norm_kind { VDMI_NORM_NONE = -1, VDMI_NORM_RMS = 0, VDMI_NORM_LAYER = 1 };
+
+typedef struct vdmi_block_norm_args {
+    int32_t dtype, c, kind, post_kind;
+    int64_t rows, rows_per_sample;
+    float eps, alpha;
+    const void* x; const void* h;
+    void* out; void* y;                                  /* forward */
+    const void* dout; const void* dy;                    /* backward */
+    void* dx; void* dh;
+    int64_t ldx, ldh, ldo, ldy, lddo, lddy, lddx, lddh;
+    const float* post_weight; const float* gate; const float* weight; const float* scale; const float* shift;
+    int64_t gate_stride, scale_stride, shift_stride;
+    float* dpost_weight; float* dgate; float* dweight; float* dscale; float* dshift;
+    void* workspace;
+    int64_t workspace_bytes;
+} vdmi_block_norm_args;
+
+int vdmi_block_norm_fwd(const vdmi_block_norm_args* a, vdmi_stream stream);
+size_t vdmi_block_norm_bwd_workspace_bytes(const vdmi_block_norm_args* a);                 /* HOST */
+int vdmi_block_norm_bwd(const vdmi_block_norm_args* a, vdmi_stream stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Activation checkpoints in 8 bits (no counterpart in the reference, which keeps what autograd saves): rows [rows][c], c a
+ * multiple of 8, as codes uint8 [rows][c] (e4m3: 4 exponent, 3 fraction bits, largest 448, no infinities) and exps uint8
+ * [rows][ceil(c / 32)] (e + 127): x ~ code 2^e, e per row and 32 consecutive channels the least exponent whose 448 2^e holds
+ * the group's largest finite magnitude, in -118 .. 119 (magnitudes beyond 448 2^119 become that); rounded to nearest even; infinities and NaN become NaN.
+ * vdmi_rows8_wgrad: weight gradient of a Linear whose input was kept, dw float [cout][cin] = sum_r dy[r][o] x[r][i], from
+ * the codes and bf16 rows dy [rows][cout] (pitch lddy), and db float [cout] = sum_r dy[r][o] (NULL: not wanted); cin, cout
+ * multiples of 8; workspace as stated by vdmi_rows8_wgrad_workspace_bytes().
+ * ------------------------------------------------------------------------------------------ */
+int vdmi_rows8_pack(const void* x, int64_t ldx, void* codes, void* exps, int dtype, int64_t rows, int c, vdmi_stream stream);
+int vdmi_rows8_unpack(const void* codes, const void* exps, void* x, int64_t ldx, int dtype, int64_t rows, int c, vdmi_stream stream);
+size_t vdmi_rows8_wgrad_workspace_bytes(int cin, int cout, int64_t rows);                  /* HOST */
+int vdmi_rows8_wgrad(const void* codes, const void* exps, const void* dy, int64_t lddy, float* dw, float* db, int cin, int cout,
+                     int64_t rows, void* workspace, vdmi_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -4,8 +4,8 @@ definition in 64 bits.
 Tolerances, set before the first run.  u = half a step of the element type (bf16 2^-8, fp16 2^-11).  A kernel rounds the
 weighted pairs (or the state) once as a matrix operand and the result once, so an output element is off by at most
 u (A + |o|), A the same sum with absolute values; 2^-16 A more covers float32 sums.  In the 2-norm the roundings are
-independent, each u / sqrt(3) of what it rounds at most: 1.25 u.  A state sees one split into a high and a low operand
-(u^2 of each product for bf16, 2^-16; independent) and float32 sums: 1e-5 in the 2-norm."""
+independent, each u / sqrt(3) of what it rounds at most: 1.25 u.  A state sees products of sums of 16-bit operands (2^-16
+of them may be lost) and float32 sums: 1e-5 in the 2-norm."""
 import ctypes as C
 
 import pytest

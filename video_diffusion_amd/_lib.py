@@ -101,6 +101,21 @@ class DecayArgs(C.Structure):
                 ("workspace_bytes", C.c_int64)]
 
 
+NORM_KINDS = {None: -1, "rms": 0, "layer": 1}           # enum vdmi_norm_kind
+
+
+class BlockNormArgs(C.Structure):
+    """include/vdmi.h: vdmi_block_norm_args"""
+    _fields_ = ([(f, C.c_int32) for f in ("dtype", "c", "kind", "post_kind")] +
+                [("rows", C.c_int64), ("rows_per_sample", C.c_int64), ("eps", C.c_float), ("alpha", C.c_float)] +
+                [(f, C.c_void_p) for f in ("x", "h", "out", "y", "dout", "dy", "dx", "dh")] +
+                [(f, C.c_int64) for f in ("ldx", "ldh", "ldo", "ldy", "lddo", "lddy", "lddx", "lddh")] +
+                [(f, C.c_void_p) for f in ("post_weight", "gate", "weight", "scale", "shift")] +
+                [(f, C.c_int64) for f in ("gate_stride", "scale_stride", "shift_stride")] +
+                [(f, C.c_void_p) for f in ("dpost_weight", "dgate", "dweight", "dscale", "dshift", "workspace")] +
+                [("workspace_bytes", C.c_int64)])
+
+
 class VdmiError(RuntimeError):
     pass
 
@@ -234,6 +249,14 @@ _SIGNATURES = {
     "vdmi_decay_attn_bwd": (C.c_int, [C.POINTER(DecayArgs), C.c_void_p]),
     "vdmi_decay_attn_step": (C.c_int, [C.c_void_p] * 4 + [C.POINTER(C.c_int64)] + [C.c_void_p] * 2 +
                              [C.c_int, C.c_int64, C.c_int, C.c_int, C.c_float, C.c_void_p]),
+    "vdmi_block_norm_fwd": (C.c_int, [C.POINTER(BlockNormArgs), C.c_void_p]),
+    "vdmi_block_norm_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(BlockNormArgs)]),
+    "vdmi_block_norm_bwd": (C.c_int, [C.POINTER(BlockNormArgs), C.c_void_p]),
+    "vdmi_rows8_pack": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_void_p]),
+    "vdmi_rows8_unpack": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_int64, C.c_int, C.c_void_p]),
+    "vdmi_rows8_wgrad_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int64]),
+    "vdmi_rows8_wgrad": (C.c_int, [C.c_void_p] * 3 + [C.c_int64] + [C.c_void_p] * 2 + [C.c_int, C.c_int, C.c_int64, C.c_void_p,
+                                                                                      C.c_void_p]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -20,7 +20,7 @@
 //     so that the accumulator registers 8s .. 8s+7 of S and O^T are the eight consecutive features 16s + 8 half ..:
 //     the state's registers are then the A operand of q S, whose B operand is a q row as it lies;
 //   * the state stays in float32 registers (16 (d / 32) per lane).  Its update has to be as good as float32 (it is handed
-//     on): lambda^(31-j) v_j is split into a high and a low 16-bit operand (2^-17 of the product is lost), two MFMAs.
+//     on): lambda^(31-j) v_j is the sum of three bfloat16 operands or two halfs (under 2^-22 of it is lost).
 // Few sequences, long: the time axis is cut into segments.  A first launch computes every segment's own contribution to
 // the state (reading k and v only), a second one runs along the segments, a third computes all outputs.
 #include "block_common.h"
@@ -54,10 +54,11 @@ __device__ __forceinline__ float log2_decay(const float* log_decay, int head) {
     return fmaxf(log_decay[head] * LOG2E, -1e4f);
 }
 
-// The matrix cores take subnormal half operands as zeros: the low operands (2^-11 of the values at most) are multiplied up
+// lambda^(..) v as a sum of 16-bit operands: three of bfloat16 (8 bits each), two halfs (11 bits each).
+// The matrix cores take subnormal half operands as zeros: the low halfs (2^-11 of the values at most) are multiplied up
 // by 2^11, and a value that is itself below the normal range goes into the low operand as a whole.  bfloat16 has float's range.
-template <typename T> struct Low { static constexpr float SCALE = 1.f; };
-template <> struct Low<_Float16> { static constexpr float SCALE = 2048.f; };
+template <typename T> struct Low { static constexpr float SCALE = 1.f; static constexpr bool THREE = true; };
+template <> struct Low<_Float16> { static constexpr float SCALE = 2048.f; static constexpr bool THREE = false; };
 template <typename T>
 __device__ __forceinline__ T high_part(float x) { return (T)x; }
 template <>
@@ -68,6 +69,7 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
     typedef x8_t<T> x8;
     constexpr int KS = D / 16, KT = D / 32, KP = 2 * D + 16;
     constexpr float LOW = Low<T>::SCALE;
+    constexpr bool THREE = Low<T>::THREE;
     __shared__ __attribute__((aligned(16))) char kimg_all[DW][32 * KP];
     __shared__ __attribute__((aligned(16))) char vimg_all[DW][32 * VP];
     const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
@@ -203,14 +205,19 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
             token_decays(cnt);
             whole = __builtin_amdgcn_exp2f(l2 * (float)cnt);
         }
-        x8 h0, h1, e0, e1;                  // lambda^(..) v as a high and a low operand
+        x8 h0, h1, e0, e1, f0, f1;          // lambda^(..) v as a sum of operands
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float x0 = (float)v0[j] * uw[j], x1 = (float)v1[j] * uw[8 + j];
             h0[j] = high_part<T>(x0);
             h1[j] = high_part<T>(x1);
-            e0[j] = (T)((x0 - (float)h0[j]) * LOW);
-            e1[j] = (T)((x1 - (float)h1[j]) * LOW);
+            const float y0 = (x0 - (float)h0[j]) * LOW, y1 = (x1 - (float)h1[j]) * LOW;
+            e0[j] = (T)y0;
+            e1[j] = (T)y1;
+            if (THREE) {
+                f0[j] = (T)(y0 - (float)e0[j]);
+                f1[j] = (T)(y1 - (float)e1[j]);
+            }
         }
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
@@ -221,6 +228,12 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
             S[kt] = mfma16(k0, h0, S[kt]);
             add = mfma16(k1, e1, add);
             S[kt] = mfma16(k1, h1, S[kt]);
+            if (THREE) {
+                f32x16 last = mfma16(k0, f0, zero16());
+                last = mfma16(k1, f1, last);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) add[r] += last[r];
+            }
 #pragma unroll
             for (int r = 0; r < 16; ++r) S[kt][r] += add[r] * (1.f / LOW);
         }
