@@ -665,7 +665,8 @@ void vdmi_sla_rows_mfma_enable(int on);
  * sequence so; other sequences are unaffected.
  * Sequences of up to 32 tokens without states share 32-row tiles (one launch forward, one backward).  Others are scanned;
  * few long ones in segments, which takes `workspace` (vdmi_decay_attn_workspace_bytes() bytes, 16-byte aligned, contents
- * irrelevant; the same for both directions, 0 where none is needed).
+ * irrelevant; as many for both directions, 0 where none is needed); the backward then also takes the forward call's
+ * workspace as that call left it, in fwd_workspace.  Token strides (.n) from 0 to VDMI_DECAY_MAX_PITCH elements.
  * ------------------------------------------------------------------------------------------ */
 enum vdmi_dtype { VDMI_DT_BF16 = 0, VDMI_DT_F16 = 1, VDMI_DT_F32 = 2 };
 
@@ -688,7 +689,9 @@ typedef struct vdmi_decay_args {
     float* dstate_out;
     void* workspace;
     int64_t workspace_bytes;
+    const void* fwd_workspace;        /* backward */
 } vdmi_decay_args;
+#define VDMI_DECAY_MAX_PITCH (1LL << 25)
 
 size_t vdmi_decay_attn_workspace_bytes(const vdmi_decay_args* a);                          /* HOST */
 int vdmi_decay_attn_fwd(const vdmi_decay_args* a, vdmi_stream stream);

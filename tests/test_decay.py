@@ -380,6 +380,23 @@ def test_offsets_beyond_32_bits():
 
 
 @gpu
+@pytest.mark.parametrize("inner", [1, 2, 3, 7, 64, 1000, 4097])
+def test_many_sites(inner):
+    """Short sequences find their rows by a division by the number of sites."""
+    q, k, v, do, decay, *_ = inputs(3, inner, 5, 1, 32, torch.bfloat16, inner)
+    check_all(f"sites.{inner}", q, k, v, do, decay, None, None, None)
+
+
+@gpu
+def test_pitches_beyond_the_kernels():
+    """Token strides of more than 2^25 elements are read from a copy."""
+    big = torch.zeros(3 * (1 << 25) + 3 * 4096, device=DEV, dtype=torch.bfloat16)
+    t = big.as_strided((1, 1, 3, 2, 32), (0, 0, (1 << 25) + 1024, 32, 1))
+    t.copy_(torch.randn(1, 1, 3, 2, 32, device=DEV))
+    check_all("pitch", t, t, t, t, torch.tensor([-0.1, -0.5], device=DEV), None, None, None)
+
+
+@gpu
 def test_no_tokens_and_no_sequences():
     from video_diffusion_amd import block_hip as B
     decay = torch.zeros(2, device=DEV)
@@ -429,7 +446,10 @@ def test_entry_points_refuse_bad_arguments():
     need = lib.vdmi_decay_attn_workspace_bytes(C.byref(_args(**long)))
     assert need > 0 and need % (2 * 64 * 64 * 4) == 0
     assert fwd(**long) == E_ARG and fwd(**long, workspace=256, workspace_bytes=need - 1) == E_ARG
-    assert bwd(**long, workspace=256, workspace_bytes=need - 1) == E_ARG
+    assert bwd(**long, workspace=256, workspace_bytes=need - 1, fwd_workspace=256) == E_ARG
+    assert bwd(**long, workspace=256, workspace_bytes=need) == E_ARG            # the forward's states
+    for f, r in ((fwd, "q_n"), (fwd, "o_n"), (bwd, "v_n"), (bwd, "dk_n")):
+        assert f(**{r: (1 << 25) + 8}) == E_SHAPE and f(**{r: -8}) == E_SHAPE
     assert lib.vdmi_decay_attn_workspace_bytes(C.byref(_args(d=48))) == 0
     st = (C.c_int64 * 8)(*[64, 32] * 4)
     step = lambda *a: lib.vdmi_decay_attn_step(*a, None)

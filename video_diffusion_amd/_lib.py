@@ -98,8 +98,10 @@ class DecayArgs(C.Structure):
                 ("dout", Rows4), ("dq", Rows4), ("dk", Rows4), ("dv", Rows4),
                 ("log_decay", C.c_void_p), ("lengths", C.c_void_p), ("state_in", C.c_void_p), ("state_out", C.c_void_p),
                 ("dstate_in", C.c_void_p), ("dstate_out", C.c_void_p), ("workspace", C.c_void_p),
-                ("workspace_bytes", C.c_int64)]
+                ("workspace_bytes", C.c_int64), ("fwd_workspace", C.c_void_p)]
 
+
+DECAY_MAX_PITCH = 1 << 25
 
 NORM_KINDS = {None: -1, "rms": 0, "layer": 1}           # enum vdmi_norm_kind
 

@@ -24,55 +24,76 @@ from ._lib import VdmiError, check
 from .train_hip import _plain
 
 _DTYPES = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16, torch.float32: _lib.DT_F32}
+_FLOAT16S = (torch.bfloat16, torch.float16)
 
 
-def _stream_of(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+class _on_device:
+    """`with _on_device(t) as stream:` - t's device is the current one inside, stream its current stream's handle."""
+    __slots__ = ("index", "prev")
+
+    def __init__(self, t: torch.Tensor):
+        self.index = t.device.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+        return False
 
 
-def _require(ok, what: str):
-    if not ok:
-        raise VdmiError(what)
-
-
-def _on_gpu(*ts):
-    first = next(t for t in ts if t is not None)
+def _on_gpu(first, *ts):
+    dev = first.device
+    if dev.type != "cuda":
+        raise VdmiError("the block operators need CUDA (HIP) tensors; there is no CPU path")
     for t in ts:
-        if t is None:
-            continue
-        _require(t.is_cuda, "the block operators need CUDA (HIP) tensors; there is no CPU path")
-        _require(t.device == first.device, f"tensors on different devices: {t.device} and {first.device}")
+        if t is not None and t.device != dev:
+            raise VdmiError("the block operators need CUDA (HIP) tensors; there is no CPU path" if not t.is_cuda else
+                            f"tensors on different devices: {t.device} and {dev}")
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _wants_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # attention over time with a decay per head
 # ---------------------------------------------------------------------------------------------------------------------
-def _rows4(t: torch.Tensor) -> "_lib.Rows4":
-    """t: [b, inner, n, heads, d]"""
-    return _lib.Rows4(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.stride(3))
-
-
 def _row_operand(t: torch.Tensor) -> torch.Tensor:
-    """t as the kernels read it - 16-byte pieces of d contiguous features at any non-negative strides - or a copy that is."""
-    pieces = all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
-    if t.stride(-1) == 1 and pieces and t.data_ptr() % 16 == 0:
-        if all(n > 1 or s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])):
-            return t
-        # a dimension of one element may have any stride; the library is told 0
-        return t.as_strided(t.shape, [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])] + [1])
-    return t.contiguous()
+    """t [b, inner, n, heads, d] as the kernels read it - 16-byte pieces of d contiguous features at any non-negative
+    strides - or a copy that is."""
+    s = t.stride()
+    if s[4] == 1 and not ((s[0] | s[1] | s[2] | s[3]) & 7) and s[2] <= _lib.DECAY_MAX_PITCH and not t.data_ptr() & 15:
+        return t
+    # a dimension of one element may have any stride: the library is told 0
+    fixed = [x if n > 1 else 0 for x, n in zip(s[:4], t.shape[:4])]
+    if s[4] == 1 and not any(x & 7 for x in fixed) and fixed[2] <= _lib.DECAY_MAX_PITCH and not t.data_ptr() & 15:
+        return t.as_strided(t.shape, fixed + [1])
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _empty_like_rows(t: torch.Tensor) -> torch.Tensor:
     """An uninitialised dense tensor of t's shape whose dimensions lie in memory in t's order: the sites of a frame stay
     next to each other where t is a permuted view of (batch, frame, site) rows.  Broadcast dimensions of t become real."""
-    order = sorted(range(t.dim() - 1), key=lambda i: (-t.stride(i), i)) + [t.dim() - 1]
-    out = torch.empty([t.shape[i] for i in order], device=t.device, dtype=t.dtype)
-    return out.permute([order.index(i) for i in range(t.dim())])
+    shape, s = t.shape, t.stride()
+    strides, pitch = [0, 0, 0, 0, 1], shape[4]
+    for i in sorted(range(4), key=lambda i: (s[i], -i)):
+        strides[i] = pitch
+        pitch *= shape[i]
+    return t.new_empty_strided(shape, strides)
+
+
+def _set_rows(r: "_lib.Rows4", t: torch.Tensor):
+    r.p = t.data_ptr()
+    r.b, r.i, r.n, r.h, _ = t.stride()
 
 
 def _decay_args(q, k, v, log_decay, lengths, state, scale) -> "_lib.DecayArgs":
@@ -80,17 +101,36 @@ def _decay_args(q, k, v, log_decay, lengths, state, scale) -> "_lib.DecayArgs":
     a.dtype = _DTYPES[q.dtype]
     a.b, a.inner, a.n, a.heads, a.d = q.shape
     a.scale = scale
-    a.q, a.k, a.v = _rows4(q), _rows4(k), _rows4(v)
+    _set_rows(a.q, q)
+    _set_rows(a.k, k)
+    _set_rows(a.v, v)
     a.log_decay, a.lengths, a.state_in = log_decay.data_ptr(), _ptr(lengths), _ptr(state)
     return a
 
 
-def _run_decay(fn: str, a, device, stream):
-    lib = _lib.lib()
-    a.workspace_bytes = lib.vdmi_decay_attn_workspace_bytes(C.byref(a))
-    ws = torch.empty(a.workspace_bytes, device=device, dtype=torch.uint8) if a.workspace_bytes else None
-    a.workspace = _ptr(ws)
-    check(getattr(lib, fn)(C.byref(a), stream), fn)
+def _decay_workspace(a, like):
+    size = _lib.lib().vdmi_decay_attn_workspace_bytes(C.byref(a))
+    if not size:
+        return None
+    ws = torch.empty(size, device=like.device, dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), size
+    return ws
+
+
+def _decay_forward(q, k, v, state, log_decay, lengths, scale, return_state):
+    """(o, last state or None, the workspace) of operands as the kernels read them."""
+    with _on_device(q) as stream:
+        o = _empty_like_rows(q)
+        last = None
+        a = _decay_args(q, k, v, log_decay, lengths, state, scale)
+        _set_rows(a.o, o)
+        if return_state:
+            b, inner, _, h, d = q.shape
+            last = torch.empty((b, inner, h, d, d), device=q.device, dtype=torch.float32)
+            a.state_out = last.data_ptr()
+        ws = _decay_workspace(a, q)
+        check(_lib.lib().vdmi_decay_attn_fwd(C.byref(a), stream), "vdmi_decay_attn_fwd")
+    return o, last, ws
 
 
 class DecayAttnFn(torch.autograd.Function):
@@ -98,59 +138,65 @@ class DecayAttnFn(torch.autograd.Function):
     lengths, scale."""
 
     @staticmethod
-    @_plain
     def forward(ctx, q, k, v, state, log_decay, lengths, scale, return_state):
         q, k, v = _row_operand(q), _row_operand(k), _row_operand(v)
-        with torch.cuda.device(q.device):
-            o = _empty_like_rows(q)
-            b, inner, n, h, d = q.shape
-            last = torch.empty(b, inner, h, d, d, device=q.device, dtype=torch.float32) if return_state else None
-            a = _decay_args(q, k, v, log_decay, lengths, state, scale)
-            a.o, a.state_out = _rows4(o), _ptr(last)
-            _run_decay("vdmi_decay_attn_fwd", a, q.device, _stream_of(q))
-        ctx.save_for_backward(q, k, v, state, log_decay, lengths)
+        o, last, ws = _decay_forward(q, k, v, state, log_decay, lengths, scale, return_state)
+        ctx.save_for_backward(q, k, v, state, log_decay, lengths, ws)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         return o, last
 
     @staticmethod
-    @_plain
     def backward(ctx, do, dlast):
-        q, k, v, state, log_decay, lengths = ctx.saved_tensors
+        q, k, v, state, log_decay, lengths, fwd_ws = ctx.saved_tensors
         need = ctx.needs_input_grad
         if do is None and dlast is None:
             return (None,) * 8
-        with torch.cuda.device(q.device):
-            do = torch.zeros_like(q) if do is None else do
-            do = _row_operand(do.to(q.dtype))
+        with _on_device(q) as stream:
+            do = torch.zeros_like(q) if do is None else _row_operand(do.to(q.dtype))
             dlast = None if dlast is None else dlast.to(torch.float32).contiguous()
             dq, dk, dv = _empty_like_rows(q), _empty_like_rows(k), _empty_like_rows(v)
-            dstate = torch.empty_like(state) if need[3] and state is not None else None
             a = _decay_args(q, k, v, log_decay, lengths, state, ctx.scale)
-            a.dout, a.dq, a.dk, a.dv = _rows4(do), _rows4(dq), _rows4(dk), _rows4(dv)
-            a.dstate_in, a.dstate_out = _ptr(dlast), _ptr(dstate)
-            _run_decay("vdmi_decay_attn_bwd", a, q.device, _stream_of(q))
+            _set_rows(a.dout, do)
+            _set_rows(a.dq, dq)
+            _set_rows(a.dk, dk)
+            _set_rows(a.dv, dv)
+            dstate = None
+            if need[3]:
+                dstate = torch.empty_like(state)
+                a.dstate_out = dstate.data_ptr()
+            a.dstate_in, a.fwd_workspace = _ptr(dlast), _ptr(fwd_ws)
+            ws = _decay_workspace(a, q)
+            check(_lib.lib().vdmi_decay_attn_bwd(C.byref(a), stream), "vdmi_decay_attn_bwd")
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dstate, None, None, None, None)
 
 
 def _check_decay(q, k, v, log_decay, state, lead, heads, d):
-    _on_gpu(q, k, v, log_decay, state)
-    _require(q.dtype in (torch.bfloat16, torch.float16), f"q, k, v are bfloat16 or float16 (got {q.dtype})")
-    _require(k.dtype == q.dtype and v.dtype == q.dtype, f"q, k, v have one dtype (got {q.dtype}, {k.dtype}, {v.dtype})")
-    _require(k.shape == q.shape and v.shape == q.shape,
-             f"q, k, v have one shape (got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)})")
-    _require(d in (32, 64, 128), f"heads of 32, 64 or 128 features (got {d})")
-    _require(log_decay.dtype == torch.float32 and log_decay.shape == (heads,),
-             f"log_decay is float32 [{heads}] (got {log_decay.dtype} {tuple(log_decay.shape)})")
-    _require(not log_decay.requires_grad, "log_decay is a constant of the layer: no gradient is computed for it")
-    if state is not None:
-        _require(state.dtype == torch.float32 and tuple(state.shape) == (*lead, heads, d, d),
-                 f"the state is float32 {(*lead, heads, d, d)} (got {state.dtype} {tuple(state.shape)})")
+    if (q.dtype in _FLOAT16S and k.dtype == q.dtype and v.dtype == q.dtype and k.shape == q.shape and v.shape == q.shape and
+            d in (32, 64, 128) and log_decay.dtype == torch.float32 and log_decay.shape == (heads,) and not log_decay.requires_grad and
+            (state is None or (state.dtype == torch.float32 and state.shape == (*lead, heads, d, d)))):
+        return
+    if q.dtype not in _FLOAT16S:
+        raise VdmiError(f"q, k, v are bfloat16 or float16 (got {q.dtype})")
+    if not (k.dtype == q.dtype and v.dtype == q.dtype):
+        raise VdmiError(f"q, k, v have one dtype (got {q.dtype}, {k.dtype}, {v.dtype})")
+    if not (k.shape == q.shape and v.shape == q.shape):
+        raise VdmiError(f"q, k, v have one shape (got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)})")
+    if d not in (32, 64, 128):
+        raise VdmiError(f"heads of 32, 64 or 128 features (got {d})")
+    if log_decay.requires_grad:
+        raise VdmiError("log_decay is a constant of the layer: no gradient is computed for it")
+    if not (log_decay.dtype == torch.float32 and log_decay.shape == (heads,)):
+        raise VdmiError(f"log_decay is float32 [{heads}] (got {log_decay.dtype} {tuple(log_decay.shape)})")
+    raise VdmiError(f"the state is float32 {(*lead, heads, d, d)} (got {state.dtype} {tuple(state.shape)})")
 
 
 def _scale(scale, d):
-    scale = d ** -0.5 if scale is None else float(scale)
-    _require(scale != 0 and abs(scale) < 3e38, f"scale is finite and not zero (got {scale})")
+    if scale is None:
+        return d ** -0.5
+    scale = float(scale)
+    if scale == 0 or not abs(scale) < 3e38:
+        raise VdmiError(f"scale is finite and not zero (got {scale})")
     return scale
 
 
@@ -164,14 +210,16 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengt
     the first token (zeros by default).  lengths: int32 [b(, sites)] - tokens from there on are padding: they are not read,
     their outputs and gradients are zeros.  return_state: also return S after the last token, for decay_attention_step or
     the next piece of the sequence.  Returns o like q (in q's order of dimensions in memory), or (o, state)."""
-    _require(q.dim() in (4, 5), f"q is [b, n, heads, d] or [b, sites, n, heads, d] (got {q.dim()} dimensions)")
-    lead, (n, heads, d) = tuple(q.shape[:-3]), q.shape[-3:]
+    dims = q.dim()
+    if dims not in (4, 5):
+        raise VdmiError(f"q is [b, n, heads, d] or [b, sites, n, heads, d] (got {dims} dimensions)")
+    lead, (n, heads, d) = q.shape[:-3], q.shape[-3:]
+    _on_gpu(q, k, v, log_decay, initial_state, lengths)
     _check_decay(q, k, v, log_decay, initial_state, lead, heads, d)
     scale = _scale(scale, d)
     if lengths is not None:
-        _on_gpu(q, lengths)
-        _require(lengths.dtype == torch.int32 and tuple(lengths.shape) == lead,
-                 f"lengths is int32 {lead} (got {lengths.dtype} {tuple(lengths.shape)})")
+        if not (lengths.dtype == torch.int32 and lengths.shape == lead):
+            raise VdmiError(f"lengths is int32 {tuple(lead)} (got {lengths.dtype} {tuple(lengths.shape)})")
         lengths = lengths.contiguous()
     if q.numel() == 0:
         # no sequences, or sequences of no tokens: the state stays
@@ -179,15 +227,20 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengt
         if not return_state:
             return o
         return o, (torch.zeros(*lead, heads, d, d, device=q.device) if initial_state is None else initial_state.clone())
-    four = q.dim() == 4
-    if four:
+    if dims == 4:
         q, k, v = q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1)
-    b, inner = q.shape[:2]
-    state = None if initial_state is None else initial_state.reshape(b, inner, heads, d, d).contiguous()
-    if state is not None and state.data_ptr() % 16:
-        state = state.clone()
-    o, last = DecayAttnFn.apply(q, k, v, state, log_decay.contiguous(), lengths, scale, bool(return_state))
-    o = o.squeeze(1) if four else o
+    state = initial_state
+    if state is not None:
+        state = state.reshape(*q.shape[:2], heads, d, d).contiguous()
+        if state.data_ptr() & 15:
+            state = state.clone()
+    log_decay = log_decay.contiguous()
+    if _wants_grad(q, k, v, state):
+        o, last = DecayAttnFn.apply(q, k, v, state, log_decay, lengths, scale, bool(return_state))
+    else:
+        o, last, _ = _decay_forward(_row_operand(q), _row_operand(k), _row_operand(v), state, log_decay, lengths, scale, return_state)
+    if dims == 4:
+        o = o.squeeze(1)
     return (o, last.view(*lead, heads, d, d)) if return_state else o
 
 
@@ -195,27 +248,28 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
     """One more token of every sequence: state (float32 [..., heads, d, d], contiguous) is updated in place to
     exp(log_decay) state + k v^T, and scale * q state is returned.  q, k, v: bfloat16 or float16 [..., heads, d].  For
     sampling: no gradients."""
-    _require(q.dim() >= 2, f"q is [..., heads, d] (got {q.dim()} dimensions)")
-    lead, (heads, d) = tuple(q.shape[:-2]), q.shape[-2:]
+    if q.dim() < 2:
+        raise VdmiError(f"q is [..., heads, d] (got {q.dim()} dimensions)")
+    shape = q.shape
+    lead, (heads, d) = shape[:-2], shape[-2:]
+    _on_gpu(q, k, v, log_decay, state)
     _check_decay(q, k, v, log_decay, state, lead, heads, d)
     scale = _scale(scale, d)
-    _require(state.is_contiguous() and state.data_ptr() % 16 == 0, "the state is contiguous and 16-byte aligned")
-    _require(not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state))),
-             "decay_attention_step computes no gradients: call it under torch.no_grad(), or decay_attention")
-    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    if not state.is_contiguous() or state.data_ptr() & 15:
+        raise VdmiError("the state is contiguous and 16-byte aligned")
+    if _wants_grad(q, k, v, state):
+        raise VdmiError("decay_attention_step computes no gradients: call it under torch.no_grad(), or decay_attention")
+    o = torch.empty(shape, device=q.device, dtype=q.dtype)
     if q.numel() == 0:
         return o
-
-    def flat(t):
-        t = t.reshape(-1, heads, d)
-        return t if t.stride(-1) == 1 else t.contiguous()
-
-    ops = [flat(q), flat(k), flat(v), o.view(-1, heads, d)]
-    strides = (C.c_int64 * 8)(*[s for t in ops for s in t.stride()[:2]])
-    with torch.cuda.device(q.device):
-        check(_lib.lib().vdmi_decay_attn_step(*[t.data_ptr() for t in ops], strides, log_decay.contiguous().data_ptr(),
-                                              state.data_ptr(), _DTYPES[q.dtype], ops[0].shape[0], heads, d, scale,
-                                              _stream_of(q)), "vdmi_decay_attn_step")
+    if q.dim() != 3:
+        q, k, v = q.reshape(-1, heads, d), k.reshape(-1, heads, d), v.reshape(-1, heads, d)
+    q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
+    strides = (C.c_int64 * 8)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], heads * d, d)
+    with _on_device(q) as stream:
+        check(_lib.lib().vdmi_decay_attn_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), strides,
+                                              log_decay.contiguous().data_ptr(), state.data_ptr(), _DTYPES[q.dtype], q.shape[0],
+                                              heads, d, scale, stream), "vdmi_decay_attn_step")
     return o
 
 
@@ -236,30 +290,23 @@ class BlockNormFn(torch.autograd.Function):
     """(out, y) of rows x, h and parameters; out None without h, y None unless want_y."""
 
     @staticmethod
-    @_plain
     def forward(ctx, x, h, post_weight, gate, weight, scale, shift, alpha, kind, post_kind, eps, want_y):
-        params = [None if p is None else p.detach().contiguous() for p in (post_weight, gate, weight, scale, shift)]
+        params = [None if p is None else p.contiguous() for p in (post_weight, gate, weight, scale, shift)]
         xr, hr = _rows2(x), None if h is None else _rows2(h)
-        with torch.cuda.device(x.device):
-            out = None if h is None else torch.empty(x.shape, device=x.device, dtype=x.dtype)
-            y = torch.empty(x.shape, device=x.device, dtype=x.dtype) if want_y else None
-            a = _norm_args(xr, hr, params, x.shape[0], alpha, kind, post_kind, eps)
-            a.out, a.y, a.ldo, a.ldy = _ptr(out), _ptr(y), x.shape[-1], x.shape[-1]
-            check(_lib.lib().vdmi_block_norm_fwd(C.byref(a), _stream_of(x)), "vdmi_block_norm_fwd")
+        out, y = _norm_forward(x, xr, hr, params, alpha, kind, post_kind, eps, want_y)
         ctx.save_for_backward(xr, hr, *params)
         ctx.meta = (tuple(x.shape), alpha, kind, post_kind, eps)
         ctx.set_materialize_grads(False)
         return out, y
 
     @staticmethod
-    @_plain
     def backward(ctx, dout, dy):
         xr, hr, *params = ctx.saved_tensors
         shape, alpha, kind, post_kind, eps = ctx.meta
         need = ctx.needs_input_grad
         if dout is None and dy is None:
             return (None,) * 12
-        with torch.cuda.device(xr.device):
+        with _on_device(xr) as stream:
             dout, dy = (None if g is None else _rows2(g.to(xr.dtype)) for g in (dout, dy))
             dx = torch.empty(shape, device=xr.device, dtype=xr.dtype) if need[0] else None
             dh = torch.empty(shape, device=xr.device, dtype=xr.dtype) if need[1] else None
@@ -277,8 +324,19 @@ class BlockNormFn(torch.autograd.Function):
             a.workspace_bytes = lib.vdmi_block_norm_bwd_workspace_bytes(C.byref(a))
             ws = torch.empty(a.workspace_bytes, device=xr.device, dtype=torch.uint8) if a.workspace_bytes else None
             a.workspace = _ptr(ws)
-            check(lib.vdmi_block_norm_bwd(C.byref(a), _stream_of(xr)), "vdmi_block_norm_bwd")
+            check(lib.vdmi_block_norm_bwd(C.byref(a), stream), "vdmi_block_norm_bwd")
         return (dx, dh, *grads, None, None, None, None, None)
+
+
+def _norm_forward(x, xr, hr, params, alpha, kind, post_kind, eps, want_y):
+    with _on_device(xr) as stream:
+        out = None if hr is None else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        y = torch.empty(x.shape, device=x.device, dtype=x.dtype) if want_y else None
+        a = _norm_args(xr, hr, params, x.shape[0], alpha, kind, post_kind, eps)
+        a.out, a.y = _ptr(out), _ptr(y)
+        a.ldo = a.ldy = x.shape[-1]
+        check(_lib.lib().vdmi_block_norm_fwd(C.byref(a), stream), "vdmi_block_norm_fwd")
+    return out, y
 
 
 def _norm_args(xr, hr, params, samples, alpha, kind, post_kind, eps) -> "_lib.BlockNormArgs":
@@ -297,23 +355,32 @@ def _norm_args(xr, hr, params, samples, alpha, kind, post_kind, eps) -> "_lib.Bl
 
 def _block_norm(x, h, post_weight, gate, weight, scale, shift, alpha, kind, post_kind, eps, want_y):
     _on_gpu(x, h, post_weight, gate, weight, scale, shift)
-    _require(x.dtype in _DTYPES, f"rows are bfloat16, float16 or float32 (got {x.dtype})")
-    _require(x.dim() >= 2 and 1 <= x.shape[-1] <= 8192, f"rows are [samples, ..., c] with c from 1 to 8192 (got {tuple(x.shape)})")
-    _require(h is None or (h.dtype == x.dtype and h.shape == x.shape),
-             None if h is None else f"x and h are alike (got {x.dtype} {tuple(x.shape)}, {h.dtype} {tuple(h.shape)})")
+    if x.dtype not in _DTYPES:
+        raise VdmiError(f"rows are bfloat16, float16 or float32 (got {x.dtype})")
+    if x.dim() < 2 or not 1 <= x.shape[-1] <= 8192:
+        raise VdmiError(f"rows are [samples, ..., c] with c from 1 to 8192 (got {tuple(x.shape)})")
+    if h is not None and not (h.dtype == x.dtype and h.shape == x.shape):
+        raise VdmiError(f"x and h are alike (got {x.dtype} {tuple(x.shape)}, {h.dtype} {tuple(h.shape)})")
     b, c = x.shape[0], x.shape[-1]
     for name, p in (("post_weight", post_weight), ("weight", weight)):
-        _require(p is None or (p.dtype == torch.float32 and tuple(p.shape) == (c,)), f"{name} is float32 [{c}]")
+        if p is not None and not (p.dtype == torch.float32 and p.shape == (c,)):
+            raise VdmiError(f"{name} is float32 [{c}]")
     for name, p in (("gate", gate), ("scale", scale), ("shift", shift)):
-        _require(p is None or (p.dtype == torch.float32 and tuple(p.shape) in ((c,), (1, c), (b, c))),
-                 f"{name} is float32 [{c}], [1, {c}] or [{b}, {c}]")
-    _require(kind in ("rms", "layer"), f"kind is 'rms' or 'layer' (got {kind!r})")
-    _require(post_kind in ("rms", "layer", None), f"the kind of the norm after the block is 'rms', 'layer' or None (got {post_kind!r})")
+        if p is not None and not (p.dtype == torch.float32 and (p.shape == (b, c) or p.shape == (c,) or p.shape == (1, c))):
+            raise VdmiError(f"{name} is float32 [{c}], [1, {c}] or [{b}, {c}]")
+    if kind not in ("rms", "layer"):
+        raise VdmiError(f"kind is 'rms' or 'layer' (got {kind!r})")
+    if post_kind not in ("rms", "layer", None):
+        raise VdmiError(f"the kind of the norm after the block is 'rms', 'layer' or None (got {post_kind!r})")
     eps, alpha = float(eps), float(alpha)
-    _require(0 <= eps < 1e30 and abs(alpha) < 3e38, f"eps is not negative and alpha finite (got {eps}, {alpha})")
+    if not (0 <= eps < 1e30 and abs(alpha) < 3e38):
+        raise VdmiError(f"eps is not negative and alpha finite (got {eps}, {alpha})")
     if x.numel() == 0:
         return (None if h is None else x + h), (x * 1 if want_y else None)
-    return BlockNormFn.apply(x, h, post_weight, gate, weight, scale, shift, alpha, kind, post_kind, eps, want_y)
+    if _wants_grad(x, h, post_weight, gate, weight, scale, shift):
+        return BlockNormFn.apply(x, h, post_weight, gate, weight, scale, shift, alpha, kind, post_kind, eps, want_y)
+    params = [None if p is None else p.contiguous() for p in (post_weight, gate, weight, scale, shift)]
+    return _norm_forward(x, _rows2(x), None if h is None else _rows2(h), params, alpha, kind, post_kind, eps, want_y)
 
 
 def norm_before(x, weight=None, scale=None, shift=None, *, kind="rms", eps=1e-5):
@@ -351,14 +418,21 @@ class Rows8:
     def unpack(self, dtype=None) -> torch.Tensor:
         """The values the codes stand for, in the packed tensor's shape."""
         dtype = self.dtype if dtype is None else dtype
-        _require(dtype in _DTYPES, f"rows are bfloat16, float16 or float32 (got {dtype})")
+        if dtype not in _DTYPES:
+            raise VdmiError(f"rows are bfloat16, float16 or float32 (got {dtype})")
         out = torch.empty(self.shape, device=self.codes.device, dtype=dtype)
         if out.numel():
             rows, c = self.codes.shape
-            with torch.cuda.device(out.device):
+            with _on_device(out) as stream:
                 check(_lib.lib().vdmi_rows8_unpack(self.codes.data_ptr(), self.exps.data_ptr(), out.data_ptr(), c, _DTYPES[dtype],
-                                                   rows, c, _stream_of(out)), "vdmi_rows8_unpack")
+                                                   rows, c, stream), "vdmi_rows8_unpack")
         return out
+
+
+def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """_rows2 of t's values, at 16-byte aligned rows."""
+    r = _rows2(t.detach())
+    return r.clone(memory_format=torch.contiguous_format) if r.data_ptr() & 15 or _pitch(r) % 8 else r
 
 
 def pack_rows8(x: torch.Tensor) -> Rows8:
@@ -366,18 +440,18 @@ def pack_rows8(x: torch.Tensor) -> Rows8:
     row and 32 channels that holds the largest magnitude.  Off by 2^-4 of a value at most (2^-18 of its group's largest for
     the smallest ones); infinities and NaN come back as NaN, magnitudes beyond 448 * 2^119 as that."""
     _on_gpu(x)
-    _require(x.dtype in _DTYPES, f"rows are bfloat16, float16 or float32 (got {x.dtype})")
-    _require(x.dim() >= 1 and x.shape[-1] > 0 and x.shape[-1] % 8 == 0, f"rows of a multiple of 8 channels (got {tuple(x.shape)})")
-    with torch.no_grad(), torch.cuda.device(x.device):
-        r = _rows2(x.detach())
-        if r.data_ptr() % 16 or _pitch(r) % 8:
-            r = r.contiguous().clone() if r.is_contiguous() else r.contiguous()
+    if x.dtype not in _DTYPES:
+        raise VdmiError(f"rows are bfloat16, float16 or float32 (got {x.dtype})")
+    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 8:
+        raise VdmiError(f"rows of a multiple of 8 channels (got {tuple(x.shape)})")
+    with _on_device(x) as stream:
+        r = _aligned_rows(x)
         rows, c = r.shape
-        codes = torch.empty(rows, c, device=x.device, dtype=torch.uint8)
-        exps = torch.empty(rows, (c + 31) // 32, device=x.device, dtype=torch.uint8)
+        codes = torch.empty((rows, c), device=x.device, dtype=torch.uint8)
+        exps = torch.empty((rows, (c + 31) // 32), device=x.device, dtype=torch.uint8)
         if rows:
             check(_lib.lib().vdmi_rows8_pack(r.data_ptr(), _pitch(r), codes.data_ptr(), exps.data_ptr(), _DTYPES[x.dtype], rows, c,
-                                             _stream_of(x)), "vdmi_rows8_pack")
+                                             stream), "vdmi_rows8_pack")
     return Rows8(codes, exps, tuple(x.shape), x.dtype)
 
 
@@ -387,22 +461,23 @@ def rows8_wgrad(kept: Rows8, dy: torch.Tensor, bias: bool = False):
     _on_gpu(kept.codes, dy)
     rows, cin = kept.codes.shape
     cout = dy.shape[-1]
-    _require(dy.dtype == torch.bfloat16, f"dy is bfloat16 (got {dy.dtype})")
-    _require(cout > 0 and cout % 8 == 0, f"a multiple of 8 output channels (got {cout})")
-    _require(dy.numel() == rows * cout, f"dy has a row for each of the {rows} kept rows (got {tuple(dy.shape)})")
-    with torch.no_grad(), torch.cuda.device(dy.device):
-        d = _rows2(dy.detach())
-        if d.data_ptr() % 16 or _pitch(d) % 8:
-            d = d.contiguous().clone() if d.is_contiguous() else d.contiguous()
+    if dy.dtype != torch.bfloat16:
+        raise VdmiError(f"dy is bfloat16 (got {dy.dtype})")
+    if cout == 0 or cout % 8:
+        raise VdmiError(f"a multiple of 8 output channels (got {cout})")
+    if dy.numel() != rows * cout:
+        raise VdmiError(f"dy has a row for each of the {rows} kept rows (got {tuple(dy.shape)})")
+    with _on_device(dy) as stream:
         if rows == 0:
             dw, db = torch.zeros(cout, cin, device=dy.device), torch.zeros(cout, device=dy.device)
             return (dw, db) if bias else dw
+        d = _aligned_rows(dy)
         lib = _lib.lib()
-        dw = torch.empty(cout, cin, device=dy.device, dtype=torch.float32)
+        dw = torch.empty((cout, cin), device=dy.device, dtype=torch.float32)
         db = torch.empty(cout, device=dy.device, dtype=torch.float32) if bias else None
         ws = torch.empty(lib.vdmi_rows8_wgrad_workspace_bytes(cin, cout, rows), device=dy.device, dtype=torch.uint8)
         check(lib.vdmi_rows8_wgrad(kept.codes.data_ptr(), kept.exps.data_ptr(), d.data_ptr(), _pitch(d), dw.data_ptr(), _ptr(db),
-                                   cin, cout, rows, ws.data_ptr(), _stream_of(dy)), "vdmi_rows8_wgrad")
+                                   cin, cout, rows, ws.data_ptr(), stream), "vdmi_rows8_wgrad")
     return (dw, db) if bias else dw
 
 
@@ -413,7 +488,7 @@ class LinearRows8Fn(torch.autograd.Function):
     @_plain
     def forward(ctx, x, weight, bias):
         from .train_hip import _linear_pack, conv_rows
-        with torch.cuda.device(x.device):
+        with _on_device(x):
             xr = x.reshape(-1, x.shape[-1]).contiguous()
             y = conv_rows(xr, _linear_pack(weight.detach(), False), None if bias is None else bias.detach().float().contiguous(),
                           1, 1, 1, xr.shape[0])
@@ -429,7 +504,7 @@ class LinearRows8Fn(torch.autograd.Function):
         weight, *kept = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dw = db = None
-        with torch.cuda.device(dy.device):
+        with _on_device(dy):
             d = dy.to(torch.bfloat16).reshape(-1, dy.shape[-1]).contiguous()
             if need[0]:
                 dx = conv_rows(d, _linear_pack(weight.detach(), True), None, 1, 1, 1, d.shape[0]).view(ctx.shape)
@@ -446,12 +521,14 @@ def linear_rows8(x: torch.Tensor, weight: torch.Tensor, bias=None) -> torch.Tens
     (multiples of 32), whose input is kept for the weight gradient in 8 bits (about half of a bfloat16 copy).  Output and input gradient are exactly
     those of the bfloat16 path; only the weight gradient sees the rounding to 8 bits.  Needs the bfloat16 build."""
     _on_gpu(x, weight, bias)
-    _require(_lib.PRECISION == "bf16", "the training layers exchange bfloat16 rows: VDMI_PRECISION=f16 serves sampling only")
-    _require(x.dtype == torch.bfloat16 and weight.dtype == torch.float32 and weight.dim() == 2,
-             f"x is bfloat16 and weight float32 [cout, cin] (got {x.dtype}, {weight.dtype} {tuple(weight.shape)})")
-    _require(x.shape[-1] == weight.shape[1] and (bias is None or tuple(bias.shape) == (weight.shape[0],)),
-             f"x [..., cin], weight [cout, cin], bias [cout] (got {tuple(x.shape)}, {tuple(weight.shape)})")
-    _require(weight.shape[0] % 32 == 0 and weight.shape[1] % 32 == 0, f"multiples of 32 channels (got {tuple(weight.shape)})")
+    if _lib.PRECISION != "bf16":
+        raise VdmiError("the training layers exchange bfloat16 rows: VDMI_PRECISION=f16 serves sampling only")
+    if not (x.dtype == torch.bfloat16 and weight.dtype == torch.float32 and weight.dim() == 2):
+        raise VdmiError(f"x is bfloat16 and weight float32 [cout, cin] (got {x.dtype}, {weight.dtype} {tuple(weight.shape)})")
+    if x.shape[-1] != weight.shape[1] or (bias is not None and bias.shape != (weight.shape[0],)):
+        raise VdmiError(f"x [..., cin], weight [cout, cin], bias [cout] (got {tuple(x.shape)}, {tuple(weight.shape)})")
+    if weight.shape[0] % 32 or weight.shape[1] % 32:
+        raise VdmiError(f"multiples of 32 channels (got {tuple(weight.shape)})")
     if x.numel() == 0:
         return torch.nn.functional.linear(x, weight.to(x.dtype), None if bias is None else bias.to(x.dtype))
     return LinearRows8Fn.apply(x, weight, bias)

@@ -7,7 +7,7 @@
 // The gradients are the same scan with the operands in other roles:
 //     dq : forward in time over (q, k, v) := (do, v, k), with S^T
 //     dv : backward in time over (k, q, do) with R = dS / m, where R collects lambda^(i+1) q_i do_i^T
-//     dk : backward in time over (v, do, q), with R^T;   the gradient of the first state is m R at the sequence's start
+//     dk : backward in time over (v, do, q), with R^T (one walk with dv);   the gradient of the first state is m R there
 //
 // What bounds it: memory.  A tile of one head takes 2 d (d + 32) products per token and tensor element moved - an order
 // under what the matrix cores do in the time the rows take - so the kernels are built to keep loads in flight: a wave
@@ -47,11 +47,31 @@ struct ScanArgs {
     long long tasks;
 };
 
+struct GradArgs {                       // dk and dv
+    const void* q; const void* k; const void* v; const void* g; void* dk; void* dv;
+    Strides qs, ks, vs, gs, dks, dvs;
+    const float* log_decay;
+    const int* lengths;
+    const float* s_in; float* s_out;    // gradients of the last and of the first state
+    const float* seg;
+    int inner, n, heads, nseg, seg_len;
+    float m;
+    long long tasks;
+};
+
 __device__ __forceinline__ int swap23(int l) { return (l & 0x13) | ((l & 4) << 1) | ((l & 8) >> 1); }
+__device__ __forceinline__ int acc_row(int reg, int half) { return (reg & 3) + 8 * (reg >> 2) + 4 * half; }
 
 // log2 lambda, bounded so that exponents of zero tokens stay zero (lambda^1 has underflowed long before -1e4)
 __device__ __forceinline__ float log2_decay(const float* log_decay, int head) {
     return fmaxf(log_decay[head] * LOG2E, -1e4f);
+}
+
+// p * w where w = 0 marks a pair that does not exist: zero whatever p is (0 * inf and 0 * NaN are 0)
+__device__ __forceinline__ float weigh(float p, float w) {
+    float r;
+    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(p), "v"(w));
+    return r;
 }
 
 // lambda^(..) v as a sum of 16-bit operands: three of bfloat16 (8 bits each), two halfs (11 bits each).
@@ -64,117 +84,211 @@ __device__ __forceinline__ T high_part(float x) { return (T)x; }
 template <>
 __device__ __forceinline__ _Float16 high_part<_Float16>(float x) { return (_Float16)(fabsf(x) < 0x1p-14f ? 0.f : x); }
 
+template <typename T>
+struct Split {
+    x8_t<T> h[2], e[2], f[2];
+    // w: the weights of the 32 tokens, in LDS
+    __device__ __forceinline__ Split(const x8_t<T>& v0, const x8_t<T>& v1, const float* w, int half) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const f32x4 w0 = *reinterpret_cast<const f32x4*>(w + 16 * s + 4 * half), w1 = *reinterpret_cast<const f32x4*>(w + 16 * s + 8 + 4 * half);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = (float)(s ? v1 : v0)[j] * (j < 4 ? w0[j & 3] : w1[j & 3]);
+                h[s][j] = high_part<T>(x);
+                const float y = (x - (float)h[s][j]) * Low<T>::SCALE;
+                e[s][j] = (T)y;
+                if (Low<T>::THREE) f[s][j] = (T)(y - (float)e[s][j]);
+            }
+        }
+    }
+    // S[kt] <- whole S[kt] + (columns 32 kt .. of the image at tr)^T (the split rows)
+    template <int KT>
+    __device__ __forceinline__ void update(f32x16 (&S)[KT], float whole, const char* tr, int pitch) const {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+            const x8_t<T> k0 = tr_operand<T>(tr + 64 * kt, 8 * pitch), k1 = tr_operand<T>(tr + 64 * kt + 16 * pitch, 8 * pitch);
+            f32x16 add = mfma16(k0, e[0], zero16());
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[kt][r] *= whole;
+            S[kt] = mfma16(k0, h[0], S[kt]);
+            add = mfma16(k1, e[1], add);
+            S[kt] = mfma16(k1, h[1], S[kt]);
+            if (Low<T>::THREE) {
+                add = mfma16(k0, f[0], add);
+                S[kt] = mfma16(k1, f[1], S[kt]);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[kt][r] += add[r] * (1.f / Low<T>::SCALE);
+        }
+    }
+};
+
+// Rows of one head, 32 tokens at a time: a buffer resource per tile, based on the tile's first row in memory, and 32-bit
+// lane offsets that stay the same from tile to tile; rows past the tile's last token get an offset past the resource's
+// end, which loads as zero and is not stored.  The tokens run backwards in memory where REVERSE.
+constexpr unsigned NOWHERE = 0x80000000u;
+
+struct Rows {
+    const char* base;
+    long long pitch;            // bytes
+    unsigned records;           // bytes of a tile
+
+    __device__ __forceinline__ Rows(const void* p, const Strides& s, long long bb, long long ii, int head, int col0, int width)
+        : base(static_cast<const char*>(p) + 2 * (bb * s.b + ii * s.i + head * s.h + col0)), pitch(2 * s.n),
+          records((unsigned)(31 * 2 * s.n) + 2 * width) {}
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile(int first) const {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + first * pitch), 0, records, 0x00020000);
+    }
+    // offset of column byte `col` of token `row` of a tile of cnt tokens
+    __device__ __forceinline__ unsigned at(int row, int cnt, bool reverse, int col) const {
+        return row < cnt ? (unsigned)(reverse ? cnt - 1 - row : row) * (unsigned)pitch + col : NOWHERE;
+    }
+};
+
+typedef __attribute__((ext_vector_type(4))) unsigned u4;
+template <typename T>
+__device__ __forceinline__ x8_t<T> load16(__amdgpu_buffer_rsrc_t r, unsigned off) {
+    return __builtin_bit_cast(x8_t<T>, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+}
+template <typename T>
+__device__ __forceinline__ void store16(__amdgpu_buffer_rsrc_t r, unsigned off, const x8_t<T>& v) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), r, off, 0, 0);
+}
+
+// a wave's place: (sequence, head, segment, 32-column slice) and its tokens
+struct Place {
+    int slice, head, seg, len, t_begin, t_stop, t_end;
+    long long seq, bb, ii;
+    template <typename A>
+    __device__ __forceinline__ Place(const A& a, long long w, int slices, int segs) {
+        slice = (int)(w % slices); w /= slices;
+        head = (int)(w % a.heads); w /= a.heads;
+        seg = (int)(w % segs);
+        seq = w / segs;
+        bb = seq / a.inner;
+        ii = seq - bb * a.inner;
+        len = a.n;
+        if (a.lengths) len = min(max(a.lengths[seq], 0), a.n);
+        t_begin = seg * a.seg_len;
+        t_stop = min(a.n, t_begin + a.seg_len);
+        t_end = min(len, t_stop);
+    }
+    // the segment's rows behind the sequence's end become zeros
+    template <typename T>
+    __device__ __forceinline__ void clear(void* o, const Strides& s, int lane) const {
+        x8_t<T> z;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = (T)0.f;
+        T* p = static_cast<T*>(o) + bb * s.b + ii * s.i + head * s.h + 32 * slice + 8 * (lane & 3);
+        for (int t = max(len, t_begin) + (lane >> 2); t < t_stop; t += 16) *reinterpret_cast<x8_t<T>*>(p + t * s.n) = z;
+    }
+};
+
+// transposed reads of a [token][column] image: lane 4 q + p of a 16-lane group supplies row q, four columns; its half's
+// contraction values are rows 4 half + 0..3 and + 8 (accumulator-row order), the column pieces in swapped order (see above)
+__device__ __forceinline__ int tr_offset(int lane, int pitch) {
+    const int g16 = lane >> 4, tq = (lane >> 2) & 3, tp = lane & 3;
+    return (4 * (g16 >> 1) + tq) * pitch + (16 * (g16 & 1) + 4 * (((tp & 1) << 1) | (tp >> 1))) * 2;
+}
+
 template <typename T, int D, bool STATE_ONLY>
 __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a) {
     typedef x8_t<T> x8;
-    constexpr int KS = D / 16, KT = D / 32, KP = 2 * D + 16;
-    constexpr float LOW = Low<T>::SCALE;
-    constexpr bool THREE = Low<T>::THREE;
+    constexpr int KS = D / 16, KT = D / 32, KP = 2 * D + 16, RS = 512 / D;      // RS: rows that 64 16-byte pieces cover
     __shared__ __attribute__((aligned(16))) char kimg_all[DW][32 * KP];
     __shared__ __attribute__((aligned(16))) char vimg_all[DW][32 * VP];
+    __shared__ __attribute__((aligned(16))) float uw_all[DW][32];
     const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     char* kimg = kimg_all[wave];
     char* vimg = vimg_all[wave];
-    long long w = (long long)blockIdx.x * DW + wave;
+    const long long w = (long long)blockIdx.x * DW + wave;
     if (w >= a.tasks) return;
-    const int slice = (int)(w % KT); w /= KT;
-    const int head = (int)(w % a.heads); w /= a.heads;
-    const int nseg_run = STATE_ONLY && !a.s_out ? a.nseg - 1 : a.nseg;      // nobody reads the last segment's sum
-    const int seg = (int)(w % nseg_run);
-    const long long seq = w / nseg_run;
-    const long long bb = seq / a.inner, ii = seq - bb * a.inner;
-    int len = a.n;
-    if (a.lengths) len = min(max(a.lengths[seq], 0), a.n);
-    const int t_begin = seg * a.seg_len, t_stop = min(a.n, t_begin + a.seg_len), t_end = min(len, t_stop);
-    const T* qp = static_cast<const T*>(a.q) + bb * a.qs.b + ii * a.qs.i + head * a.qs.h;
-    const T* kp = static_cast<const T*>(a.k) + bb * a.ks.b + ii * a.ks.i + head * a.ks.h;
-    const T* vp = static_cast<const T*>(a.v) + bb * a.vs.b + ii * a.vs.i + head * a.vs.h + slice * 32;
-    T* op = static_cast<T*>(a.o) + bb * a.os.b + ii * a.os.i + head * a.os.h + slice * 32;
-    x8 zero8;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) zero8[j] = (T)0.f;
+    const Place at(a, w, KT, STATE_ONLY && !a.s_out ? a.nseg - 1 : a.nseg);     // nobody reads the last segment's sum
+    const bool reverse = a.reverse;
+    const Rows qr(a.q, a.qs, at.bb, at.ii, at.head, 0, D), kr(a.k, a.ks, at.bb, at.ii, at.head, 0, D),
+        vr(a.v, a.vs, at.bb, at.ii, at.head, 32 * at.slice, 32), orow(a.o, a.os, at.bb, at.ii, at.head, 32 * at.slice, 32);
+    if (!STATE_ONLY) at.clear<T>(a.o, a.os, lane);
 
-    if (!STATE_ONLY) {                      // rows behind the sequence's end
-        for (int t = max(len, t_begin) + (lane >> 2); t < t_stop; t += 16)
-            *reinterpret_cast<x8*>(op + (long long)t * a.os.n + 8 * (lane & 3)) = zero8;
-    }
-
-    const float l2 = log2_decay(a.log_decay, head);
-    const long long state0 = (seq * a.heads + head) * (long long)(D * D);
+    const float l2 = log2_decay(a.log_decay, at.head);
+    const long long state0 = (at.seq * a.heads + at.head) * (long long)(D * D);
     // this lane's elements of S: row 32 kt + 16 (r >> 3) + 8 half + (r & 7), column 32 slice + swap23(l31)
-    const int s_col = (32 * slice + swap23(l31)) * a.cs;
+    const int s_col = (32 * at.slice + swap23(l31)) * a.cs;
     f32x16 S[KT];
     {
         const float* src = nullptr;
         float mul = 1.f;
         if (!STATE_ONLY) {
-            if (a.nseg > 1) src = a.seg + (state0 * a.nseg + (long long)seg * (D * D));
+            if (a.nseg > 1) src = a.seg + (state0 * a.nseg + (long long)at.seg * (D * D));
             else if (a.s_in) { src = a.s_in + state0; mul = a.s_in_mul; }
         }
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+        for (int kt = 0; kt < KT; ++kt) S[kt] = zero16();
+        if (src) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                S[kt][r] = src ? src[(32 * kt + 16 * (r >> 3) + 8 * half + (r & 7)) * a.rs + s_col] * mul : 0.f;
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) S[kt][r] = src[(32 * kt + 16 * (r >> 3) + 8 * half + (r & 7)) * a.rs + s_col] * mul;
+        }
     }
     // decays: of a pair (register = key, lane = query), of the state towards a query, of a token towards the tile's end
-    float dw[16], uw[16];
+    float dw[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        const int key = (r & 3) + 8 * (r >> 2) + 4 * half;
-        dw[r] = a.m * __builtin_amdgcn_exp2f(l2 * (float)max(l31 - key, 0));
+        const int gap = l31 - acc_row(r, half);
+        dw[r] = gap >= 0 ? a.m * __builtin_amdgcn_exp2f(l2 * (float)gap) : 0.f;
     }
     const float ow = a.m * __builtin_amdgcn_exp2f(l2 * (float)(l31 + a.e_out));
+    float* uw = uw_all[wave];
     auto token_decays = [&](int cnt) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-            uw[r] = __builtin_amdgcn_exp2f(l2 * (float)(max(cnt - 1 - ((r & 3) + 8 * (r >> 2) + 4 * half), 0) + a.e_u));
+        if (half == 0) uw[l31] = __builtin_amdgcn_exp2f(l2 * (float)(max(cnt - 1 - l31, 0) + a.e_u));
     };
     token_decays(32);
     float whole = __builtin_amdgcn_exp2f(l2 * 32.f);
 
-    x8 kreg[KS], vreg[2], qreg[KS];
-    auto row_at = [&](int t) { return (long long)(a.reverse ? len - 1 - t : t); };
-    auto load = [&](int t0) {
+    x8 kreg[KS], vreg[2], q[KS];
+    unsigned kofs[KS], vofs[2], qofs;
+    auto offsets = [&](int cnt) {
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            const int p = lane + 64 * i, t = t0 + p / (D / 8);
-            kreg[i] = t < t_end ? *reinterpret_cast<const x8*>(kp + row_at(t) * a.ks.n + 8 * (p % (D / 8))) : zero8;
-        }
+        for (int i = 0; i < KS; ++i) kofs[i] = kr.at(lane / (D / 8) + RS * i, cnt, reverse, 16 * (lane % (D / 8)));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int t = t0 + 16 * i + (lane >> 2);
-            vreg[i] = t < t_end ? *reinterpret_cast<const x8*>(vp + row_at(t) * a.vs.n + 8 * (lane & 3)) : zero8;
-        }
-        if (!STATE_ONLY) {
-            const int t = t0 + l31;
-            const T* p = qp + row_at(t) * a.qs.n + 8 * half;
-#pragma unroll
-            for (int i = 0; i < KS; ++i) qreg[i] = t < t_end ? *reinterpret_cast<const x8*>(p + 16 * i) : zero8;
-        }
+        for (int i = 0; i < 2; ++i) vofs[i] = vr.at(16 * i + (lane >> 2), cnt, reverse, 16 * (lane & 3));
+        qofs = qr.at(l31, cnt, reverse, 16 * half);
     };
-    // transposed reads: lane 4 q + p of a 16-lane group supplies row q, four columns; its half's contraction values are
-    // rows 4 half + 0..3 and + 8 (accumulator-row order), the column pieces in swapped order (see above)
-    const int g16 = lane >> 4, tq = (lane >> 2) & 3, tp = lane & 3;
-    const int tr_row = 4 * (g16 >> 1) + tq, tr_col = (16 * (g16 & 1) + 4 * (((tp & 1) << 1) | (tp >> 1))) * 2;
-    const char* ktr = kimg + tr_row * KP + tr_col;
-    const char* vtr = vimg + tr_row * VP + tr_col;
-
-    if (t_begin < t_end) load(t_begin);
-    for (int t0 = t_begin; t0 < t_end; t0 += 32) {
-        const int cnt = min(32, t_end - t0);
+    auto first_row = [&](int t0, int cnt) { return reverse ? at.len - t0 - cnt : t0; };
+    auto load_kv = [&](int t0, int cnt) {
+        const auto rk = kr.tile(first_row(t0, cnt)), rv = vr.tile(first_row(t0, cnt));
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            const int p = lane + 64 * i;
-            *reinterpret_cast<x8*>(kimg + (p / (D / 8)) * KP + 16 * (p % (D / 8))) = kreg[i];
-        }
+        for (int i = 0; i < KS; ++i) kreg[i] = load16<T>(rk, kofs[i]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) vreg[i] = load16<T>(rv, vofs[i]);
+    };
+    auto load_q = [&](int t0, int cnt) {
+        const auto rq = qr.tile(first_row(t0, cnt));
+#pragma unroll
+        for (int i = 0; i < KS; ++i) q[i] = load16<T>(rq, qofs + 32 * i);
+    };
+    const char* ktr = kimg + tr_offset(lane, KP);
+    const char* vtr = vimg + tr_offset(lane, VP);
+
+    int cnt = min(32, at.t_end - at.t_begin);
+    if (cnt > 0) {
+        offsets(cnt);
+        load_kv(at.t_begin, cnt);
+        if (!STATE_ONLY) load_q(at.t_begin, cnt);
+    }
+    for (int t0 = at.t_begin; t0 < at.t_end; t0 += 32) {
+        cnt = min(32, at.t_end - t0);
+        const int next = min(32, at.t_end - t0 - 32);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) *reinterpret_cast<x8*>(kimg + (lane / (D / 8) + RS * i) * KP + 16 * (lane % (D / 8))) = kreg[i];
 #pragma unroll
         for (int i = 0; i < 2; ++i) *reinterpret_cast<x8*>(vimg + (16 * i + (lane >> 2)) * VP + 16 * (lane & 3)) = vreg[i];
-        x8 q[KS];
-#pragma unroll
-        for (int i = 0; i < KS; ++i) q[i] = qreg[i];
-        if (t0 + 32 < t_end) load(t0 + 32);
+        if (next > 0) {
+            if (next < 32) offsets(next);
+            load_kv(t0 + 32, next);
+        }
         const x8 v0 = tr_operand<T>(vtr, 8 * VP), v1 = tr_operand<T>(vtr + 16 * VP, 8 * VP);
         if (!STATE_ONLY) {
             f32x16 st = zero16(), o = zero16();
@@ -184,9 +298,10 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
                 st = mfma16(kf, q[ks], st);
                 o = mfma16(acc_operand<T>(S[ks >> 1], ks & 1), q[ks], o);
             }
+            if (next > 0) load_q(t0 + 32, next);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                st[r] = (r & 3) + 8 * (r >> 2) + 4 * half <= l31 ? st[r] * dw[r] : 0.f;
+                st[r] = weigh(st[r], dw[r]);
                 o[r] *= ow;
             }
             o = mfma16(v0, acc_operand<T>(st, 0), o);
@@ -194,59 +309,192 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
             // through LDS (the tile's v image is in registers by now) to 16-byte stores, four lanes on a row's 64 bytes
             *reinterpret_cast<x8*>(vimg + l31 * VP + 16 * half) = acc_operand<T>(o, 0);
             *reinterpret_cast<x8*>(vimg + l31 * VP + 32 + 16 * half) = acc_operand<T>(o, 1);
+            const auto ro = orow.tile(first_row(t0, cnt));
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int row = 16 * i + (lane >> 2);
-                const x8 piece = *reinterpret_cast<const x8*>(vimg + row * VP + 16 * (lane & 3));
-                if (row < cnt) *reinterpret_cast<x8*>(op + row_at(t0 + row) * a.os.n + 8 * (lane & 3)) = piece;
+                store16<T>(ro, orow.at(row, cnt, reverse, 16 * (lane & 3)), *reinterpret_cast<const x8*>(vimg + row * VP + 16 * (lane & 3)));
             }
         }
         if (cnt < 32) {
             token_decays(cnt);
             whole = __builtin_amdgcn_exp2f(l2 * (float)cnt);
         }
-        x8 h0, h1, e0, e1, f0, f1;          // lambda^(..) v as a sum of operands
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float x0 = (float)v0[j] * uw[j], x1 = (float)v1[j] * uw[8 + j];
-            h0[j] = high_part<T>(x0);
-            h1[j] = high_part<T>(x1);
-            const float y0 = (x0 - (float)h0[j]) * LOW, y1 = (x1 - (float)h1[j]) * LOW;
-            e0[j] = (T)y0;
-            e1[j] = (T)y1;
-            if (THREE) {
-                f0[j] = (T)(y0 - (float)e0[j]);
-                f1[j] = (T)(y1 - (float)e1[j]);
-            }
-        }
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            const x8 k0 = tr_operand<T>(ktr + 64 * kt, 8 * KP), k1 = tr_operand<T>(ktr + 64 * kt + 16 * KP, 8 * KP);
-            f32x16 add = mfma16(k0, e0, zero16());
-#pragma unroll
-            for (int r = 0; r < 16; ++r) S[kt][r] *= whole;
-            S[kt] = mfma16(k0, h0, S[kt]);
-            add = mfma16(k1, e1, add);
-            S[kt] = mfma16(k1, h1, S[kt]);
-            if (THREE) {
-                f32x16 last = mfma16(k0, f0, zero16());
-                last = mfma16(k1, f1, last);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) add[r] += last[r];
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) S[kt][r] += add[r] * (1.f / LOW);
-        }
+        const Split<T> sv(v0, v1, uw, half);
+        sv.update(S, whole, ktr, KP);
     }
     float* dst = nullptr;
     float mul = 1.f;
-    if (STATE_ONLY) dst = a.seg + (state0 * a.nseg + (long long)seg * (D * D));
+    if (STATE_ONLY) dst = a.seg + (state0 * a.nseg + (long long)at.seg * (D * D));
     else if (a.s_out && a.nseg == 1) { dst = a.s_out + state0; mul = a.s_out_mul; }
     if (dst) {
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
             for (int r = 0; r < 16; ++r) dst[(32 * kt + 16 * (r >> 3) + 8 * half + (r & 7)) * a.rs + s_col] = S[kt][r] * mul;
+    }
+}
+
+// dk and dv in one walk backward in time: both read q, k, v and do, and what one of them needs of R = dS / m by columns the
+// other needs by rows.  A wave computes 32 columns of dv and the same 32 columns of dk and holds R[all dk][its columns of
+// dv] and R^T[all dv][its columns of dk].
+template <typename T, int D>
+__global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(const GradArgs a) {
+    typedef x8_t<T> x8;
+    constexpr int KS = D / 16, KT = D / 32, KP = 2 * D + 16, RS = 512 / D;
+    __shared__ __attribute__((aligned(16))) char qimg_all[DW][32 * KP];
+    __shared__ __attribute__((aligned(16))) char gimg_all[DW][32 * KP];
+    __shared__ __attribute__((aligned(16))) float uw_all[DW][32];
+    const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    char* qimg = qimg_all[wave];
+    char* gimg = gimg_all[wave];
+    const long long w = (long long)blockIdx.x * DW + wave;
+    if (w >= a.tasks) return;
+    const Place at(a, w, KT, a.nseg);
+    const Rows qr(a.q, a.qs, at.bb, at.ii, at.head, 0, D), kr(a.k, a.ks, at.bb, at.ii, at.head, 0, D),
+        vr(a.v, a.vs, at.bb, at.ii, at.head, 0, D), gr(a.g, a.gs, at.bb, at.ii, at.head, 0, D),
+        dkr(a.dk, a.dks, at.bb, at.ii, at.head, 32 * at.slice, 32), dvr(a.dv, a.dvs, at.bb, at.ii, at.head, 32 * at.slice, 32);
+    at.clear<T>(a.dk, a.dks, lane);
+    at.clear<T>(a.dv, a.dvs, lane);
+
+    const float l2 = log2_decay(a.log_decay, at.head);
+    const long long state0 = (at.seq * a.heads + at.head) * (long long)(D * D);
+    const int col = 32 * at.slice + swap23(l31);
+    f32x16 R[KT], Rt[KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) R[kt] = Rt[kt] = zero16();
+    const float* src = a.nseg > 1 ? a.seg + (state0 * a.nseg + (long long)at.seg * (D * D)) : a.s_in ? a.s_in + state0 : nullptr;
+    if (src) {
+        const float mul = a.nseg > 1 ? 1.f : 1.f / a.m;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = 32 * kt + 16 * (r >> 3) + 8 * half + (r & 7);
+                R[kt][r] = src[row * D + col] * mul;
+                Rt[kt][r] = src[col * D + row] * mul;
+            }
+    }
+    float dw[16];                       // as in the scan; register = query, lane = key, both counted backward in time
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int gap = l31 - acc_row(r, half);
+        dw[r] = gap >= 0 ? a.m * __builtin_amdgcn_exp2f(l2 * (float)gap) : 0.f;
+    }
+    const float ow = a.m * __builtin_amdgcn_exp2f(l2 * (float)l31);
+    float* uw = uw_all[wave];
+    auto token_decays = [&](int cnt) {
+        if (half == 0) uw[l31] = __builtin_amdgcn_exp2f(l2 * (float)(max(cnt - 1 - l31, 0) + 1));
+    };
+    token_decays(32);
+    float whole = __builtin_amdgcn_exp2f(l2 * 32.f);
+
+    x8 qreg[KS], greg[KS], k[KS], v[KS];
+    unsigned qofs[KS], gofs[KS], kofs, vofs;
+    auto offsets = [&](int cnt) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            qofs[i] = qr.at(lane / (D / 8) + RS * i, cnt, true, 16 * (lane % (D / 8)));
+            gofs[i] = gr.at(lane / (D / 8) + RS * i, cnt, true, 16 * (lane % (D / 8)));
+        }
+        kofs = kr.at(l31, cnt, true, 16 * half);
+        vofs = vr.at(l31, cnt, true, 16 * half);
+    };
+    auto load_qg = [&](int t0, int cnt) {
+        const auto rq = qr.tile(at.len - t0 - cnt), rg = gr.tile(at.len - t0 - cnt);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            qreg[i] = load16<T>(rq, qofs[i]);
+            greg[i] = load16<T>(rg, gofs[i]);
+        }
+    };
+    auto load_kv = [&](int t0, int cnt) {
+        const auto rk = kr.tile(at.len - t0 - cnt), rv = vr.tile(at.len - t0 - cnt);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            k[i] = load16<T>(rk, kofs + 32 * i);
+            v[i] = load16<T>(rv, vofs + 32 * i);
+        }
+    };
+    const char* qtr = qimg + tr_offset(lane, KP);
+    const char* gtr = gimg + tr_offset(lane, KP);
+
+    int cnt = min(32, at.t_end - at.t_begin);
+    if (cnt > 0) {
+        offsets(cnt);
+        load_qg(at.t_begin, cnt);
+        load_kv(at.t_begin, cnt);
+    }
+    for (int t0 = at.t_begin; t0 < at.t_end; t0 += 32) {
+        cnt = min(32, at.t_end - t0);
+        const int next = min(32, at.t_end - t0 - 32);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            *reinterpret_cast<x8*>(qimg + (lane / (D / 8) + RS * i) * KP + 16 * (lane % (D / 8))) = qreg[i];
+            *reinterpret_cast<x8*>(gimg + (lane / (D / 8) + RS * i) * KP + 16 * (lane % (D / 8))) = greg[i];
+        }
+        if (next > 0) {
+            if (next < 32) offsets(next);
+            load_qg(t0 + 32, next);
+        }
+        // [query x key]: q k and do v;  [column x key]: R k and R^T v
+        f32x16 p = zero16(), dp = zero16(), ov = zero16(), ok = zero16();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const x8 qf = *reinterpret_cast<const x8*>(qimg + l31 * KP + 32 * ks + 16 * half);
+            const x8 gf = *reinterpret_cast<const x8*>(gimg + l31 * KP + 32 * ks + 16 * half);
+            p = mfma16(qf, k[ks], p);
+            dp = mfma16(gf, v[ks], dp);
+            ov = mfma16(acc_operand<T>(R[ks >> 1], ks & 1), k[ks], ov);
+            ok = mfma16(acc_operand<T>(Rt[ks >> 1], ks & 1), v[ks], ok);
+        }
+        if (next > 0) load_kv(t0 + 32, next);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            p[r] = weigh(p[r], dw[r]);
+            dp[r] = weigh(dp[r], dw[r]);
+            ov[r] *= ow;
+            ok[r] *= ow;
+        }
+        const x8 g0 = tr_operand<T>(gtr + 64 * at.slice, 8 * KP), g1 = tr_operand<T>(gtr + 64 * at.slice + 16 * KP, 8 * KP);
+        const x8 q0 = tr_operand<T>(qtr + 64 * at.slice, 8 * KP), q1 = tr_operand<T>(qtr + 64 * at.slice + 16 * KP, 8 * KP);
+        ov = mfma16(g0, acc_operand<T>(p, 0), ov);
+        ok = mfma16(q0, acc_operand<T>(dp, 0), ok);
+        ov = mfma16(g1, acc_operand<T>(p, 1), ov);
+        ok = mfma16(q1, acc_operand<T>(dp, 1), ok);
+        if (cnt < 32) {
+            token_decays(cnt);
+            whole = __builtin_amdgcn_exp2f(l2 * (float)cnt);
+        }
+        {
+            const Split<T> sg(g0, g1, uw, half);
+            sg.update(R, whole, qtr, KP);
+        }
+        {
+            const Split<T> sq(q0, q1, uw, half);
+            sq.update(Rt, whole, gtr, KP);
+        }
+        // the images are done with: results through them to 16-byte stores, four lanes on a row's 64 bytes
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            *reinterpret_cast<x8*>(qimg + l31 * VP + 32 * s + 16 * half) = acc_operand<T>(ok, s);
+            *reinterpret_cast<x8*>(gimg + l31 * VP + 32 * s + 16 * half) = acc_operand<T>(ov, s);
+        }
+        const auto rk = dkr.tile(at.len - t0 - cnt), rv = dvr.tile(at.len - t0 - cnt);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = 16 * i + (lane >> 2);
+            store16<T>(rk, dkr.at(row, cnt, true, 16 * (lane & 3)), *reinterpret_cast<const x8*>(qimg + row * VP + 16 * (lane & 3)));
+            store16<T>(rv, dvr.at(row, cnt, true, 16 * (lane & 3)), *reinterpret_cast<const x8*>(gimg + row * VP + 16 * (lane & 3)));
+        }
+    }
+    if (a.s_out && a.nseg == 1) {
+        float* dst = a.s_out + state0;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dst[(32 * kt + 16 * (r >> 3) + 8 * half + (r & 7)) * D + col] = R[kt][r] * a.m;
     }
 }
 
@@ -289,96 +537,112 @@ __global__ __launch_bounds__(256) void decay_segments_kernel(const ScanArgs a, i
 
 // ------------------------------------------------------------------------------------------------------------------
 // Sequences of up to 32 tokens without states (the frames of a site): g = 32 / n whole sequences share a tile of 32
-// rows, pairs of different sequences are masked, and the backward pass does all three gradients from one read of q, k,
+// rows, pairs of different sequences weigh nothing, and the backward pass does all three gradients from one read of q, k,
 // v and do (dP^T = V dO^T with lane = query for dq; P = Q K^T and dP = dO V^T with lane = key for dv and dk).  A wave
 // takes (tile, head) units one after the other, always of the same head, the next unit's rows in flight.
-// A row that is not finite must not reach the other sequences of its tile (zero times infinity): such a tile is
-// computed once per sequence with the others' rows as zeros.
+// A row that is not finite must not reach the other sequences of its tile (zero times infinity in the second product):
+// such a tile is computed once per sequence with the others' rows as zeros.
 // ------------------------------------------------------------------------------------------------------------------
+struct Strides32 { unsigned b, i, n; };            // bytes
+
 struct ShortArgs {
     const void* q; const void* k; const void* v; const void* g;        // g: gradient of o
     void* o; void* dq; void* dk; void* dv;
-    Strides qs, ks, vs, gs, os, dqs, dks, dvs;
+    Strides32 qs, ks, vs, gs, os, dqs, dks, dvs;
+    long long qh, kh, vh, gh, oh, dqh, dkh, dvh;                        // head strides, elements
     const float* log_decay;
     const int* lengths;
-    int inner, n, heads, per_tile;
+    int n, heads, per_tile, tiles;
+    unsigned inner, magic;
+    int shift;                          // seq / inner = umulhi(seq, magic) >> shift; shift < 0: inner is 1
     float m;
-    long long nseq, units;
+    unsigned nseq;
 };
 
-template <typename T>
-__device__ __forceinline__ bool not_finite(const x8_t<T>& x) {
-    const uint4 w = __builtin_bit_cast(uint4, x);
-    const unsigned lo = Pack<T>::EXP, hi = lo << 16;
-    bool bad = false;
-    for (unsigned u : {w.x, w.y, w.z, w.w}) bad |= (u & lo) == lo || (u & hi) == hi;
-    return bad;
+template <typename T, int N>
+__device__ __forceinline__ bool finite(const x8_t<T> (&x)[N]) {
+    typedef __attribute__((ext_vector_type(2))) unsigned short us2;
+    us2 top = {0, 0};
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+        const u4 w = __builtin_bit_cast(u4, x[s]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(us2, w[i] & 0x7fff7fffu));
+    }
+    return top[0] < Pack<T>::EXP && top[1] < Pack<T>::EXP;
 }
 
 template <typename T, int D, bool BWD>
-__global__ __launch_bounds__(DW * 64, D == 128 ? 1 : 2) void decay_short_kernel(const ShortArgs a) {
+__global__ __launch_bounds__(DW * 64, D == 128 && BWD ? 1 : D == 32 && !BWD ? 3 : 2) void decay_short_kernel(const ShortArgs a) {
     typedef x8_t<T> x8;
     constexpr int KS = D / 16, DT = D / 32, P = 2 * D + 16, NI = BWD ? 3 : 1;
+    constexpr bool AHEAD = D == 32 || (D == 64 && !BWD);       // the next unit's rows in flight, where registers allow it
     __shared__ __attribute__((aligned(16))) char img_all[DW][NI][32 * P];       // forward: v; backward: k, q, do
-    __shared__ __attribute__((aligned(16))) char out_all[DW][32 * VP];
     const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    char* oimg = out_all[wave];
-    const long long gid = (long long)blockIdx.x * DW + wave, stride = (long long)gridDim.x * DW;   // stride % heads == 0
+    const unsigned gid = blockIdx.x * DW + wave, step = gridDim.x * DW / a.heads;      // gridDim.x is a multiple of the heads
     const int head = (int)(gid % a.heads), n = a.n;
     const int slot = l31 / n, ti = l31 - slot * n;
     const bool in_tile = slot < a.per_tile;
     const float l2 = log2_decay(a.log_decay, head);
-    // decays of (register = key, lane = query) and, for the backward, (register = query, lane = key); zero bits of the
-    // masks: later keys, other sequences
-    float dw[16], dwt[16];
-    unsigned mask = 0, maskt = 0;
+    // weights of (register = key, lane = query) and, for the backward, (register = query, lane = key)
+    float dw[16], dwt[BWD ? 16 : 1];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        const int t = (r & 3) + 8 * (r >> 2) + 4 * half;
+        const int t = acc_row(r, half), gap = l31 - t;
         const bool same = in_tile && t / n == slot;
-        if (same && t <= l31) mask |= 1u << r;
-        if (same && t >= l31) maskt |= 1u << r;
-        dw[r] = a.m * __builtin_amdgcn_exp2f(l2 * (float)max(l31 - t, 0));
-        dwt[r] = a.m * __builtin_amdgcn_exp2f(l2 * (float)max(t - l31, 0));
+        const float d = a.m * __builtin_amdgcn_exp2f(l2 * fabsf((float)gap));
+        dw[r] = same && gap >= 0 ? d : 0.f;
+        if constexpr (BWD) dwt[r] = same && gap <= 0 ? d : 0.f;
     }
     x8 zero8;
 #pragma unroll
     for (int j = 0; j < 8; ++j) zero8[j] = (T)0.f;
-    const int g16 = lane >> 4, tq = (lane >> 2) & 3, tp = lane & 3;
-    const int tr_off = (4 * (g16 >> 1) + tq) * P + (16 * (g16 & 1) + 4 * (((tp & 1) << 1) | (tp >> 1))) * 2;
+    const int tr_off = tr_offset(lane, P);
 
-    // the sequence of a unit's row, as (outer, inner) batch indexes
-    auto seq_of = [&](long long u, int sl, long long& bb, long long& ii) {
-        const long long seq = (u / a.heads) * a.per_tile + sl;
-        if (sl >= a.per_tile || seq >= a.nseq) return false;
-        bb = seq / a.inner;
-        ii = seq - bb * a.inner;
-        return true;
+    struct Unit {
+        x8 q[KS], k[KS], v[KS], g[BWD ? KS : 1];
+        unsigned bb, ii;
+        bool ok;                        // this lane's row is one of the call's
     };
-    struct Unit { x8 q[KS], k[KS], v[KS], g[BWD ? KS : 1]; };
-    auto fetch = [&](long long u, Unit& x) {
-        long long bb = 0, ii = 0;
-        bool ok = u < a.units && seq_of(u, slot, bb, ii);
-        if (ok && a.lengths) ok = ti < a.lengths[bb * a.inner + ii];
-        const T* qp = static_cast<const T*>(a.q) + bb * a.qs.b + ii * a.qs.i + ti * a.qs.n + head * a.qs.h + 8 * half;
-        const T* kp = static_cast<const T*>(a.k) + bb * a.ks.b + ii * a.ks.i + ti * a.ks.n + head * a.ks.h + 8 * half;
-        const T* vp = static_cast<const T*>(a.v) + bb * a.vs.b + ii * a.vs.i + ti * a.vs.n + head * a.vs.h + 8 * half;
-        const T* gp = static_cast<const T*>(a.g) + bb * a.gs.b + ii * a.gs.i + ti * a.gs.n + head * a.gs.h + 8 * half;
+    auto rows_of = [&](const void* p, const Strides32& s, long long h, const Unit& x) {
+        return reinterpret_cast<const x8*>(static_cast<const char*>(p) + 2 * head * h + (unsigned long long)x.bb * s.b +
+                                           (unsigned long long)x.ii * s.i + (unsigned long long)((unsigned)ti * s.n + 16 * half));
+    };
+    auto fetch = [&](unsigned tile, Unit& x) {
+        unsigned seq = tile * (unsigned)a.per_tile + (unsigned)min(slot, a.per_tile - 1);
+        x.ok = in_tile && tile < (unsigned)a.tiles && seq < a.nseq;
+        seq = min(seq, a.nseq - 1);     // lanes without a row load one that is there; nothing of it is stored
+        x.bb = a.shift < 0 ? seq : __umulhi(seq, a.magic) >> a.shift;
+        x.ii = seq - x.bb * a.inner;
+        const x8* qp = rows_of(a.q, a.qs, a.qh, x);
+        const x8* kp = rows_of(a.k, a.ks, a.kh, x);
+        const x8* vp = rows_of(a.v, a.vs, a.vh, x);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            x.q[s] = ok ? *reinterpret_cast<const x8*>(qp + 16 * s) : zero8;
-            x.k[s] = ok ? *reinterpret_cast<const x8*>(kp + 16 * s) : zero8;
-            x.v[s] = ok ? *reinterpret_cast<const x8*>(vp + 16 * s) : zero8;
-            if constexpr (BWD) x.g[s] = ok ? *reinterpret_cast<const x8*>(gp + 16 * s) : zero8;
+            x.q[s] = qp[2 * s];
+            x.k[s] = kp[2 * s];
+            x.v[s] = vp[2 * s];
+        }
+        if constexpr (BWD) {
+            const x8* gp = rows_of(a.g, a.gs, a.gh, x);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) x.g[s] = gp[2 * s];
+        }
+        if (a.lengths && ti >= a.lengths[seq]) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                x.q[s] = x.k[s] = x.v[s] = zero8;
+                if constexpr (BWD) x.g[s] = zero8;
+            }
         }
     };
     auto to_image = [&](char* im, const x8 (&x)[KS]) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) *reinterpret_cast<x8*>(im + l31 * P + 32 * s + 16 * half) = x[s];
     };
-    // [features x features] contraction of two row sets, in two accumulators (no chain of dependent products)
-    auto pairs = [&](const x8 (&x)[KS], const x8 (&y)[KS]) {
+    // contraction over the features of two row sets, weighed (two accumulators: no chain of dependent products)
+    auto pairs = [&](const x8 (&x)[KS], const x8 (&y)[KS], const float (&d)[16]) {
         f32x16 p = zero16(), p2 = zero16();
 #pragma unroll
         for (int s = 0; s < KS; s += 2) {
@@ -386,78 +650,67 @@ __global__ __launch_bounds__(DW * 64, D == 128 ? 1 : 2) void decay_short_kernel(
             p2 = mfma16(x[s + 1], y[s + 1], p2);
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] += p2[r];
+        for (int r = 0; r < 16; ++r) p[r] = weigh(p[r] + p2[r], d[r]);
         return p;
     };
-    auto weigh = [&](f32x16& p, const float (&d)[16], unsigned m) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] = ((m >> r) & 1u) ? p[r] * d[r] : 0.f;
-    };
-    // rows of 32 tokens x D: (transposed image)^T x pairs, stored for the sequences [s_lo, s_hi) of the tile
-    auto product = [&](const char* im, const f32x16& p, void* dst, const Strides& ds, long long u, int s_lo, int s_hi) {
+    // (an image)^T x pairs: this lane's row, 16 bytes at features 8 half .. and 16 + 8 half .. of every 32
+    auto product = [&](const char* im, const f32x16& p, void* dst, const Strides32& s, long long h, const Unit& x, bool mine) {
         const x8 p0 = acc_operand<T>(p, 0), p1 = acc_operand<T>(p, 1);
+        x8* row = const_cast<x8*>(rows_of(dst, s, h, x));
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             f32x16 o = mfma16(tr_operand<T>(im + tr_off + 64 * dt, 8 * P), p0, zero16());
             o = mfma16(tr_operand<T>(im + tr_off + 64 * dt + 16 * P, 8 * P), p1, o);
-            *reinterpret_cast<x8*>(oimg + l31 * VP + 16 * half) = acc_operand<T>(o, 0);
-            *reinterpret_cast<x8*>(oimg + l31 * VP + 32 + 16 * half) = acc_operand<T>(o, 1);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int row = 16 * i + (lane >> 2), sl = row / n;
-                const x8 piece = *reinterpret_cast<const x8*>(oimg + row * VP + 16 * (lane & 3));
-                long long bb, ii;
-                if (sl >= s_lo && sl < s_hi && seq_of(u, sl, bb, ii))
-                    *reinterpret_cast<x8*>(static_cast<T*>(dst) + bb * ds.b + ii * ds.i + (row - sl * n) * ds.n + head * ds.h +
-                                           32 * dt + 8 * (lane & 3)) = piece;
+            if (mine) {
+                row[4 * dt] = acc_operand<T>(o, 0);
+                row[4 * dt + 2] = acc_operand<T>(o, 1);
             }
+        }
+    };
+    auto compute = [&](const Unit& x, bool mine) {
+        char (*im)[32 * P] = img_all[wave];
+        if constexpr (!BWD) {
+            to_image(im[0], x.v);
+            product(im[0], pairs(x.k, x.q, dw), a.o, a.os, a.oh, x, mine);
+        } else {
+            to_image(im[0], x.k);
+            to_image(im[1], x.q);
+            to_image(im[2], x.g);
+            product(im[0], pairs(x.v, x.g, dw), a.dq, a.dqs, a.dqh, x, mine);          // [key x query]
+            product(im[2], pairs(x.q, x.k, dwt), a.dv, a.dvs, a.dvh, x, mine);         // [query x key]
+            product(im[1], pairs(x.g, x.v, dwt), a.dk, a.dks, a.dkh, x, mine);
         }
     };
 
     Unit nx;
-    fetch(gid, nx);
-    for (long long u = gid; u < a.units; u += stride) {
-        const Unit c = nx;
-        fetch(u + stride, nx);
-        bool bad = false;
-        if (a.per_tile > 1) {
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                bad |= not_finite<T>(c.v[s]);
-                if constexpr (BWD) bad |= not_finite<T>(c.k[s]) || not_finite<T>(c.q[s]) || not_finite<T>(c.g[s]);
-            }
+    const unsigned tile0 = gid / a.heads;
+    if (AHEAD && tile0 < (unsigned)a.tiles) fetch(tile0, nx);
+    for (unsigned tile = tile0; tile < (unsigned)a.tiles; tile += step) {
+        Unit c;
+        if constexpr (AHEAD) {
+            c = nx;
+            if (tile + step < (unsigned)a.tiles) fetch(tile + step, nx);
+        } else {
+            fetch(tile, c);
         }
-        const bool apart = __builtin_amdgcn_ballot_w64(bad) != 0;
-        const int passes = apart ? a.per_tile : 1;
-        for (int pass = 0; pass < passes; ++pass) {
-            const int s_lo = apart ? pass : 0, s_hi = apart ? pass + 1 : a.per_tile;
-            const bool on = !apart || slot == pass;
-            Unit x;
+        bool fine = true;
+        if (a.per_tile > 1) {
+            fine = finite<T>(c.v);
+            if constexpr (BWD) fine = fine && finite<T>(c.k) && finite<T>(c.q) && finite<T>(c.g);
+        }
+        if (__builtin_amdgcn_ballot_w64(!fine) == 0) {
+            compute(c, c.ok);
+        } else {
+            for (int pass = 0; pass < a.per_tile; ++pass) {
+                Unit x = c;
+                if (slot != pass) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                x.q[s] = on ? c.q[s] : zero8;
-                x.k[s] = on ? c.k[s] : zero8;
-                x.v[s] = on ? c.v[s] : zero8;
-                if constexpr (BWD) x.g[s] = on ? c.g[s] : zero8;
-            }
-            if constexpr (!BWD) {
-                to_image(img_all[wave][0], x.v);
-                f32x16 st = pairs(x.k, x.q);
-                weigh(st, dw, mask);
-                product(img_all[wave][0], st, a.o, a.os, u, s_lo, s_hi);
-            } else {
-                to_image(img_all[wave][0], x.k);
-                to_image(img_all[wave][1], x.q);
-                to_image(img_all[wave][2], x.g);
-                f32x16 p = pairs(x.v, x.g);                 // [key x query]
-                weigh(p, dw, mask);
-                product(img_all[wave][0], p, a.dq, a.dqs, u, s_lo, s_hi);
-                p = pairs(x.q, x.k);                        // [query x key]
-                weigh(p, dwt, maskt);
-                product(img_all[wave][2], p, a.dv, a.dvs, u, s_lo, s_hi);
-                p = pairs(x.g, x.v);
-                weigh(p, dwt, maskt);
-                product(img_all[wave][1], p, a.dk, a.dks, u, s_lo, s_hi);
+                    for (int s = 0; s < KS; ++s) {
+                        x.q[s] = x.k[s] = x.v[s] = zero8;
+                        if constexpr (BWD) x.g[s] = zero8;
+                    }
+                }
+                compute(x, c.ok && slot == pass);
             }
         }
     }
@@ -530,6 +783,12 @@ bool rows_ok(const vdmi_rows4& r) {
     return r.p && aligned16(r.p) && r.b % 8 == 0 && r.i % 8 == 0 && r.n % 8 == 0 && r.h % 8 == 0;
 }
 
+// the 32 rows of a tile within a 31-bit offset of each other
+bool pitch_ok(const vdmi_rows4& r) { return r.n >= 0 && r.n <= VDMI_DECAY_MAX_PITCH; }
+
+// the short-sequence kernel multiplies batch indexes with 32-bit byte strides
+bool strides32_ok(const vdmi_rows4& r) { return r.b >= 0 && r.i >= 0 && r.b < 0x7fffffffLL && r.i < 0x7fffffffLL; }
+
 int check_args(const vdmi_decay_args* a) {
     if (!a || !a->log_decay) return VDMI_E_ARG;
     if (a->dtype != VDMI_DT_BF16 && a->dtype != VDMI_DT_F16) return VDMI_E_ARG;
@@ -539,6 +798,7 @@ int check_args(const vdmi_decay_args* a) {
     if ((long long)a->b * a->inner > 0x7fffffffLL / a->heads || a->n > (1 << 30)) return VDMI_E_SHAPE;
     if (!a->q.p || !a->k.p || !a->v.p) return VDMI_E_ARG;
     if (!rows_ok(a->q) || !rows_ok(a->k) || !rows_ok(a->v)) return VDMI_E_ALIGN;
+    if (!pitch_ok(a->q) || !pitch_ok(a->k) || !pitch_ok(a->v)) return VDMI_E_SHAPE;
     return VDMI_OK;
 }
 
@@ -549,6 +809,7 @@ Plan plan(const vdmi_decay_args* a, bool states) {
     Plan p;
     p.nseq = (long long)a->b * a->inner;
     p.is_short = a->n <= 32 && !states;
+    for (const vdmi_rows4* r : {&a->q, &a->k, &a->v, &a->o, &a->dout, &a->dq, &a->dk, &a->dv}) p.is_short = p.is_short && strides32_ok(*r);
     p.nseg = 1;
     p.seg_len = a->n;
     p.bytes = 0;
@@ -617,19 +878,33 @@ ScanArgs scan_args(const vdmi_decay_args* a, const Plan& p) {
     return s;
 }
 
+Strides32 strides32(const vdmi_rows4& r) { return Strides32{(unsigned)(2 * r.b), (unsigned)(2 * r.i), (unsigned)(2 * r.n)}; }
+
 int launch_short(const vdmi_decay_args* a, const Plan& p, bool bwd, hipStream_t st) {
     ShortArgs s = {};
     s.q = a->q.p; s.k = a->k.p; s.v = a->v.p; s.g = a->dout.p;
     s.o = a->o.p; s.dq = a->dq.p; s.dk = a->dk.p; s.dv = a->dv.p;
-    s.qs = strides_of(a->q); s.ks = strides_of(a->k); s.vs = strides_of(a->v); s.gs = strides_of(a->dout);
-    s.os = strides_of(a->o); s.dqs = strides_of(a->dq); s.dks = strides_of(a->dk); s.dvs = strides_of(a->dv);
+    s.qs = strides32(a->q); s.ks = strides32(a->k); s.vs = strides32(a->v); s.gs = strides32(a->dout);
+    s.os = strides32(a->o); s.dqs = strides32(a->dq); s.dks = strides32(a->dk); s.dvs = strides32(a->dv);
+    s.qh = a->q.h; s.kh = a->k.h; s.vh = a->v.h; s.gh = a->dout.h;
+    s.oh = a->o.h; s.dqh = a->dq.h; s.dkh = a->dk.h; s.dvh = a->dv.h;
     s.log_decay = a->log_decay; s.lengths = a->lengths;
-    s.inner = a->inner; s.n = a->n; s.heads = a->heads; s.per_tile = 32 / a->n;
+    s.n = a->n; s.heads = a->heads; s.per_tile = 32 / a->n;
     s.m = a->scale;
-    s.nseq = p.nseq;
-    s.units = (p.nseq + s.per_tile - 1) / s.per_tile * a->heads;
+    s.nseq = (unsigned)p.nseq;
+    s.tiles = (int)((p.nseq + s.per_tile - 1) / s.per_tile);
+    // division by inner of numbers below 2^31: with 2^(l-1) < inner <= 2^l and magic = floor(2^(31+l) / inner) + 1 the
+    // error of the quotient stays under 1 / inner
+    s.inner = (unsigned)a->inner;
+    s.shift = -1;
+    if (a->inner > 1) {
+        int l = 0;
+        while ((1LL << l) < a->inner) ++l;
+        s.magic = (unsigned)((1ULL << (31 + l)) / (unsigned)a->inner + 1);
+        s.shift = l - 1;
+    }
     // a wave keeps its head: the number of waves is a multiple of the heads
-    long long wgs = (s.units + DW - 1) / DW;
+    long long wgs = ((long long)s.tiles * a->heads + DW - 1) / DW;
     if (wgs > 2048) wgs = 2048;
     wgs = (wgs + a->heads - 1) / a->heads * a->heads;
     const dim3 grid((unsigned)wgs), block(DW * 64);
@@ -639,6 +914,29 @@ int launch_short(const vdmi_decay_args* a, const Plan& p, bool bwd, hipStream_t 
     if (a->dtype == VDMI_DT_BF16) SHORT_D(__bf16); else SHORT_D(_Float16);
 #undef SHORT_D
 #undef SHORT
+    VDMI_LAUNCH_CHECK();
+    return VDMI_OK;
+}
+
+int launch_grad(const vdmi_decay_args* a, const Plan& p, hipStream_t st) {
+    GradArgs g = {};
+    g.q = a->q.p; g.k = a->k.p; g.v = a->v.p; g.g = a->dout.p; g.dk = a->dk.p; g.dv = a->dv.p;
+    g.qs = strides_of(a->q); g.ks = strides_of(a->k); g.vs = strides_of(a->v); g.gs = strides_of(a->dout);
+    g.dks = strides_of(a->dk); g.dvs = strides_of(a->dv);
+    g.log_decay = a->log_decay; g.lengths = a->lengths;
+    g.s_in = a->dstate_in; g.s_out = a->dstate_out;
+    g.seg = static_cast<const float*>(a->workspace);
+    g.inner = a->inner; g.n = a->n; g.heads = a->heads; g.nseg = p.nseg; g.seg_len = p.seg_len;
+    g.m = a->scale;
+    g.tasks = p.nseq * a->heads * p.nseg * (a->d / 32);
+    const long long wgs = (g.tasks + DW - 1) / DW;
+    if (wgs > 0x7fffffffLL) return VDMI_E_SHAPE;
+    const dim3 grid((unsigned)wgs), block(DW * 64);
+#define GRAD_D(T) do { if (a->d == 32) hipLaunchKernelGGL((decay_grad_kernel<T, 32>), grid, block, 0, st, g); \
+                       else if (a->d == 64) hipLaunchKernelGGL((decay_grad_kernel<T, 64>), grid, block, 0, st, g); \
+                       else hipLaunchKernelGGL((decay_grad_kernel<T, 128>), grid, block, 0, st, g); } while (0)
+    if (a->dtype == VDMI_DT_BF16) GRAD_D(__bf16); else GRAD_D(_Float16);
+#undef GRAD_D
     VDMI_LAUNCH_CHECK();
     return VDMI_OK;
 }
@@ -655,6 +953,7 @@ extern "C" int vdmi_decay_attn_fwd(const vdmi_decay_args* a, vdmi_stream stream)
     if (ok != VDMI_OK) return ok;
     if (!a->o.p) return VDMI_E_ARG;
     if (!rows_ok(a->o)) return VDMI_E_ALIGN;
+    if (!pitch_ok(a->o)) return VDMI_E_SHAPE;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const Plan p = plan(a, wants_states(a));
     if (p.is_short) return launch_short(a, p, false, st);
@@ -673,37 +972,34 @@ extern "C" int vdmi_decay_attn_bwd(const vdmi_decay_args* a, vdmi_stream stream)
     if (ok != VDMI_OK) return ok;
     if (!a->dout.p || !a->dq.p || !a->dk.p || !a->dv.p) return VDMI_E_ARG;
     if (!rows_ok(a->dout) || !rows_ok(a->dq) || !rows_ok(a->dk) || !rows_ok(a->dv)) return VDMI_E_ALIGN;
+    if (!pitch_ok(a->dout) || !pitch_ok(a->dq) || !pitch_ok(a->dk) || !pitch_ok(a->dv)) return VDMI_E_SHAPE;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const Plan p = plan(a, wants_states(a));
     if (p.is_short) return launch_short(a, p, true, st);
-    if (p.bytes && (!a->workspace || a->workspace_bytes < (int64_t)p.bytes)) return VDMI_E_ARG;
-    int r;
-    // dq: forward in time, S^T
+    if (p.bytes && (!a->workspace || a->workspace_bytes < (int64_t)p.bytes || !a->fwd_workspace)) return VDMI_E_ARG;
+    // dq: forward in time over (do, v, k) with S^T; the states at the segments' starts are the forward's
     ScanArgs s = scan_args(a, p);
+    s.seg = const_cast<float*>(static_cast<const float*>(a->fwd_workspace));
     s.s_in = a->state_in;
     s.e_out = 1;
-    role(s, a->q, a->k, a->v, a->dq);
-    if ((r = segment_states(s, a, p, st)) != VDMI_OK) return r;
+    s.rs = 1;
+    s.cs = a->d;
     role(s, a->dout, a->v, a->k, a->dq);
-    s.rs = 1;
-    s.cs = a->d;
-    if ((r = launch_scan<false>(s, a, p, st)) != VDMI_OK) return r;
+    int r = launch_scan<false>(s, a, p, st);
+    if (r != VDMI_OK) return r;
     // dv and dk: backward in time; R = dS / m collects lambda^(i+1) q_i do_i^T
-    s = scan_args(a, p);
-    s.reverse = 1;
-    s.e_u = 1;
-    s.s_in = a->dstate_in;
-    s.s_in_mul = 1.f / a->scale;
-    s.s_out = a->dstate_out;
-    s.s_out_mul = a->scale;
-    role(s, a->k, a->q, a->dout, a->dv);
-    if ((r = segment_states(s, a, p, st)) != VDMI_OK) return r;
-    if ((r = launch_scan<false>(s, a, p, st)) != VDMI_OK) return r;
-    s.s_out = nullptr;
-    role(s, a->v, a->dout, a->q, a->dk);
-    s.rs = 1;
-    s.cs = a->d;
-    return launch_scan<false>(s, a, p, st);
+    if (p.nseg > 1) {
+        s = scan_args(a, p);
+        s.reverse = 1;
+        s.e_u = 1;
+        s.s_in = a->dstate_in;
+        s.s_in_mul = 1.f / a->scale;
+        s.s_out = a->dstate_out;
+        s.s_out_mul = a->scale;
+        role(s, a->k, a->q, a->dout, a->dv);
+        if ((r = segment_states(s, a, p, st)) != VDMI_OK) return r;
+    }
+    return launch_grad(a, p, st);
 }
 
 extern "C" int vdmi_decay_attn_step(const void* q, const void* k, const void* v, void* o, const int64_t* strides,
