@@ -745,9 +745,10 @@ int vdmi_block_norm_bwd(const vdmi_block_norm_args* a, vdmi_stream stream);
  * [rows][ceil(c / 32)] (e + 127): x ~ code 2^e, e per row and 32 consecutive channels the least exponent whose 448 2^e holds
  * the group's largest finite magnitude, in -118 .. 119 (magnitudes beyond 448 2^119 become that); rounded to nearest even; infinities and NaN become NaN.
  * vdmi_rows8_wgrad: weight gradient of a Linear whose input was kept, dw float [cout][cin] = sum_r dy[r][o] x[r][i], from
- * the codes and bf16 rows dy [rows][cout] (pitch lddy), and db float [cout] = sum_r dy[r][o] (NULL: not wanted); cin, cout
+ * the codes and bf16 rows dy [rows][cout] (pitch lddy, at most VDMI_ROWS8_MAX_PITCH), and db float [cout] = sum_r dy[r][o] (NULL: not wanted); cin, cout
  * multiples of 8; workspace as stated by vdmi_rows8_wgrad_workspace_bytes().
  * ------------------------------------------------------------------------------------------ */
+#define VDMI_ROWS8_MAX_PITCH (1LL << 23)
 int vdmi_rows8_pack(const void* x, int64_t ldx, void* codes, void* exps, int dtype, int64_t rows, int c, vdmi_stream stream);
 int vdmi_rows8_unpack(const void* codes, const void* exps, void* x, int64_t ldx, int dtype, int64_t rows, int c, vdmi_stream stream);
 size_t vdmi_rows8_wgrad_workspace_bytes(int cin, int cout, int64_t rows);                  /* HOST */

@@ -102,6 +102,7 @@ class DecayArgs(C.Structure):
 
 
 DECAY_MAX_PITCH = 1 << 25
+ROWS8_MAX_PITCH = 1 << 23
 
 NORM_KINDS = {None: -1, "rms": 0, "layer": 1}           # enum vdmi_norm_kind
 

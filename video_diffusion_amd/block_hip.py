@@ -432,7 +432,7 @@ class Rows8:
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     """_rows2 of t's values, at 16-byte aligned rows."""
     r = _rows2(t.detach())
-    return r.clone(memory_format=torch.contiguous_format) if r.data_ptr() & 15 or _pitch(r) % 8 else r
+    return r.clone(memory_format=torch.contiguous_format) if r.data_ptr() & 15 or _pitch(r) % 8 or _pitch(r) > _lib.ROWS8_MAX_PITCH else r
 
 
 def pack_rows8(x: torch.Tensor) -> Rows8:

@@ -127,6 +127,32 @@ __device__ __forceinline__ void store_row(const float (&v)[P * 8], void* base, l
     }
 }
 
+// the lane's columns of a parameter row (any element alignment), `absent` where there is none
+template <bool VEC, int L, int P>
+__device__ __forceinline__ void load_params(float (&v)[P * 8], const float* src, float absent, int c, int l) {
+    typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+    for (int i = 0; i < P * 8; ++i) v[i] = absent;
+    if (!src) return;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        if constexpr (VEC) {
+            const int col = column<true, L>(p, 0, l);
+            if (col < c) {
+                const f4u x = *reinterpret_cast<const f4u*>(src + col), y = *reinterpret_cast<const f4u*>(src + col + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { v[8 * p + e] = x[e]; v[8 * p + 4 + e] = y[e]; }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int col = column<false, L>(p, e, l);
+                if (col < c) v[8 * p + e] = src[col];
+            }
+        }
+    }
+}
+
 // v -> its norm in place; returns the factor
 template <bool VEC, int L, int P>
 __device__ __forceinline__ float normalise(float (&v)[P * 8], RowSum<L>& sum, int kind, int c, float inv_c, float eps, int l) {
@@ -177,18 +203,21 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const NormArgs a) {
     const float inv_c = 1.f / (float)c;
     // per column: a = weight (1 + scale), gate * post_weight, shift
     float wa[N], pg[N], sh[BWD ? 1 : N];
+    load_params<VEC, L, P>(wa, a.w, 1.f, c, l);
+    load_params<VEC, L, P>(pg, a.pw, 1.f, c, l);
+    if (a.scale) {
+        float t[N];
+        load_params<VEC, L, P>(t, a.scale + sample * a.scale_bs, 0.f, c, l);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int col = column<VEC, L>(i >> 3, i & 7, l);
-        const bool on = col < c;
-        float v = a.w && on ? a.w[col] : 1.f;
-        if (a.scale && on) v *= 1.f + a.scale[sample * a.scale_bs + col];
-        wa[i] = v;
-        v = a.pw && on ? a.pw[col] : 1.f;
-        if (a.gate && on) v *= a.gate[sample * a.gate_bs + col];
-        pg[i] = v;
-        if constexpr (!BWD) sh[i] = a.shift && on ? a.shift[sample * a.shift_bs + col] : 0.f;
+        for (int i = 0; i < N; ++i) wa[i] *= 1.f + t[i];
     }
+    if (a.gate) {
+        float t[N];
+        load_params<VEC, L, P>(t, a.gate + sample * a.gate_bs, 0.f, c, l);
+#pragma unroll
+        for (int i = 0; i < N; ++i) pg[i] *= t[i];
+    }
+    if constexpr (!BWD) load_params<VEC, L, P>(sh, a.shift ? a.shift + sample * a.shift_bs : nullptr, 0.f, c, l);
     float s1[BWD ? N : 1], s2[BWD ? N : 1], s3[BWD ? N : 1];
     if constexpr (BWD) {
 #pragma unroll
@@ -364,11 +393,11 @@ __global__ __launch_bounds__(1024) void norm_sample_sums_kernel(const SumArgs a)
     if (a.dgate && !a.gate_bs) a.dgate[col] = (a.pw ? a.pw[col] : 1.f) * u[2];
 }
 
-// Lanes and pieces of a row.  Up to 512 columns (1024 backward) a wave or less holds a row; wider rows spread over the
-// workgroup once a lane would hold more than 16 (forward: 32) columns of every operand.
+// Lanes and pieces of a row: a wave or less holds up to 1024 columns, 16 per lane; wider rows spread over the workgroup
+// (3711 float32 rows of 2048 columns forward: 29 us, 4.2 TB/s; with a wave per row and 32 columns per lane 95 us).
 struct Shape { bool vec; int lanes, pieces; };
 
-Shape shape_of(const vdmi_block_norm_args* a, bool bwd) {
+Shape shape_of(const vdmi_block_norm_args* a) {
     const int g = (a->c + 7) / 8;
     Shape s;
     const int64_t pitches[8] = {a->ldx, a->h ? a->ldh : 0, a->out ? a->ldo : 0, a->y ? a->ldy : 0, a->dout ? a->lddo : 0,
@@ -379,7 +408,7 @@ Shape shape_of(const vdmi_block_norm_args* a, bool bwd) {
     if (s.vec && g <= 8) s.lanes = 8;
     else if (s.vec && g <= 16) s.lanes = 16;
     else if (s.vec && g <= 32) s.lanes = 32;
-    else if (g <= (s.vec ? (bwd ? 128 : 256) : 64)) s.lanes = 64;
+    else if (g <= (s.vec ? 128 : 64)) s.lanes = 64;
     else s.lanes = 256;
     s.pieces = (g + s.lanes - 1) / s.lanes;
     if (s.pieces == 3) s.pieces = 4;
@@ -393,10 +422,11 @@ NormPlan norm_plan(const vdmi_block_norm_args* a, bool bwd) {
     const bool per_sample = (a->gate && a->gate_stride) || (a->scale && a->scale_stride) || (a->shift && a->shift_stride);
     p.samples = per_sample ? a->rows / a->rows_per_sample : 1;
     p.rps = per_sample ? a->rows_per_sample : a->rows;
-    const Shape s = shape_of(a, bwd);
+    const Shape s = shape_of(a);
     const long long at_once = 256 / s.lanes;
     // about four workgroups per CU backward (each writes its column sums), eight forward
     long long per = (p.samples * p.rps + (bwd ? 1024 : 2048) - 1) / (bwd ? 1024 : 2048);
+    if (bwd && s.lanes == 256 && per < 8) per = 8;      // a workgroup writes 12 c bytes of sums: not for fewer rows
     per = (per + at_once - 1) / at_once * at_once;
     const long long most = (p.rps + at_once - 1) / at_once * at_once;
     if (per > most) per = most;
@@ -448,9 +478,6 @@ int launch_norm(const NormArgs& n, const Shape& s, unsigned grid, hipStream_t st
             case 32 * 8 + 1: NORM(true, 32, 1); break;
             case 64 * 8 + 1: NORM(true, 64, 1); break;
             case 64 * 8 + 2: NORM(true, 64, 2); break;
-            case 64 * 8 + 4:
-                if constexpr (!BWD) { NORM(true, 64, 4); break; }
-                return VDMI_E_SHAPE;
             case 256 * 8 + 1: NORM(true, 256, 1); break;
             case 256 * 8 + 2: NORM(true, 256, 2); break;
             case 256 * 8 + 4: NORM(true, 256, 4); break;
@@ -485,7 +512,7 @@ template <bool BWD>
 int run_norm(const vdmi_block_norm_args* a, const NormArgs& n, const NormPlan& p, hipStream_t st) {
     const long long grid = p.samples * p.parts;
     if (grid > 0x7fffffffLL) return VDMI_E_SHAPE;
-    const Shape s = shape_of(a, BWD);
+    const Shape s = shape_of(a);
     if (a->dtype == VDMI_DT_BF16) return launch_norm<__bf16, BWD>(n, s, (unsigned)grid, st);
     if (a->dtype == VDMI_DT_F16) return launch_norm<_Float16, BWD>(n, s, (unsigned)grid, st);
     return launch_norm<float, BWD>(n, s, (unsigned)grid, st);

@@ -41,10 +41,10 @@ struct ScanArgs {
     const float* s_in; float* s_out;    // [seq][head][d][d] or null
     float s_in_mul, s_out_mul;
     float* seg;                         // [seq][head][nseg][d][d]: a segment's own sum, then the state at its start
-    int rs, cs;                         // strides of (row, column) of S in those three
+    int rs;                             // the stride of S's rows in s_in and seg: d, or 1 where S is read transposed
     int inner, n, heads, nseg, seg_len, reverse, e_out, e_u;
     float m;
-    long long tasks;
+    unsigned tasks;
 };
 
 struct GradArgs {                       // dk and dv
@@ -56,7 +56,7 @@ struct GradArgs {                       // dk and dv
     const float* seg;
     int inner, n, heads, nseg, seg_len;
     float m;
-    long long tasks;
+    unsigned tasks;
 };
 
 __device__ __forceinline__ int swap23(int l) { return (l & 0x13) | ((l & 4) << 1) | ((l & 8) >> 1); }
@@ -67,12 +67,10 @@ __device__ __forceinline__ float log2_decay(const float* log_decay, int head) {
     return fmaxf(log_decay[head] * LOG2E, -1e4f);
 }
 
-// p * w where w = 0 marks a pair that does not exist: zero whatever p is (0 * inf and 0 * NaN are 0)
-__device__ __forceinline__ float weigh(float p, float w) {
-    float r;
-    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(p), "v"(w));
-    return r;
-}
+// p * w where w = 0 marks a pair that does not exist: zero whatever p is (0 * inf and 0 * NaN are 0).  v_mul_legacy_f32 as
+// the compiler's intrinsic, so that it keeps the waits between a matrix instruction and the first use of its result.
+extern "C" __device__ float vdmi_mul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
+__device__ __forceinline__ float weigh(float p, float w) { return vdmi_mul_legacy(p, w); }
 
 // lambda^(..) v as a sum of 16-bit operands: three of bfloat16 (8 bits each), two halfs (11 bits each).
 // The matrix cores take subnormal half operands as zeros: the low halfs (2^-11 of the values at most) are multiplied up
@@ -127,8 +125,6 @@ struct Split {
 // Rows of one head, 32 tokens at a time: a buffer resource per tile, based on the tile's first row in memory, and 32-bit
 // lane offsets that stay the same from tile to tile; rows past the tile's last token get an offset past the resource's
 // end, which loads as zero and is not stored.  The tokens run backwards in memory where REVERSE.
-constexpr unsigned NOWHERE = 0x80000000u;
-
 struct Rows {
     const char* base;
     long long pitch;            // bytes
@@ -138,7 +134,7 @@ struct Rows {
         : base(static_cast<const char*>(p) + 2 * (bb * s.b + ii * s.i + head * s.h + col0)), pitch(2 * s.n),
           records((unsigned)(31 * 2 * s.n) + 2 * width) {}
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile(int first) const {
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + first * pitch), 0, records, 0x00020000);
+        return vdmi_rsrc(base + first * pitch, records);
     }
     // offset of column byte `col` of token `row` of a tile of cnt tokens
     __device__ __forceinline__ unsigned at(int row, int cnt, bool reverse, int col) const {
@@ -146,28 +142,21 @@ struct Rows {
     }
 };
 
-typedef __attribute__((ext_vector_type(4))) unsigned u4;
-template <typename T>
-__device__ __forceinline__ x8_t<T> load16(__amdgpu_buffer_rsrc_t r, unsigned off) {
-    return __builtin_bit_cast(x8_t<T>, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
-}
-template <typename T>
-__device__ __forceinline__ void store16(__amdgpu_buffer_rsrc_t r, unsigned off, const x8_t<T>& v) {
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), r, off, 0, 0);
-}
-
 // a wave's place: (sequence, head, segment, 32-column slice) and its tokens
 struct Place {
     int slice, head, seg, len, t_begin, t_stop, t_end;
     long long seq, bb, ii;
     template <typename A>
-    __device__ __forceinline__ Place(const A& a, long long w, int slices, int segs) {
+    __device__ __forceinline__ Place(const A& a, unsigned w, unsigned slices, unsigned segs) {
         slice = (int)(w % slices); w /= slices;
-        head = (int)(w % a.heads); w /= a.heads;
-        seg = (int)(w % segs);
-        seq = w / segs;
-        bb = seq / a.inner;
-        ii = seq - bb * a.inner;
+        const unsigned r = w / (unsigned)a.heads;
+        head = (int)(w - r * (unsigned)a.heads);
+        const unsigned sq = r / segs;
+        seg = (int)(r - sq * segs);
+        const unsigned ob = sq / (unsigned)a.inner;
+        seq = sq;
+        bb = ob;
+        ii = sq - ob * (unsigned)a.inner;
         len = a.n;
         if (a.lengths) len = min(max(a.lengths[seq], 0), a.n);
         t_begin = seg * a.seg_len;
@@ -203,49 +192,13 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     char* kimg = kimg_all[wave];
     char* vimg = vimg_all[wave];
-    const long long w = (long long)blockIdx.x * DW + wave;
+    const unsigned w = blockIdx.x * DW + wave;
     if (w >= a.tasks) return;
     const Place at(a, w, KT, STATE_ONLY && !a.s_out ? a.nseg - 1 : a.nseg);     // nobody reads the last segment's sum
     const bool reverse = a.reverse;
     const Rows qr(a.q, a.qs, at.bb, at.ii, at.head, 0, D), kr(a.k, a.ks, at.bb, at.ii, at.head, 0, D),
         vr(a.v, a.vs, at.bb, at.ii, at.head, 32 * at.slice, 32), orow(a.o, a.os, at.bb, at.ii, at.head, 32 * at.slice, 32);
     if (!STATE_ONLY) at.clear<T>(a.o, a.os, lane);
-
-    const float l2 = log2_decay(a.log_decay, at.head);
-    const long long state0 = (at.seq * a.heads + at.head) * (long long)(D * D);
-    // this lane's elements of S: row 32 kt + 16 (r >> 3) + 8 half + (r & 7), column 32 slice + swap23(l31)
-    const int s_col = (32 * at.slice + swap23(l31)) * a.cs;
-    f32x16 S[KT];
-    {
-        const float* src = nullptr;
-        float mul = 1.f;
-        if (!STATE_ONLY) {
-            if (a.nseg > 1) src = a.seg + (state0 * a.nseg + (long long)at.seg * (D * D));
-            else if (a.s_in) { src = a.s_in + state0; mul = a.s_in_mul; }
-        }
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) S[kt] = zero16();
-        if (src) {
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) S[kt][r] = src[(32 * kt + 16 * (r >> 3) + 8 * half + (r & 7)) * a.rs + s_col] * mul;
-        }
-    }
-    // decays: of a pair (register = key, lane = query), of the state towards a query, of a token towards the tile's end
-    float dw[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int gap = l31 - acc_row(r, half);
-        dw[r] = gap >= 0 ? a.m * __builtin_amdgcn_exp2f(l2 * (float)gap) : 0.f;
-    }
-    const float ow = a.m * __builtin_amdgcn_exp2f(l2 * (float)(l31 + a.e_out));
-    float* uw = uw_all[wave];
-    auto token_decays = [&](int cnt) {
-        if (half == 0) uw[l31] = __builtin_amdgcn_exp2f(l2 * (float)(max(cnt - 1 - l31, 0) + a.e_u));
-    };
-    token_decays(32);
-    float whole = __builtin_amdgcn_exp2f(l2 * 32.f);
 
     x8 kreg[KS], vreg[2], q[KS];
     unsigned kofs[KS], vofs[2], qofs;
@@ -278,6 +231,51 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
         load_kv(at.t_begin, cnt);
         if (!STATE_ONLY) load_q(at.t_begin, cnt);
     }
+    const float l2 = log2_decay(a.log_decay, at.head);
+    const long long state0 = (at.seq * a.heads + at.head) * (long long)(D * D);
+    // this lane's elements of S: row 32 kt + 16 (r >> 3) + 8 half + (r & 7), column 32 slice + swap23(l31)
+    const int s_col = (32 * at.slice + swap23(l31)) * (a.rs == 1 ? D : 1);
+    f32x16 S[KT];
+    {
+        const float* src = nullptr;
+        float mul = 1.f;
+        if (!STATE_ONLY) {
+            if (a.nseg > 1) src = a.seg + (state0 * a.nseg + (long long)at.seg * (D * D));
+            else if (a.s_in) { src = a.s_in + state0; mul = a.s_in_mul; }
+        }
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) S[kt] = zero16();
+        if (src && a.rs == 1) {             // a column's rows are contiguous: eight at a time
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(src + s_col + 32 * kt + 16 * (q >> 1) + 8 * half + 4 * (q & 1));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) S[kt][4 * q + e] = x[e] * mul;
+                }
+        } else if (src) {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) S[kt][r] = src[(32 * kt + 16 * (r >> 3) + 8 * half + (r & 7)) * D + s_col] * mul;
+        }
+    }
+    // decays: of a pair (register = key, lane = query), of the state towards a query, of a token towards the tile's end
+    float dw[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int gap = l31 - acc_row(r, half);
+        dw[r] = gap >= 0 ? a.m * __builtin_amdgcn_exp2f(l2 * (float)gap) : 0.f;
+    }
+    const float ow = a.m * __builtin_amdgcn_exp2f(l2 * (float)(l31 + a.e_out));
+    float* uw = uw_all[wave];
+    auto token_decays = [&](int cnt) {
+        if (half == 0) uw[l31] = __builtin_amdgcn_exp2f(l2 * (float)(max(cnt - 1 - l31, 0) + a.e_u));
+    };
+    token_decays(32);
+    float whole = __builtin_amdgcn_exp2f(l2 * 32.f);
+
     for (int t0 = at.t_begin; t0 < at.t_end; t0 += 32) {
         cnt = min(32, at.t_end - t0);
         const int next = min(32, at.t_end - t0 - 32);
@@ -285,6 +283,7 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
         for (int i = 0; i < KS; ++i) *reinterpret_cast<x8*>(kimg + (lane / (D / 8) + RS * i) * KP + 16 * (lane % (D / 8))) = kreg[i];
 #pragma unroll
         for (int i = 0; i < 2; ++i) *reinterpret_cast<x8*>(vimg + (16 * i + (lane >> 2)) * VP + 16 * (lane & 3)) = vreg[i];
+        wave_lds_order();
         if (next > 0) {
             if (next < 32) offsets(next);
             load_kv(t0 + 32, next);
@@ -307,8 +306,10 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
             o = mfma16(v0, acc_operand<T>(st, 0), o);
             o = mfma16(v1, acc_operand<T>(st, 1), o);
             // through LDS (the tile's v image is in registers by now) to 16-byte stores, four lanes on a row's 64 bytes
+            wave_lds_order();
             *reinterpret_cast<x8*>(vimg + l31 * VP + 16 * half) = acc_operand<T>(o, 0);
             *reinterpret_cast<x8*>(vimg + l31 * VP + 32 + 16 * half) = acc_operand<T>(o, 1);
+            wave_lds_order();
             const auto ro = orow.tile(first_row(t0, cnt));
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -319,9 +320,11 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
         if (cnt < 32) {
             token_decays(cnt);
             whole = __builtin_amdgcn_exp2f(l2 * (float)cnt);
+            wave_lds_order();
         }
         const Split<T> sv(v0, v1, uw, half);
         sv.update(S, whole, ktr, KP);
+        wave_lds_order();               // the images and weights are read: the next tile may come
     }
     float* dst = nullptr;
     float mul = 1.f;
@@ -331,7 +334,7 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) dst[(32 * kt + 16 * (r >> 3) + 8 * half + (r & 7)) * a.rs + s_col] = S[kt][r] * mul;
+            for (int r = 0; r < 16; ++r) dst[(32 * kt + 16 * (r >> 3) + 8 * half + (r & 7)) * D + s_col] = S[kt][r] * mul;
     }
 }
 
@@ -349,7 +352,7 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     char* qimg = qimg_all[wave];
     char* gimg = gimg_all[wave];
-    const long long w = (long long)blockIdx.x * DW + wave;
+    const unsigned w = blockIdx.x * DW + wave;
     if (w >= a.tasks) return;
     const Place at(a, w, KT, a.nseg);
     const Rows qr(a.q, a.qs, at.bb, at.ii, at.head, 0, D), kr(a.k, a.ks, at.bb, at.ii, at.head, 0, D),
@@ -357,38 +360,6 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
         dkr(a.dk, a.dks, at.bb, at.ii, at.head, 32 * at.slice, 32), dvr(a.dv, a.dvs, at.bb, at.ii, at.head, 32 * at.slice, 32);
     at.clear<T>(a.dk, a.dks, lane);
     at.clear<T>(a.dv, a.dvs, lane);
-
-    const float l2 = log2_decay(a.log_decay, at.head);
-    const long long state0 = (at.seq * a.heads + at.head) * (long long)(D * D);
-    const int col = 32 * at.slice + swap23(l31);
-    f32x16 R[KT], Rt[KT];
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) R[kt] = Rt[kt] = zero16();
-    const float* src = a.nseg > 1 ? a.seg + (state0 * a.nseg + (long long)at.seg * (D * D)) : a.s_in ? a.s_in + state0 : nullptr;
-    if (src) {
-        const float mul = a.nseg > 1 ? 1.f : 1.f / a.m;
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row = 32 * kt + 16 * (r >> 3) + 8 * half + (r & 7);
-                R[kt][r] = src[row * D + col] * mul;
-                Rt[kt][r] = src[col * D + row] * mul;
-            }
-    }
-    float dw[16];                       // as in the scan; register = query, lane = key, both counted backward in time
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int gap = l31 - acc_row(r, half);
-        dw[r] = gap >= 0 ? a.m * __builtin_amdgcn_exp2f(l2 * (float)gap) : 0.f;
-    }
-    const float ow = a.m * __builtin_amdgcn_exp2f(l2 * (float)l31);
-    float* uw = uw_all[wave];
-    auto token_decays = [&](int cnt) {
-        if (half == 0) uw[l31] = __builtin_amdgcn_exp2f(l2 * (float)(max(cnt - 1 - l31, 0) + 1));
-    };
-    token_decays(32);
-    float whole = __builtin_amdgcn_exp2f(l2 * 32.f);
 
     x8 qreg[KS], greg[KS], k[KS], v[KS];
     unsigned qofs[KS], gofs[KS], kofs, vofs;
@@ -426,6 +397,38 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
         load_qg(at.t_begin, cnt);
         load_kv(at.t_begin, cnt);
     }
+    const float l2 = log2_decay(a.log_decay, at.head);
+    const long long state0 = (at.seq * a.heads + at.head) * (long long)(D * D);
+    const int col = 32 * at.slice + swap23(l31);
+    f32x16 R[KT], Rt[KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) R[kt] = Rt[kt] = zero16();
+    const float* src = a.nseg > 1 ? a.seg + (state0 * a.nseg + (long long)at.seg * (D * D)) : a.s_in ? a.s_in + state0 : nullptr;
+    if (src) {
+        const float mul = a.nseg > 1 ? 1.f : 1.f / a.m;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = 32 * kt + 16 * (r >> 3) + 8 * half + (r & 7);
+                R[kt][r] = src[row * D + col] * mul;
+                Rt[kt][r] = src[col * D + row] * mul;
+            }
+    }
+    float dw[16];                       // as in the scan; register = query, lane = key, both counted backward in time
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int gap = l31 - acc_row(r, half);
+        dw[r] = gap >= 0 ? a.m * __builtin_amdgcn_exp2f(l2 * (float)gap) : 0.f;
+    }
+    const float ow = a.m * __builtin_amdgcn_exp2f(l2 * (float)l31);
+    float* uw = uw_all[wave];
+    auto token_decays = [&](int cnt) {
+        if (half == 0) uw[l31] = __builtin_amdgcn_exp2f(l2 * (float)(max(cnt - 1 - l31, 0) + 1));
+    };
+    token_decays(32);
+    float whole = __builtin_amdgcn_exp2f(l2 * 32.f);
+
     for (int t0 = at.t_begin; t0 < at.t_end; t0 += 32) {
         cnt = min(32, at.t_end - t0);
         const int next = min(32, at.t_end - t0 - 32);
@@ -434,6 +437,7 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
             *reinterpret_cast<x8*>(qimg + (lane / (D / 8) + RS * i) * KP + 16 * (lane % (D / 8))) = qreg[i];
             *reinterpret_cast<x8*>(gimg + (lane / (D / 8) + RS * i) * KP + 16 * (lane % (D / 8))) = greg[i];
         }
+        wave_lds_order();
         if (next > 0) {
             if (next < 32) offsets(next);
             load_qg(t0 + 32, next);
@@ -466,6 +470,7 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
         if (cnt < 32) {
             token_decays(cnt);
             whole = __builtin_amdgcn_exp2f(l2 * (float)cnt);
+            wave_lds_order();
         }
         {
             const Split<T> sg(g0, g1, uw, half);
@@ -476,11 +481,13 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
             sq.update(Rt, whole, gtr, KP);
         }
         // the images are done with: results through them to 16-byte stores, four lanes on a row's 64 bytes
+        wave_lds_order();
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             *reinterpret_cast<x8*>(qimg + l31 * VP + 32 * s + 16 * half) = acc_operand<T>(ok, s);
             *reinterpret_cast<x8*>(gimg + l31 * VP + 32 * s + 16 * half) = acc_operand<T>(ov, s);
         }
+        wave_lds_order();
         const auto rk = dkr.tile(at.len - t0 - cnt), rv = dvr.tile(at.len - t0 - cnt);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -488,6 +495,7 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
             store16<T>(rk, dkr.at(row, cnt, true, 16 * (lane & 3)), *reinterpret_cast<const x8*>(qimg + row * VP + 16 * (lane & 3)));
             store16<T>(rv, dvr.at(row, cnt, true, 16 * (lane & 3)), *reinterpret_cast<const x8*>(gimg + row * VP + 16 * (lane & 3)));
         }
+        wave_lds_order();
     }
     if (a.s_out && a.nseg == 1) {
         float* dst = a.s_out + state0;
@@ -539,7 +547,7 @@ __global__ __launch_bounds__(256) void decay_segments_kernel(const ScanArgs a, i
 // Sequences of up to 32 tokens without states (the frames of a site): g = 32 / n whole sequences share a tile of 32
 // rows, pairs of different sequences weigh nothing, and the backward pass does all three gradients from one read of q, k,
 // v and do (dP^T = V dO^T with lane = query for dq; P = Q K^T and dP = dO V^T with lane = key for dv and dk).  A wave
-// takes (tile, head) units one after the other, always of the same head, the next unit's rows in flight.
+// computes one (tile, head) and ends: enough of them share a SIMD to cover each other's loads.
 // A row that is not finite must not reach the other sequences of its tile (zero times infinity in the second product):
 // such a tile is computed once per sequence with the others' rows as zeros.
 // ------------------------------------------------------------------------------------------------------------------
@@ -553,7 +561,7 @@ struct ShortArgs {
     const float* log_decay;
     const int* lengths;
     int n, heads, per_tile, tiles;
-    unsigned inner, magic;
+    unsigned inner, magic, inv_n;       // row / n = row * inv_n >> 16 for row < 32
     int shift;                          // seq / inner = umulhi(seq, magic) >> shift; shift < 0: inner is 1
     float m;
     unsigned nseq;
@@ -565,153 +573,166 @@ __device__ __forceinline__ bool finite(const x8_t<T> (&x)[N]) {
     us2 top = {0, 0};
 #pragma unroll
     for (int s = 0; s < N; ++s) {
-        const u4 w = __builtin_bit_cast(u4, x[s]);
+        const vdmi_u4 w = __builtin_bit_cast(vdmi_u4, x[s]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(us2, w[i] & 0x7fff7fffu));
     }
     return top[0] < Pack<T>::EXP && top[1] < Pack<T>::EXP;
 }
 
-template <typename T, int D, bool BWD>
-__global__ __launch_bounds__(DW * 64, D == 128 && BWD ? 1 : D == 32 && !BWD ? 3 : 2) void decay_short_kernel(const ShortArgs a) {
+// NH heads of D features side by side in memory are one row of W columns, moved as 16-byte pieces with all lanes of a row
+// next to each other and transposed to operands through LDS.  Measured over 16 frames of 16384 sites with 8 heads of 32
+// features (537 MB forward, 940 MB backward): 122 us and 197 us, 4.4 and 4.8 TB/s; one head at a time (64-byte rows) 127
+// and 234 us; every lane loading and storing its own token's row as operands (32 bytes of a row per instruction) 150 and 283.
+constexpr int short_waves(int d, bool bwd) { return d == 128 && bwd ? 1 : 2; }
+
+template <typename T, int D, int NH, bool BWD>
+__global__ __launch_bounds__((short_waves(D, BWD) * 64), D == 128 ? 1 : 2) void decay_short_kernel(const ShortArgs a) {
     typedef x8_t<T> x8;
-    constexpr int KS = D / 16, DT = D / 32, P = 2 * D + 16, NI = BWD ? 3 : 1;
-    constexpr bool AHEAD = D == 32 || (D == 64 && !BWD);       // the next unit's rows in flight, where registers allow it
-    __shared__ __attribute__((aligned(16))) char img_all[DW][NI][32 * P];       // forward: v; backward: k, q, do
+    constexpr int SW = short_waves(D, BWD), W = D * NH, KS = D / 16, DT = D / 32, P = 2 * W + 16, NT = BWD ? 4 : 3;
+    constexpr int PR = W / 8, RPI = 64 / PR, NI = 32 / RPI;       // 16-byte pieces of a row, rows per load, loads
+    __shared__ __attribute__((aligned(16))) char img_all[SW][NT][32 * P];       // q, k, v, do; results take their places
+    __shared__ float fade_all[SW][64];
     const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const unsigned gid = blockIdx.x * DW + wave, step = gridDim.x * DW / a.heads;      // gridDim.x is a multiple of the heads
-    const int head = (int)(gid % a.heads), n = a.n;
-    const int slot = l31 / n, ti = l31 - slot * n;
-    const bool in_tile = slot < a.per_tile;
-    const float l2 = log2_decay(a.log_decay, head);
-    // weights of (register = key, lane = query) and, for the backward, (register = query, lane = key)
-    float dw[16], dwt[BWD ? 16 : 1];
+    const unsigned groups = (unsigned)a.heads / NH, unit = blockIdx.x * SW + wave, tile = unit / groups;
+    if (tile >= (unsigned)a.tiles) return;
+    const int head0 = (int)(unit - tile * groups) * NH, n = a.n;
+    char (*im)[32 * P] = img_all[wave];
+
+    // rows RPI i + lane / PR of the tile, piece lane % PR: their sequence, whether they are the call's, whether live
+    const int piece = lane % PR;
+    unsigned bb[NI], ii[NI], tt[NI];
+    bool mine[NI], live[NI];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int t = acc_row(r, half), gap = l31 - t;
-        const bool same = in_tile && t / n == slot;
-        const float d = a.m * __builtin_amdgcn_exp2f(l2 * fabsf((float)gap));
-        dw[r] = same && gap >= 0 ? d : 0.f;
-        if constexpr (BWD) dwt[r] = same && gap <= 0 ? d : 0.f;
+    for (int i = 0; i < NI; ++i) {
+        const unsigned row = RPI * i + lane / PR, slot = row * a.inv_n >> 16;
+        tt[i] = row - slot * n;
+        unsigned seq = tile * (unsigned)a.per_tile + slot;
+        mine[i] = slot < (unsigned)a.per_tile && seq < a.nseq;
+        seq = min(seq, a.nseq - 1);     // a row that is not there loads another one; nothing of it is stored
+        bb[i] = a.shift < 0 ? seq : __umulhi(seq, a.magic) >> a.shift;
+        ii[i] = seq - bb[i] * a.inner;
+        live[i] = !a.lengths || (int)tt[i] < a.lengths[seq];
     }
+    auto row_of = [&](const void* p, const Strides32& s, long long h, int i) {
+        return const_cast<x8*>(reinterpret_cast<const x8*>(static_cast<const char*>(p) + 2 * head0 * h + (unsigned long long)bb[i] * s.b +
+                                                           (unsigned long long)ii[i] * s.i + (unsigned long long)(tt[i] * s.n + 16 * piece)));
+    };
     x8 zero8;
 #pragma unroll
     for (int j = 0; j < 8; ++j) zero8[j] = (T)0.f;
-    const int tr_off = tr_offset(lane, P);
-
-    struct Unit {
-        x8 q[KS], k[KS], v[KS], g[BWD ? KS : 1];
-        unsigned bb, ii;
-        bool ok;                        // this lane's row is one of the call's
-    };
-    auto rows_of = [&](const void* p, const Strides32& s, long long h, const Unit& x) {
-        return reinterpret_cast<const x8*>(static_cast<const char*>(p) + 2 * head * h + (unsigned long long)x.bb * s.b +
-                                           (unsigned long long)x.ii * s.i + (unsigned long long)((unsigned)ti * s.n + 16 * half));
-    };
-    auto fetch = [&](unsigned tile, Unit& x) {
-        unsigned seq = tile * (unsigned)a.per_tile + (unsigned)min(slot, a.per_tile - 1);
-        x.ok = in_tile && tile < (unsigned)a.tiles && seq < a.nseq;
-        seq = min(seq, a.nseq - 1);     // lanes without a row load one that is there; nothing of it is stored
-        x.bb = a.shift < 0 ? seq : __umulhi(seq, a.magic) >> a.shift;
-        x.ii = seq - x.bb * a.inner;
-        const x8* qp = rows_of(a.q, a.qs, a.qh, x);
-        const x8* kp = rows_of(a.k, a.ks, a.kh, x);
-        const x8* vp = rows_of(a.v, a.vs, a.vh, x);
+    // rows of the sequences [s_lo, s_hi) of the tile into the images, the others as zeros; whether all of it is finite
+    auto load = [&](int s_lo, int s_hi) {
+        x8 x[NT][NI];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            x.q[s] = qp[2 * s];
-            x.k[s] = kp[2 * s];
-            x.v[s] = vp[2 * s];
+        for (int i = 0; i < NI; ++i) {
+            x[0][i] = *row_of(a.q, a.qs, a.qh, i);
+            x[1][i] = *row_of(a.k, a.ks, a.kh, i);
+            x[2][i] = *row_of(a.v, a.vs, a.vh, i);
+            if constexpr (BWD) x[3][i] = *row_of(a.g, a.gs, a.gh, i);
         }
-        if constexpr (BWD) {
-            const x8* gp = rows_of(a.g, a.gs, a.gh, x);
+        if (a.lengths || s_hi - s_lo < a.per_tile) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) x.g[s] = gp[2 * s];
-        }
-        if (a.lengths && ti >= a.lengths[seq]) {
+            for (int i = 0; i < NI; ++i) {
+                const int slot = (int)((RPI * i + lane / PR) * a.inv_n >> 16);
+                if (!live[i] || slot < s_lo || slot >= s_hi) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                x.q[s] = x.k[s] = x.v[s] = zero8;
-                if constexpr (BWD) x.g[s] = zero8;
+                    for (int t = 0; t < NT; ++t) x[t][i] = zero8;
+                }
             }
         }
-    };
-    auto to_image = [&](char* im, const x8 (&x)[KS]) {
+        bool fine = true;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) *reinterpret_cast<x8*>(im + l31 * P + 32 * s + 16 * half) = x[s];
+        for (int t = 0; t < NT; ++t) {
+            if (BWD || t == 2) fine = fine & finite<T>(x[t]);
+#pragma unroll
+            for (int i = 0; i < NI; ++i) *reinterpret_cast<x8*>(im[t] + (RPI * i + lane / PR) * P + 16 * piece) = x[t][i];
+        }
+        return fine;
     };
-    // contraction over the features of two row sets, weighed (two accumulators: no chain of dependent products)
-    auto pairs = [&](const x8 (&x)[KS], const x8 (&y)[KS], const float (&d)[16]) {
+    auto store = [&](const char* src, void* dst, const Strides32& s, long long h, int s_lo, int s_hi) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int slot = (int)((RPI * i + lane / PR) * a.inv_n >> 16);
+            const x8 x = *reinterpret_cast<const x8*>(src + (RPI * i + lane / PR) * P + 16 * piece);
+            if (mine[i] && slot >= s_lo && slot < s_hi) *row_of(dst, s, h, i) = x;
+        }
+    };
+
+    const int slot = (int)(l31 * a.inv_n >> 16), ti = l31 - slot * n;
+    const bool in_tile = slot < a.per_tile;
+    float* fade = fade_all[wave];
+    const int tr_off = tr_offset(lane, P);
+    // contraction over the features of two row sets, times the decays of (register, lane) = (key, query) or, by_key, (query,
+    // key): pairs within a sequence, the key not after the query
+    auto pairs = [&](const char* x, const char* y, bool by_key) {
         f32x16 p = zero16(), p2 = zero16();
 #pragma unroll
         for (int s = 0; s < KS; s += 2) {
-            p = mfma16(x[s], y[s], p);
-            p2 = mfma16(x[s + 1], y[s + 1], p2);
+            const int at = l31 * P + 32 * s + 16 * half;
+            p = mfma16(*reinterpret_cast<const x8*>(x + at), *reinterpret_cast<const x8*>(y + at), p);
+            p2 = mfma16(*reinterpret_cast<const x8*>(x + at + 32), *reinterpret_cast<const x8*>(y + at + 32), p2);
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] = weigh(p[r] + p2[r], d[r]);
+        for (int r = 0; r < 16; ++r) {
+            const int t = acc_row(r, half), gap = by_key ? t - l31 : l31 - t;
+            const float w = (unsigned)gap <= (unsigned)(by_key ? n - 1 - ti : ti) && in_tile ? fade[32 + gap] : 0.f;
+            p[r] = weigh(p[r] + p2[r], w);
+        }
         return p;
     };
-    // (an image)^T x pairs: this lane's row, 16 bytes at features 8 half .. and 16 + 8 half .. of every 32
-    auto product = [&](const char* im, const f32x16& p, void* dst, const Strides32& s, long long h, const Unit& x, bool mine) {
+    // (columns of an image)^T x pairs into the same columns of another one
+    auto product = [&](const char* src, const f32x16& p, char* dst) {
         const x8 p0 = acc_operand<T>(p, 0), p1 = acc_operand<T>(p, 1);
-        x8* row = const_cast<x8*>(rows_of(dst, s, h, x));
+        f32x16 o[DT];
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-            f32x16 o = mfma16(tr_operand<T>(im + tr_off + 64 * dt, 8 * P), p0, zero16());
-            o = mfma16(tr_operand<T>(im + tr_off + 64 * dt + 16 * P, 8 * P), p1, o);
-            if (mine) {
-                row[4 * dt] = acc_operand<T>(o, 0);
-                row[4 * dt + 2] = acc_operand<T>(o, 1);
-            }
+            o[dt] = mfma16(tr_operand<T>(src + tr_off + 64 * dt, 8 * P), p0, zero16());
+            o[dt] = mfma16(tr_operand<T>(src + tr_off + 64 * dt + 16 * P, 8 * P), p1, o[dt]);
         }
-    };
-    auto compute = [&](const Unit& x, bool mine) {
-        char (*im)[32 * P] = img_all[wave];
-        if constexpr (!BWD) {
-            to_image(im[0], x.v);
-            product(im[0], pairs(x.k, x.q, dw), a.o, a.os, a.oh, x, mine);
-        } else {
-            to_image(im[0], x.k);
-            to_image(im[1], x.q);
-            to_image(im[2], x.g);
-            product(im[0], pairs(x.v, x.g, dw), a.dq, a.dqs, a.dqh, x, mine);          // [key x query]
-            product(im[2], pairs(x.q, x.k, dwt), a.dv, a.dvs, a.dvh, x, mine);         // [query x key]
-            product(im[1], pairs(x.g, x.v, dwt), a.dk, a.dks, a.dkh, x, mine);
-        }
-    };
-
-    Unit nx;
-    const unsigned tile0 = gid / a.heads;
-    if (AHEAD && tile0 < (unsigned)a.tiles) fetch(tile0, nx);
-    for (unsigned tile = tile0; tile < (unsigned)a.tiles; tile += step) {
-        Unit c;
-        if constexpr (AHEAD) {
-            c = nx;
-            if (tile + step < (unsigned)a.tiles) fetch(tile + step, nx);
-        } else {
-            fetch(tile, c);
-        }
-        bool fine = true;
-        if (a.per_tile > 1) {
-            fine = finite<T>(c.v);
-            if constexpr (BWD) fine = fine && finite<T>(c.k) && finite<T>(c.q) && finite<T>(c.g);
-        }
-        if (__builtin_amdgcn_ballot_w64(!fine) == 0) {
-            compute(c, c.ok);
-        } else {
-            for (int pass = 0; pass < a.per_tile; ++pass) {
-                Unit x = c;
-                if (slot != pass) {
+        wave_lds_order();
 #pragma unroll
-                    for (int s = 0; s < KS; ++s) {
-                        x.q[s] = x.k[s] = x.v[s] = zero8;
-                        if constexpr (BWD) x.g[s] = zero8;
-                    }
-                }
-                compute(x, c.ok && slot == pass);
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) *reinterpret_cast<x8*>(dst + l31 * P + 64 * dt + 32 * s + 16 * half) = acc_operand<T>(o[dt], s);
+    };
+    auto compute = [&](int s_lo, int s_hi) {
+#pragma unroll
+        for (int j = 0; j < NH; ++j) {
+            wave_lds_order();
+            // m lambda^gap by gap + 32
+            fade[lane] = a.m * __builtin_amdgcn_exp2f(log2_decay(a.log_decay, head0 + j) * (float)max(lane - 32, 0));
+            wave_lds_order();
+            const int c = 2 * D * j;
+            if constexpr (!BWD) {
+                product(im[2] + c, pairs(im[1] + c, im[0] + c, false), im[0] + c);
+            } else {
+                const f32x16 p = pairs(im[2] + c, im[3] + c, false);                    // [key x query]: v do
+                const f32x16 pv = pairs(im[0] + c, im[1] + c, true);                    // [query x key]: q k
+                const f32x16 pk = pairs(im[3] + c, im[2] + c, true);                    // do v
+                product(im[1] + c, p, im[2] + c);                                       // dq, where v was
+                product(im[3] + c, pv, im[3] + c);                                      // dv, where do was
+                product(im[0] + c, pk, im[0] + c);                                      // dk, where q was
             }
+        }
+        wave_lds_order();
+        if constexpr (!BWD) {
+            store(im[0], a.o, a.os, a.oh, s_lo, s_hi);
+        } else {
+            store(im[2], a.dq, a.dqs, a.dqh, s_lo, s_hi);
+            store(im[3], a.dv, a.dvs, a.dvh, s_lo, s_hi);
+            store(im[0], a.dk, a.dks, a.dkh, s_lo, s_hi);
+        }
+    };
+    const bool fine = load(0, a.per_tile);
+    if (a.per_tile == 1 || __builtin_amdgcn_ballot_w64(!fine) == 0) {
+        compute(0, a.per_tile);
+    } else {
+        for (int pass = 0; pass < a.per_tile; ++pass) {
+            wave_lds_order();
+            load(pass, pass + 1);
+            compute(pass, pass + 1);
         }
     }
 }
@@ -834,9 +855,9 @@ template <bool STATE_ONLY>
 int launch_scan(const ScanArgs& s, const vdmi_decay_args* a, const Plan& p, hipStream_t st) {
     ScanArgs x = s;
     const long long segs = STATE_ONLY && !x.s_out ? p.nseg - 1 : p.nseg;
-    x.tasks = p.nseq * a->heads * segs * (a->d / 32);
-    const long long wgs = (x.tasks + DW - 1) / DW;
-    if (wgs > 0x7fffffffLL) return VDMI_E_SHAPE;
+    const long long tasks = p.nseq * a->heads * segs * (a->d / 32), wgs = (tasks + DW - 1) / DW;
+    if (tasks > 0x7fffffffLL) return VDMI_E_SHAPE;
+    x.tasks = (unsigned)tasks;
     const dim3 grid((unsigned)wgs), block(DW * 64);
 #define SCAN(T, D) hipLaunchKernelGGL((decay_scan_kernel<T, D, STATE_ONLY>), grid, block, 0, st, x)
 #define SCAN_D(T) do { if (a->d == 32) SCAN(T, 32); else if (a->d == 64) SCAN(T, 64); else SCAN(T, 128); } while (0)
@@ -850,8 +871,6 @@ int launch_scan(const ScanArgs& s, const vdmi_decay_args* a, const Plan& p, hipS
 // sums of the segments and the states at their starts (nothing to do for one segment)
 int segment_states(ScanArgs s, const vdmi_decay_args* a, const Plan& p, hipStream_t st) {
     if (p.nseg == 1) return VDMI_OK;
-    s.rs = a->d;
-    s.cs = 1;
     const int r = launch_scan<true>(s, a, p, st);
     if (r != VDMI_OK) return r;
     hipLaunchKernelGGL(decay_segments_kernel, dim3((unsigned)(p.nseq * a->heads), (unsigned)(a->d * a->d / 256)), dim3(256), 0, st,
@@ -871,7 +890,7 @@ ScanArgs scan_args(const vdmi_decay_args* a, const Plan& p) {
     s.lengths = a->lengths;
     s.s_in_mul = s.s_out_mul = 1.f;
     s.seg = static_cast<float*>(a->workspace);
-    s.rs = a->d; s.cs = 1;
+    s.rs = a->d;
     s.inner = a->inner; s.n = a->n; s.heads = a->heads;
     s.nseg = p.nseg; s.seg_len = p.seg_len;
     s.m = a->scale;
@@ -903,15 +922,17 @@ int launch_short(const vdmi_decay_args* a, const Plan& p, bool bwd, hipStream_t 
         s.magic = (unsigned)((1ULL << (31 + l)) / (unsigned)a->inner + 1);
         s.shift = l - 1;
     }
-    // a wave keeps its head: the number of waves is a multiple of the heads
-    long long wgs = ((long long)s.tiles * a->heads + DW - 1) / DW;
-    if (wgs > 2048) wgs = 2048;
-    wgs = (wgs + a->heads - 1) / a->heads * a->heads;
-    const dim3 grid((unsigned)wgs), block(DW * 64);
-#define SHORT(T, D) do { if (bwd) hipLaunchKernelGGL((decay_short_kernel<T, D, true>), grid, block, 0, st, s); \
-                         else hipLaunchKernelGGL((decay_short_kernel<T, D, false>), grid, block, 0, st, s); } while (0)
-#define SHORT_D(T) do { if (a->d == 32) SHORT(T, 32); else if (a->d == 64) SHORT(T, 64); else SHORT(T, 128); } while (0)
-    if (a->dtype == VDMI_DT_BF16) SHORT_D(__bf16); else SHORT_D(_Float16);
+    s.inv_n = 65536u / a->n + 1;
+    // two heads of 32 features next to each other in every tensor
+    bool two = a->d == 32 && a->heads % 2 == 0;
+    for (const vdmi_rows4* r : {&a->q, &a->k, &a->v, &a->o, &a->dout, &a->dq, &a->dk, &a->dv}) two = two && (!r->p || r->h == 32);
+#define SHORT(T, D, NH, B) do { constexpr int sw = short_waves(D, B); \
+    const long long wgs = ((long long)s.tiles * (a->heads / NH) + sw - 1) / sw; \
+    hipLaunchKernelGGL((decay_short_kernel<T, D, NH, B>), dim3((unsigned)wgs), dim3(sw * 64), 0, st, s); } while (0)
+#define SHORT_D(T, B) do { if (two) SHORT(T, 32, 2, B); else if (a->d == 32) SHORT(T, 32, 1, B); else if (a->d == 64) SHORT(T, 64, 1, B); \
+                           else SHORT(T, 128, 1, B); } while (0)
+    if (a->dtype == VDMI_DT_BF16) { if (bwd) SHORT_D(__bf16, true); else SHORT_D(__bf16, false); }
+    else { if (bwd) SHORT_D(_Float16, true); else SHORT_D(_Float16, false); }
 #undef SHORT_D
 #undef SHORT
     VDMI_LAUNCH_CHECK();
@@ -928,9 +949,9 @@ int launch_grad(const vdmi_decay_args* a, const Plan& p, hipStream_t st) {
     g.seg = static_cast<const float*>(a->workspace);
     g.inner = a->inner; g.n = a->n; g.heads = a->heads; g.nseg = p.nseg; g.seg_len = p.seg_len;
     g.m = a->scale;
-    g.tasks = p.nseq * a->heads * p.nseg * (a->d / 32);
-    const long long wgs = (g.tasks + DW - 1) / DW;
-    if (wgs > 0x7fffffffLL) return VDMI_E_SHAPE;
+    const long long tasks = p.nseq * a->heads * p.nseg * (a->d / 32), wgs = (tasks + DW - 1) / DW;
+    if (tasks > 0x7fffffffLL) return VDMI_E_SHAPE;
+    g.tasks = (unsigned)tasks;
     const dim3 grid((unsigned)wgs), block(DW * 64);
 #define GRAD_D(T) do { if (a->d == 32) hipLaunchKernelGGL((decay_grad_kernel<T, 32>), grid, block, 0, st, g); \
                        else if (a->d == 64) hipLaunchKernelGGL((decay_grad_kernel<T, 64>), grid, block, 0, st, g); \
@@ -983,7 +1004,6 @@ extern "C" int vdmi_decay_attn_bwd(const vdmi_decay_args* a, vdmi_stream stream)
     s.s_in = a->state_in;
     s.e_out = 1;
     s.rs = 1;
-    s.cs = a->d;
     role(s, a->dout, a->v, a->k, a->dq);
     int r = launch_scan<false>(s, a, p, st);
     if (r != VDMI_OK) return r;

@@ -82,6 +82,14 @@ __device__ __forceinline__ void widen8(float (&v)[8], uint2 w, unsigned exp) {
     v[4] = c[0] * s; v[5] = c[1] * s; v[6] = d[0] * s; v[7] = d[1] * s;
 }
 
+// the same to bfloat16, two codes an instruction: exact, since every code times its power of two is a bfloat16
+__device__ __forceinline__ Pack<__bf16>::x8 widen8_bf16(vdmi_u2 w, unsigned exp) {
+    const float s = __uint_as_float(exp << 23);
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, s, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, s, true);
+    const auto c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, s, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, s, true);
+    return Pack<__bf16>::x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
 struct UnpackArgs {
     const unsigned char* codes;
     const unsigned char* exps;
@@ -119,6 +127,7 @@ __global__ __launch_bounds__(256) void rows8_unpack_kernel(const UnpackArgs a) {
 // 64 x 64 each; LDS rows are 320 bytes apart (the four rows x two column blocks of a half wave's read fall into different
 // banks).  Shares are added in a fixed order by a second launch.  The bias gradient sum_r dy comes from the staged pieces.
 constexpr int WK = 64, WT = 128, WPITCH = 320;
+constexpr double WSTAGE_US = 0.7;
 
 struct Wgrad8Args {
     const unsigned char* codes; const unsigned char* exps;
@@ -126,7 +135,7 @@ struct Wgrad8Args {
     float* part;                // [split][o tiles][i tiles][128][128]
     float* bpart;               // [split][o tiles][128] or null
     long long lddy, rows, per;  // per: rows of a share
-    int cin, cout, groups, to, ti;
+    int cin, cout, groups, to, ti, splits;
 };
 
 typedef Pack<__bf16>::x8 b8;
@@ -134,52 +143,45 @@ typedef Pack<__bf16>::x8 b8;
 __global__ __launch_bounds__(256, 2) void rows8_wgrad_kernel(const Wgrad8Args a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];          // [buffer][dy | x][64][320]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, l31 = lane & 31;
-    const int ot = blockIdx.x % a.to, it = (blockIdx.x / a.to) % a.ti;
-    const long long split = blockIdx.x / (a.to * a.ti);
+    // workgroups go round the eight XCDs, each with its own L2: all tiles of a share of the rows on one of them
+    const unsigned tiles = a.to * a.ti, k = a.splits % 8 == 0 ? blockIdx.x >> 3 : blockIdx.x, share = k / tiles;
+    const int tile = (int)(k - share * tiles), it = tile / a.to, ot = tile - it * a.to;
+    const long long split = a.splits % 8 == 0 ? (blockIdx.x & 7) + 8 * share : share;
     const int o0 = ot * WT, i0 = it * WT;
     const long long r_begin = split * a.per, r_end = min(r_begin + a.per, a.rows);
     // staging: piece tid + 256 j is (row (tid >> 4) + 16 j, columns 8 (tid & 15) ..): a thread's column is fixed
     const int prow = tid >> 4, pc = tid & 15;
-    const bool a_on = o0 + 8 * pc < a.cout, b_on = i0 + 8 * pc < a.cin;
-    b8 zero8;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) zero8[e] = (__bf16)0.f;
-    b8 va[4];
-    uint2 vb[4];
-    unsigned ve[4];
+    // byte offsets within a stage; columns past the operands' ends load zeros, and so do rows past the share's end
+    const unsigned aoff = o0 + 8 * pc < a.cout ? (unsigned)(prow * a.lddy + o0 + 8 * pc) * 2 : NOWHERE;
+    const unsigned boff = i0 + 8 * pc < a.cin ? (unsigned)(prow * a.cin + i0 + 8 * pc) : NOWHERE;
+    const unsigned eoff = i0 + 8 * pc < a.cin ? (unsigned)(prow * a.groups + ((i0 + 8 * pc) >> 5)) : NOWHERE;
+    struct Staged { b8 a[4]; vdmi_u2 b[4]; unsigned e[4]; } ra, rb;
     float bias[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) bias[e] = 0.f;
-    auto load = [&](long long r0) {
+    auto load = [&](Staged& v, long long r0) {
+        const unsigned n = (unsigned)max(min(r_end - r0, (long long)WK), 0ll);
+        const auto da = vdmi_rsrc(a.dy + r0 * a.lddy, n * (unsigned)a.lddy * 2), db = vdmi_rsrc(a.codes + r0 * a.cin, n * a.cin),
+                   de = vdmi_rsrc(a.exps + r0 * a.groups, n * a.groups);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const long long r = r0 + prow + 16 * j;
-            const bool in = r < r_end;
-            va[j] = a_on && in ? *reinterpret_cast<const b8*>(a.dy + r * a.lddy + o0 + 8 * pc) : zero8;
-            vb[j] = make_uint2(0, 0);
-            ve[j] = 0;
-            if (b_on && in) {
-                vb[j] = *reinterpret_cast<const uint2*>(a.codes + r * a.cin + i0 + 8 * pc);
-                ve[j] = a.exps[r * a.groups + ((i0 + 8 * pc) >> 5)];
-            }
+            v.a[j] = load16<__bf16>(da, aoff + 32 * j * (unsigned)a.lddy);
+            v.b[j] = __builtin_amdgcn_raw_buffer_load_b64(db, boff + 16 * j * a.cin, 0, 0);
+            v.e[j] = __builtin_amdgcn_raw_buffer_load_b8(de, eoff + 16 * j * a.groups, 0, 0);
         }
     };
-    auto store = [&](int buf) {
-        char* la = lds + buf * (2 * WK * WPITCH);
-        char* lb = la + WK * WPITCH;
+    const bool sums = a.bpart && it == 0;
+    auto store = [&](const Staged& v, int buf, int j) {
+        char* la = lds + buf * (2 * WK * WPITCH) + (prow + 16 * j) * WPITCH + 16 * pc;
+        *reinterpret_cast<b8*>(la) = v.a[j];
+        *reinterpret_cast<b8*>(la + WK * WPITCH) = widen8_bf16(v.b[j], v.e[j]);
+    };
+    auto add_bias = [&](const Staged& v) {
+        if (sums) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            *reinterpret_cast<b8*>(la + (prow + 16 * j) * WPITCH + 16 * pc) = va[j];
-            float v[8];
-            widen8(v, vb[j], ve[j]);
-            b8 x;
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = (__bf16)v[e];
-            *reinterpret_cast<b8*>(lb + (prow + 16 * j) * WPITCH + 16 * pc) = x;
-            if (a.bpart && it == 0) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) bias[e] += (float)va[j][e];
-            }
+                for (int e = 0; e < 8; ++e) bias[e] += (float)v.a[j][e];
         }
     };
     const int g16 = lane >> 4, tq = (lane >> 2) & 3, tp = lane & 3;
@@ -190,32 +192,49 @@ __global__ __launch_bounds__(256, 2) void rows8_wgrad_kernel(const Wgrad8Args a)
     for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int n = 0; n < 2; ++n) acc[m][n] = zero16();
-    int cur = 0;
-    if (r_begin < r_end) {
-        load(r_begin);
-        store(0);
-        __syncthreads();
-        for (long long r0 = r_begin; r0 < r_end; r0 += WK) {
-            const bool more = r0 + WK < r_end;
-            if (more) load(r0 + WK);
-            const char* ta = lds + cur * (2 * WK * WPITCH) + tr_off + 2 * wo;
-            const char* tb = lds + cur * (2 * WK * WPITCH) + WK * WPITCH + tr_off + 2 * wi;
+    // products of the stage in `buf`; the next one's pieces go into the other buffer between them.  The order is held: loads
+    // first (they need the whole stage), then every step's fragments ahead of the products before it.
+    auto stage = [&](int buf, const Staged& next) {
+        const char* ta = lds + buf * (2 * WK * WPITCH) + tr_off + 2 * wo;
+        const char* tb = lds + buf * (2 * WK * WPITCH) + WK * WPITCH + tr_off + 2 * wi;
+        b8 A[2][2], B[2][2];
+        auto fragments = [&](int ks) {
 #pragma unroll
-            for (int ks = 0; ks < WK / 16; ++ks) {
-                b8 A[2], B[2];
-#pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    A[m] = tr_operand<__bf16>(ta + ks * 16 * WPITCH + 64 * m, 4 * WPITCH);
-                    B[m] = tr_operand<__bf16>(tb + ks * 16 * WPITCH + 64 * m, 4 * WPITCH);
-                }
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) acc[m][n] = mfma16(A[m], B[n], acc[m][n]);
+            for (int m = 0; m < 2; ++m) {
+                A[ks & 1][m] = tr_operand<__bf16>(ta + ks * 16 * WPITCH + 64 * m, 4 * WPITCH);
+                B[ks & 1][m] = tr_operand<__bf16>(tb + ks * 16 * WPITCH + 64 * m, 4 * WPITCH);
             }
-            if (more) store(cur ^ 1);
-            __syncthreads();
-            cur ^= 1;
+        };
+        __builtin_amdgcn_sched_barrier(0);
+        fragments(0);
+#pragma unroll
+        for (int ks = 0; ks < WK / 16; ++ks) {
+            if (ks + 1 < WK / 16) fragments(ks + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) acc[m][n] = mfma16(A[ks & 1][m], B[ks & 1][n], acc[m][n]);
+            store(next, buf ^ 1, ks);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        add_bias(next);
+        __syncthreads();
+    };
+    // two stages' rows are in flight in registers while a third is multiplied from LDS: one stage's products take less time
+    // than its loads.  Loads past the share's end are zeros.
+    if (r_begin < r_end) {
+        load(ra, r_begin);
+        load(rb, r_begin + WK);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) store(ra, 0, j);
+        add_bias(ra);
+        __syncthreads();
+        for (long long r0 = r_begin; r0 < r_end; r0 += 2 * WK) {
+            load(ra, r0 + 2 * WK);
+            stage(0, rb);
+            load(rb, r0 + 3 * WK);
+            stage(1, ra);
         }
     }
     float* part = a.part + ((split * a.to + ot) * a.ti + it) * (long long)(WT * WT);
@@ -266,12 +285,19 @@ int wgrad8_plan(int cin, int cout, int64_t rows, Wgrad8Plan* p) {
     p->to = (cout + WT - 1) / WT;
     p->ti = (cin + WT - 1) / WT;
     const long long tiles = (long long)p->to * p->ti, stages = (rows + WK - 1) / WK;
-    // two workgroups per CU (80 KB of LDS each)
-    long long splits = (512 + tiles - 1) / tiles;
-    if (splits > stages) splits = stages;
+    // Shares of the rows: 1, 2, 4 or a multiple of 8 (whole XCDs).  512 workgroups run at once (80 KB of LDS each); a stage
+    // takes WSTAGE of a microsecond, a share's partial sums 128 KB of traffic per tile.
+    long long splits = 1;
+    double best = 1e30;
+    for (long long k = 1; k <= 128 && k <= stages; k += k < 2 ? 1 : k < 4 ? 2 : k < 8 ? 4 : 8) {
+        const long long per = (stages + k - 1) / k;
+        const long long rounds = k % 8 ? (tiles * k + 511) / 512 : (tiles * (k / 8) + 63) / 64;
+        const double us = rounds * per * WSTAGE_US + 128e3 * tiles * k / 4e6;
+        if (us < best) { best = us; splits = k; }
+    }
     const long long per = (stages + splits - 1) / splits;
     p->per = per * WK;
-    p->splits = (int)((stages + per - 1) / per);
+    p->splits = (int)splits;            // the last ones may be empty: a multiple of 8 stays one
     if (tiles * p->splits > 0x7fffffffLL) return VDMI_E_SHAPE;
     p->part = (size_t)tiles * p->splits * WT * WT * sizeof(float);
     p->bytes = p->part + (size_t)p->splits * p->to * WT * sizeof(float);
@@ -331,7 +357,7 @@ extern "C" int vdmi_rows8_wgrad(const void* codes, const void* exps, const void*
     Wgrad8Plan p;
     const int ok = wgrad8_plan(cin, cout, rows, &p);
     if (ok != VDMI_OK) return ok;
-    if (lddy < cout || lddy % 8) return VDMI_E_SHAPE;
+    if (lddy < cout || lddy % 8 || lddy > VDMI_ROWS8_MAX_PITCH) return VDMI_E_SHAPE;
     if (!aligned16(dy) || !aligned16(dw) || !aligned16(workspace) || (reinterpret_cast<uintptr_t>(codes) & 7u)) return VDMI_E_ALIGN;
     const int lds = 4 * WK * WPITCH;
     if (vdmi_set_max_lds(reinterpret_cast<const void*>(&rows8_wgrad_kernel), g_wgrad8_lds, lds) != 0) return VDMI_E_LDS;
@@ -342,7 +368,7 @@ extern "C" int vdmi_rows8_wgrad(const void* codes, const void* exps, const void*
     a.part = static_cast<float*>(workspace);
     a.bpart = db ? a.part + p.part / sizeof(float) : nullptr;
     a.lddy = lddy; a.rows = rows; a.per = p.per;
-    a.cin = cin; a.cout = cout; a.groups = (cin + 31) / 32; a.to = p.to; a.ti = p.ti;
+    a.cin = cin; a.cout = cout; a.groups = (cin + 31) / 32; a.to = p.to; a.ti = p.ti; a.splits = p.splits;
     hipLaunchKernelGGL(rows8_wgrad_kernel, dim3((unsigned)(p.to * p.ti * p.splits)), dim3(256), lds, st, a);
     VDMI_LAUNCH_CHECK();
     const long long quads = (long long)p.to * p.ti * WT * WT / 4;
