@@ -16,6 +16,7 @@ fallback: tensors that are not on a GPU and shapes that the kernels do not take 
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -25,25 +26,26 @@ from .train_hip import _plain
 
 _DTYPES = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16, torch.float32: _lib.DT_F32}
 _FLOAT16S = (torch.bfloat16, torch.float16)
+_I64x8 = C.c_int64 * 8
 
 
-class _on_device:
-    """`with _on_device(t) as stream:` - t's device is the current one inside, stream its current stream's handle."""
-    __slots__ = ("index", "prev")
+_current_device, _raw_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
 
-    def __init__(self, t: torch.Tensor):
-        self.index = t.device.index
 
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
+def _stream_of(t: torch.Tensor) -> int:
+    """The handle of the current stream of t's device, which has to be the current one (_there)."""
+    return _raw_stream(t.device.index)
 
-    def __exit__(self, *exc):
-        if self.prev != self.index:
-            torch.cuda.set_device(self.prev)
-        return False
+
+def _there(fn):
+    """fn(t, ...) with t's device as the current one."""
+    @functools.wraps(fn)
+    def inner(t, *args):
+        if t.device.index == _current_device():
+            return fn(t, *args)
+        with torch.cuda.device(t.device):
+            return fn(t, *args)
+    return inner
 
 
 def _on_gpu(first, *ts):
@@ -91,25 +93,16 @@ def _empty_like_rows(t: torch.Tensor) -> torch.Tensor:
     return t.new_empty_strided(shape, strides)
 
 
-def _set_rows(r: "_lib.Rows4", t: torch.Tensor):
-    r.p = t.data_ptr()
-    r.b, r.i, r.n, r.h, _ = t.stride()
+_NO_ROWS = _lib.Rows4()
 
 
-def _decay_args(q, k, v, log_decay, lengths, state, scale) -> "_lib.DecayArgs":
-    a = _lib.DecayArgs()
-    a.dtype = _DTYPES[q.dtype]
-    a.b, a.inner, a.n, a.heads, a.d = q.shape
-    a.scale = scale
-    _set_rows(a.q, q)
-    _set_rows(a.k, k)
-    _set_rows(a.v, v)
-    a.log_decay, a.lengths, a.state_in = log_decay.data_ptr(), _ptr(lengths), _ptr(state)
-    return a
+def _rows4(t: torch.Tensor) -> "_lib.Rows4":
+    s = t.stride()
+    return _lib.Rows4(t.data_ptr(), s[0], s[1], s[2], s[3])
 
 
 def _decay_workspace(a, like):
-    size = _lib.lib().vdmi_decay_attn_workspace_bytes(C.byref(a))
+    size = _lib.lib().vdmi_decay_attn_workspace_bytes(a)
     if not size:
         return None
     ws = torch.empty(size, device=like.device, dtype=torch.uint8)
@@ -117,20 +110,33 @@ def _decay_workspace(a, like):
     return ws
 
 
+@_there
 def _decay_forward(q, k, v, state, log_decay, lengths, scale, return_state):
     """(o, last state or None, the workspace) of operands as the kernels read them."""
-    with _on_device(q) as stream:
-        o = _empty_like_rows(q)
-        last = None
-        a = _decay_args(q, k, v, log_decay, lengths, state, scale)
-        _set_rows(a.o, o)
-        if return_state:
-            b, inner, _, h, d = q.shape
-            last = torch.empty((b, inner, h, d, d), device=q.device, dtype=torch.float32)
-            a.state_out = last.data_ptr()
-        ws = _decay_workspace(a, q)
-        check(_lib.lib().vdmi_decay_attn_fwd(C.byref(a), stream), "vdmi_decay_attn_fwd")
+    b, inner, n, h, d = q.shape
+    o = _empty_like_rows(q)
+    last = torch.empty((b, inner, h, d, d), device=q.device, dtype=torch.float32) if return_state else None
+    a = _lib.DecayArgs(_DTYPES[q.dtype], b, inner, n, h, d, scale, 0, _rows4(q), _rows4(k), _rows4(v), _rows4(o),
+                       _NO_ROWS, _NO_ROWS, _NO_ROWS, _NO_ROWS, log_decay.data_ptr(), _ptr(lengths), _ptr(state), _ptr(last))
+    ws = _decay_workspace(a, q)
+    check(_lib.lib().vdmi_decay_attn_fwd(a, _stream_of(q)), "vdmi_decay_attn_fwd")
     return o, last, ws
+
+
+@_there
+def _decay_backward(q, k, v, state, log_decay, lengths, fwd_ws, scale, do, dlast, want_dstate):
+    do = torch.zeros_like(q) if do is None else _row_operand(do if do.dtype == q.dtype else do.to(q.dtype))
+    if dlast is not None:
+        dlast = dlast.to(torch.float32).contiguous()
+    dq, dk, dv = _empty_like_rows(q), _empty_like_rows(k), _empty_like_rows(v)
+    dstate = torch.empty_like(state) if want_dstate else None
+    b, inner, n, h, d = q.shape
+    a = _lib.DecayArgs(_DTYPES[q.dtype], b, inner, n, h, d, scale, 0, _rows4(q), _rows4(k), _rows4(v), _NO_ROWS,
+                       _rows4(do), _rows4(dq), _rows4(dk), _rows4(dv), log_decay.data_ptr(), _ptr(lengths), _ptr(state), None,
+                       _ptr(dlast), _ptr(dstate), None, 0, _ptr(fwd_ws))
+    ws = _decay_workspace(a, q)
+    check(_lib.lib().vdmi_decay_attn_bwd(a, _stream_of(q)), "vdmi_decay_attn_bwd")
+    return dq, dk, dv, dstate
 
 
 class DecayAttnFn(torch.autograd.Function):
@@ -148,26 +154,10 @@ class DecayAttnFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, do, dlast):
-        q, k, v, state, log_decay, lengths, fwd_ws = ctx.saved_tensors
-        need = ctx.needs_input_grad
         if do is None and dlast is None:
             return (None,) * 8
-        with _on_device(q) as stream:
-            do = torch.zeros_like(q) if do is None else _row_operand(do.to(q.dtype))
-            dlast = None if dlast is None else dlast.to(torch.float32).contiguous()
-            dq, dk, dv = _empty_like_rows(q), _empty_like_rows(k), _empty_like_rows(v)
-            a = _decay_args(q, k, v, log_decay, lengths, state, ctx.scale)
-            _set_rows(a.dout, do)
-            _set_rows(a.dq, dq)
-            _set_rows(a.dk, dk)
-            _set_rows(a.dv, dv)
-            dstate = None
-            if need[3]:
-                dstate = torch.empty_like(state)
-                a.dstate_out = dstate.data_ptr()
-            a.dstate_in, a.fwd_workspace = _ptr(dlast), _ptr(fwd_ws)
-            ws = _decay_workspace(a, q)
-            check(_lib.lib().vdmi_decay_attn_bwd(C.byref(a), stream), "vdmi_decay_attn_bwd")
+        need = ctx.needs_input_grad
+        dq, dk, dv, dstate = _decay_backward(*ctx.saved_tensors, ctx.scale, do, dlast, need[3])
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dstate, None, None, None, None)
 
 
@@ -264,13 +254,22 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
         return o
     if q.dim() != 3:
         q, k, v = q.reshape(-1, heads, d), k.reshape(-1, heads, d), v.reshape(-1, heads, d)
-    q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
-    strides = (C.c_int64 * 8)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], heads * d, d)
-    with _on_device(q) as stream:
-        check(_lib.lib().vdmi_decay_attn_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), strides,
-                                              log_decay.contiguous().data_ptr(), state.data_ptr(), _DTYPES[q.dtype], q.shape[0],
-                                              heads, d, scale, stream), "vdmi_decay_attn_step")
+    (qb, qh, q1), (kb, kh, k1), (vb, vh, v1) = q.stride(), k.stride(), v.stride()
+    if q1 != 1 or k1 != 1 or v1 != 1:
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+        qb = kb = vb = heads * d
+        qh = kh = vh = d
+    strides = _I64x8(qb, qh, kb, kh, vb, vh, heads * d, d)
+    _decay_step(q, k, v, o, strides, log_decay.contiguous(), state, scale)
     return o
+
+
+@_there
+def _decay_step(q, k, v, o, strides, log_decay, state, scale):
+    seqs, heads, d = q.shape
+    check(_lib.lib().vdmi_decay_attn_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), strides, log_decay.data_ptr(),
+                                          state.data_ptr(), _DTYPES[q.dtype], seqs, heads, d, scale, _stream_of(q)),
+          "vdmi_decay_attn_step")
 
 
 # ---------------------------------------------------------------------------------------------------------------------
@@ -279,11 +278,61 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
 def _rows2(t: torch.Tensor) -> torch.Tensor:
     """t [..., c] as [rows][c] with contiguous columns: a view where the rows have one pitch, else a copy."""
     r = t.reshape(-1, t.shape[-1])
-    return r if r.stride(1) == 1 and (r.shape[0] == 1 or r.stride(0) >= r.shape[1]) else r.contiguous()
+    rows, c = r.shape
+    pitch, one = r.stride()
+    return r if one == 1 and (rows == 1 or pitch >= c) else r.contiguous()
 
 
 def _pitch(r: torch.Tensor) -> int:
     return r.stride(0) if r.shape[0] > 1 else r.shape[1]
+
+
+def _stride_of(p, c: int) -> int:
+    return c if p is not None and p.dim() == 2 and p.shape[0] > 1 else 0
+
+
+@_there
+def _norm_forward(xr, hr, pw, gate, w, scale, shift, shape, alpha, kind, post_kind, eps, want_y):
+    """(out, y) of rows xr, hr [rows][c] and contiguous parameters."""
+    out = None if hr is None else xr.new_empty(shape)
+    y = xr.new_empty(shape) if want_y else None
+    rows, c = xr.shape
+    a = _lib.BlockNormArgs(
+        _DTYPES[xr.dtype], c, _lib.NORM_KINDS[kind], _lib.NORM_KINDS[post_kind], rows, rows // shape[0], eps, alpha,
+        xr.data_ptr(), _ptr(hr), _ptr(out), _ptr(y), None, None, None, None,
+        _pitch(xr), c if hr is None else _pitch(hr), c, c, c, c, c, c,
+        _ptr(pw), _ptr(gate), _ptr(w), _ptr(scale), _ptr(shift), _stride_of(gate, c), _stride_of(scale, c), _stride_of(shift, c))
+    check(_lib.lib().vdmi_block_norm_fwd(a, _stream_of(xr)), "vdmi_block_norm_fwd")
+    return out, y
+
+
+@_there
+def _norm_backward(xr, hr, pw, gate, w, scale, shift, shape, alpha, kind, post_kind, eps, need, dout, dy):
+    rows, c = xr.shape
+    if dout is not None:
+        dout = _rows2(dout if dout.dtype == xr.dtype else dout.to(xr.dtype))
+    if dy is not None:
+        dy = _rows2(dy if dy.dtype == xr.dtype else dy.to(xr.dtype))
+    dx = xr.new_empty(shape) if need[0] else None
+    dh = xr.new_empty(shape) if need[1] else None
+    # without dy nothing is learnt about the second norm's parameters
+    like = torch.empty_like if dy is not None else torch.zeros_like
+    dpw, dgate = torch.empty_like(pw) if need[2] else None, torch.empty_like(gate) if need[3] else None
+    dw, dscale, dshift = like(w) if need[4] else None, like(scale) if need[5] else None, like(shift) if need[6] else None
+    on = dy is not None
+    a = _lib.BlockNormArgs(
+        _DTYPES[xr.dtype], c, _lib.NORM_KINDS[kind], _lib.NORM_KINDS[post_kind], rows, rows // shape[0], eps, alpha,
+        xr.data_ptr(), _ptr(hr), None, None, _ptr(dout), _ptr(dy), _ptr(dx), _ptr(dh),
+        _pitch(xr), c if hr is None else _pitch(hr), c, c, c if dout is None else _pitch(dout), _pitch(dy) if on else c, c, c,
+        _ptr(pw), _ptr(gate), _ptr(w), _ptr(scale), _ptr(shift), _stride_of(gate, c), _stride_of(scale, c), _stride_of(shift, c),
+        _ptr(dpw), _ptr(dgate), _ptr(dw) if on else None, _ptr(dscale) if on else None, _ptr(dshift) if on else None)
+    lib = _lib.lib()
+    size = lib.vdmi_block_norm_bwd_workspace_bytes(a)
+    if size:
+        ws = torch.empty(size, device=xr.device, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), size
+    check(lib.vdmi_block_norm_bwd(a, _stream_of(xr)), "vdmi_block_norm_bwd")
+    return dx, dh, dpw, dgate, dw, dscale, dshift
 
 
 class BlockNormFn(torch.autograd.Function):
@@ -291,66 +340,25 @@ class BlockNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, h, post_weight, gate, weight, scale, shift, alpha, kind, post_kind, eps, want_y):
-        params = [None if p is None else p.contiguous() for p in (post_weight, gate, weight, scale, shift)]
-        xr, hr = _rows2(x), None if h is None else _rows2(h)
-        out, y = _norm_forward(x, xr, hr, params, alpha, kind, post_kind, eps, want_y)
-        ctx.save_for_backward(xr, hr, *params)
-        ctx.meta = (tuple(x.shape), alpha, kind, post_kind, eps)
+        ops = _norm_operands(x, h, post_weight, gate, weight, scale, shift)
+        shape = x.shape
+        out, y = _norm_forward(*ops, shape, alpha, kind, post_kind, eps, want_y)
+        ctx.save_for_backward(*ops)
+        ctx.meta = (shape, alpha, kind, post_kind, eps)
         ctx.set_materialize_grads(False)
         return out, y
 
     @staticmethod
     def backward(ctx, dout, dy):
-        xr, hr, *params = ctx.saved_tensors
-        shape, alpha, kind, post_kind, eps = ctx.meta
-        need = ctx.needs_input_grad
         if dout is None and dy is None:
             return (None,) * 12
-        with _on_device(xr) as stream:
-            dout, dy = (None if g is None else _rows2(g.to(xr.dtype)) for g in (dout, dy))
-            dx = torch.empty(shape, device=xr.device, dtype=xr.dtype) if need[0] else None
-            dh = torch.empty(shape, device=xr.device, dtype=xr.dtype) if need[1] else None
-            grads = [torch.empty_like(p) if n and p is not None else None for n, p in zip(need[2:7], params)]
-            if dy is None:              # nothing is learnt about the second norm's parameters
-                grads[2:] = [None if g is None else g.zero_() for g in grads[2:]]
-            a = _norm_args(xr, hr, params, shape[0], alpha, kind, post_kind, eps)
-            a.dout, a.dy, a.dx, a.dh = _ptr(dout), _ptr(dy), _ptr(dx), _ptr(dh)
-            a.lddo, a.lddy = (shape[-1] if g is None else _pitch(g) for g in (dout, dy))
-            a.lddx = a.lddh = shape[-1]
-            a.dpost_weight, a.dgate = _ptr(grads[0]), _ptr(grads[1])
-            if dy is not None:
-                a.dweight, a.dscale, a.dshift = (_ptr(g) for g in grads[2:])
-            lib = _lib.lib()
-            a.workspace_bytes = lib.vdmi_block_norm_bwd_workspace_bytes(C.byref(a))
-            ws = torch.empty(a.workspace_bytes, device=xr.device, dtype=torch.uint8) if a.workspace_bytes else None
-            a.workspace = _ptr(ws)
-            check(lib.vdmi_block_norm_bwd(C.byref(a), stream), "vdmi_block_norm_bwd")
-        return (dx, dh, *grads, None, None, None, None, None)
+        return (*_norm_backward(*ctx.saved_tensors, *ctx.meta, ctx.needs_input_grad, dout, dy), None, None, None, None, None)
 
 
-def _norm_forward(x, xr, hr, params, alpha, kind, post_kind, eps, want_y):
-    with _on_device(xr) as stream:
-        out = None if hr is None else torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        y = torch.empty(x.shape, device=x.device, dtype=x.dtype) if want_y else None
-        a = _norm_args(xr, hr, params, x.shape[0], alpha, kind, post_kind, eps)
-        a.out, a.y = _ptr(out), _ptr(y)
-        a.ldo = a.ldy = x.shape[-1]
-        check(_lib.lib().vdmi_block_norm_fwd(C.byref(a), stream), "vdmi_block_norm_fwd")
-    return out, y
-
-
-def _norm_args(xr, hr, params, samples, alpha, kind, post_kind, eps) -> "_lib.BlockNormArgs":
-    a = _lib.BlockNormArgs()
-    a.dtype, a.c, a.kind, a.post_kind = _DTYPES[xr.dtype], xr.shape[1], _lib.NORM_KINDS[kind], _lib.NORM_KINDS[post_kind]
-    a.rows, a.rows_per_sample = xr.shape[0], xr.shape[0] // samples
-    a.eps, a.alpha = eps, alpha
-    a.x, a.ldx = xr.data_ptr(), _pitch(xr)
-    if hr is not None:
-        a.h, a.ldh = hr.data_ptr(), _pitch(hr)
-    a.post_weight, a.gate, a.weight, a.scale, a.shift = (_ptr(p) for p in params)
-    a.gate_stride, a.scale_stride, a.shift_stride = (
-        a.c if p is not None and p.dim() == 2 and p.shape[0] > 1 else 0 for p in (params[1], params[3], params[4]))
-    return a
+def _norm_operands(x, h, pw, gate, w, scale, shift):
+    return (_rows2(x), None if h is None else _rows2(h), None if pw is None else pw.contiguous(),
+            None if gate is None else gate.contiguous(), None if w is None else w.contiguous(),
+            None if scale is None else scale.contiguous(), None if shift is None else shift.contiguous())
 
 
 def _block_norm(x, h, post_weight, gate, weight, scale, shift, alpha, kind, post_kind, eps, want_y):
@@ -362,12 +370,13 @@ def _block_norm(x, h, post_weight, gate, weight, scale, shift, alpha, kind, post
     if h is not None and not (h.dtype == x.dtype and h.shape == x.shape):
         raise VdmiError(f"x and h are alike (got {x.dtype} {tuple(x.shape)}, {h.dtype} {tuple(h.shape)})")
     b, c = x.shape[0], x.shape[-1]
-    for name, p in (("post_weight", post_weight), ("weight", weight)):
-        if p is not None and not (p.dtype == torch.float32 and p.shape == (c,)):
-            raise VdmiError(f"{name} is float32 [{c}]")
-    for name, p in (("gate", gate), ("scale", scale), ("shift", shift)):
-        if p is not None and not (p.dtype == torch.float32 and (p.shape == (b, c) or p.shape == (c,) or p.shape == (1, c))):
-            raise VdmiError(f"{name} is float32 [{c}], [1, {c}] or [{b}, {c}]")
+    row, one, rows, f32 = (c,), (1, c), (b, c), torch.float32
+    for p in (post_weight, weight):
+        if p is not None and not (p.dtype is f32 and p.shape == row):
+            raise VdmiError(f"{'weight' if p is weight else 'post_weight'} is float32 [{c}]")
+    for p in (gate, scale, shift):
+        if p is not None and not (p.dtype is f32 and (p.shape == rows or p.shape == row or p.shape == one)):
+            raise VdmiError(f"{'gate' if p is gate else 'scale' if p is scale else 'shift'} is float32 [{c}], [1, {c}] or [{b}, {c}]")
     if kind not in ("rms", "layer"):
         raise VdmiError(f"kind is 'rms' or 'layer' (got {kind!r})")
     if post_kind not in ("rms", "layer", None):
@@ -379,8 +388,7 @@ def _block_norm(x, h, post_weight, gate, weight, scale, shift, alpha, kind, post
         return (None if h is None else x + h), (x * 1 if want_y else None)
     if _wants_grad(x, h, post_weight, gate, weight, scale, shift):
         return BlockNormFn.apply(x, h, post_weight, gate, weight, scale, shift, alpha, kind, post_kind, eps, want_y)
-    params = [None if p is None else p.contiguous() for p in (post_weight, gate, weight, scale, shift)]
-    return _norm_forward(x, _rows2(x), None if h is None else _rows2(h), params, alpha, kind, post_kind, eps, want_y)
+    return _norm_forward(*_norm_operands(x, h, post_weight, gate, weight, scale, shift), x.shape, alpha, kind, post_kind, eps, want_y)
 
 
 def norm_before(x, weight=None, scale=None, shift=None, *, kind="rms", eps=1e-5):
@@ -422,11 +430,44 @@ class Rows8:
             raise VdmiError(f"rows are bfloat16, float16 or float32 (got {dtype})")
         out = torch.empty(self.shape, device=self.codes.device, dtype=dtype)
         if out.numel():
-            rows, c = self.codes.shape
-            with _on_device(out) as stream:
-                check(_lib.lib().vdmi_rows8_unpack(self.codes.data_ptr(), self.exps.data_ptr(), out.data_ptr(), c, _DTYPES[dtype],
-                                                   rows, c, stream), "vdmi_rows8_unpack")
+            _unpack(self.codes, self.exps, out)
         return out
+
+
+@_there
+def _unpack(codes, exps, out):
+    rows, c = codes.shape
+    check(_lib.lib().vdmi_rows8_unpack(codes.data_ptr(), exps.data_ptr(), out.data_ptr(), c, _DTYPES[out.dtype], rows, c,
+                                       _stream_of(out)), "vdmi_rows8_unpack")
+
+
+@_there
+def _pack(x):
+    r = _aligned_rows(x)
+    rows, c = r.shape
+    codes = torch.empty((rows, c), device=x.device, dtype=torch.uint8)
+    exps = torch.empty((rows, (c + 31) // 32), device=x.device, dtype=torch.uint8)
+    if rows:
+        check(_lib.lib().vdmi_rows8_pack(r.data_ptr(), _pitch(r), codes.data_ptr(), exps.data_ptr(), _DTYPES[x.dtype], rows, c,
+                                         _stream_of(x)), "vdmi_rows8_pack")
+    return Rows8(codes, exps, tuple(x.shape), x.dtype)
+
+
+@_there
+def _wgrad(dy, kept, bias):
+    rows, cin = kept.codes.shape
+    cout = dy.shape[-1]
+    if rows == 0:
+        dw, db = torch.zeros(cout, cin, device=dy.device), torch.zeros(cout, device=dy.device)
+        return (dw, db) if bias else dw
+    d = _aligned_rows(dy)
+    lib = _lib.lib()
+    dw = torch.empty((cout, cin), device=dy.device, dtype=torch.float32)
+    db = torch.empty(cout, device=dy.device, dtype=torch.float32) if bias else None
+    ws = torch.empty(lib.vdmi_rows8_wgrad_workspace_bytes(cin, cout, rows), device=dy.device, dtype=torch.uint8)
+    check(lib.vdmi_rows8_wgrad(kept.codes.data_ptr(), kept.exps.data_ptr(), d.data_ptr(), _pitch(d), dw.data_ptr(), _ptr(db),
+                               cin, cout, rows, ws.data_ptr(), _stream_of(dy)), "vdmi_rows8_wgrad")
+    return (dw, db) if bias else dw
 
 
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
@@ -444,15 +485,7 @@ def pack_rows8(x: torch.Tensor) -> Rows8:
         raise VdmiError(f"rows are bfloat16, float16 or float32 (got {x.dtype})")
     if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 8:
         raise VdmiError(f"rows of a multiple of 8 channels (got {tuple(x.shape)})")
-    with _on_device(x) as stream:
-        r = _aligned_rows(x)
-        rows, c = r.shape
-        codes = torch.empty((rows, c), device=x.device, dtype=torch.uint8)
-        exps = torch.empty((rows, (c + 31) // 32), device=x.device, dtype=torch.uint8)
-        if rows:
-            check(_lib.lib().vdmi_rows8_pack(r.data_ptr(), _pitch(r), codes.data_ptr(), exps.data_ptr(), _DTYPES[x.dtype], rows, c,
-                                             stream), "vdmi_rows8_pack")
-    return Rows8(codes, exps, tuple(x.shape), x.dtype)
+    return _pack(x)
 
 
 def rows8_wgrad(kept: Rows8, dy: torch.Tensor, bias: bool = False):
@@ -467,18 +500,7 @@ def rows8_wgrad(kept: Rows8, dy: torch.Tensor, bias: bool = False):
         raise VdmiError(f"a multiple of 8 output channels (got {cout})")
     if dy.numel() != rows * cout:
         raise VdmiError(f"dy has a row for each of the {rows} kept rows (got {tuple(dy.shape)})")
-    with _on_device(dy) as stream:
-        if rows == 0:
-            dw, db = torch.zeros(cout, cin, device=dy.device), torch.zeros(cout, device=dy.device)
-            return (dw, db) if bias else dw
-        d = _aligned_rows(dy)
-        lib = _lib.lib()
-        dw = torch.empty((cout, cin), device=dy.device, dtype=torch.float32)
-        db = torch.empty(cout, device=dy.device, dtype=torch.float32) if bias else None
-        ws = torch.empty(lib.vdmi_rows8_wgrad_workspace_bytes(cin, cout, rows), device=dy.device, dtype=torch.uint8)
-        check(lib.vdmi_rows8_wgrad(kept.codes.data_ptr(), kept.exps.data_ptr(), d.data_ptr(), _pitch(d), dw.data_ptr(), _ptr(db),
-                                   cin, cout, rows, ws.data_ptr(), stream), "vdmi_rows8_wgrad")
-    return (dw, db) if bias else dw
+    return _wgrad(dy, kept, bias)
 
 
 class LinearRows8Fn(torch.autograd.Function):
@@ -487,33 +509,40 @@ class LinearRows8Fn(torch.autograd.Function):
     @staticmethod
     @_plain
     def forward(ctx, x, weight, bias):
-        from .train_hip import _linear_pack, conv_rows
-        with _on_device(x):
-            xr = x.reshape(-1, x.shape[-1]).contiguous()
-            y = conv_rows(xr, _linear_pack(weight.detach(), False), None if bias is None else bias.detach().float().contiguous(),
-                          1, 1, 1, xr.shape[0])
-            kept = pack_rows8(xr) if ctx.needs_input_grad[1] else None
+        y, kept = _linear(x, weight, bias, ctx.needs_input_grad[1])
         ctx.save_for_backward(weight, *((kept.codes, kept.exps) if kept else ()))
         ctx.shape = tuple(x.shape)
-        return y.view(*x.shape[:-1], weight.shape[0])
+        return y
 
     @staticmethod
     @_plain
     def backward(ctx, dy):
-        from .train_hip import _linear_pack, conv_rows
         weight, *kept = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx = dw = db = None
-        with _on_device(dy):
-            d = dy.to(torch.bfloat16).reshape(-1, dy.shape[-1]).contiguous()
-            if need[0]:
-                dx = conv_rows(d, _linear_pack(weight.detach(), True), None, 1, 1, 1, d.shape[0]).view(ctx.shape)
-            if need[1]:
-                dw = rows8_wgrad(Rows8(*kept, ctx.shape, torch.bfloat16), d, bias=need[2])
-                dw, db = dw if need[2] else (dw, None)
-            elif need[2]:
-                db = d.float().sum(0)
-        return dx, dw, db
+        return _linear_backward(dy, weight, kept, ctx.shape, ctx.needs_input_grad)
+
+
+@_there
+def _linear(x, weight, bias, keep):
+    from .train_hip import _linear_pack, conv_rows
+    xr = x.reshape(-1, x.shape[-1]).contiguous()
+    y = conv_rows(xr, _linear_pack(weight.detach(), False), None if bias is None else bias.detach().float().contiguous(),
+                  1, 1, 1, xr.shape[0])
+    return y.view(*x.shape[:-1], weight.shape[0]), pack_rows8(xr) if keep else None
+
+
+@_there
+def _linear_backward(dy, weight, kept, shape, need):
+    from .train_hip import _linear_pack, conv_rows
+    dx = dw = db = None
+    d = dy.to(torch.bfloat16).reshape(-1, dy.shape[-1]).contiguous()
+    if need[0]:
+        dx = conv_rows(d, _linear_pack(weight.detach(), True), None, 1, 1, 1, d.shape[0]).view(shape)
+    if need[1]:
+        dw = rows8_wgrad(Rows8(*kept, shape, torch.bfloat16), d, bias=need[2])
+        dw, db = dw if need[2] else (dw, None)
+    elif need[2]:
+        db = d.float().sum(0)
+    return dx, dw, db
 
 
 def linear_rows8(x: torch.Tensor, weight: torch.Tensor, bias=None) -> torch.Tensor:
