@@ -458,6 +458,30 @@ def colsum_rows(x: torch.Tensor) -> torch.Tensor:
     return out
 
 
+_ROWS8 = False          # inside a rows8_checkpoints block
+
+
+class rows8_checkpoints:
+    """`with rows8_checkpoints():` around a forward - every ResnetBlock of it keeps what its backward needs of the
+    activations (its input, its hidden rows, both convolutions' outputs) as 8-bit codes with a power of two per 32 channels
+    (block_hip.pack_rows8) instead of bf16 rows: about half the memory, for gradients that see those rows rounded to 3
+    fraction bits.  Outputs are unchanged.  The backward widens a block's rows again when it gets there (the res_conv's
+    weight gradient reads the codes themselves)."""
+
+    def __init__(self, on: bool = True):
+        self.on = bool(on)
+
+    def __enter__(self):
+        global _ROWS8
+        self.prev, _ROWS8 = _ROWS8, self.on
+        return self
+
+    def __exit__(self, *exc):
+        global _ROWS8
+        _ROWS8 = self.prev
+        return False
+
+
 class ResnetBlockFn(torch.autograd.Function):
     """ResnetBlock.forward (vdp.py:442-452) with its backward; x float (B, Cin, F, H, W) -> float (B, Cout, F, H, W).
     scale / shift: float [B][Cout] (the chunks of the block's time MLP output) or None; wres / bres None = identity."""
@@ -490,7 +514,12 @@ class ResnetBlockFn(torch.autograd.Function):
         else:
             h2 = rmsnorm_silu_rows(y2, g2v, None, 0, f * hw)
             out = conv_rows(xr, param_pack(wres, False), bres.detach().float().contiguous(), frames, f, h, w, residual=h2)
-        ctx.save_for_backward(xr, y1, h1, y2, g1v, g2v, scale_c, shift_c, w1, w2, wres)
+        ctx.rows8 = _ROWS8
+        rows = (xr, y1, h1, y2)
+        if ctx.rows8:
+            from .block_hip import pack_rows8
+            rows = [t for r in rows for kept in (pack_rows8(r),) for t in (kept.codes, kept.exps)]
+        ctx.save_for_backward(g1v, g2v, scale_c, shift_c, w1, w2, wres, *rows)
         ctx.dims = (b, cin, cout, f, h, w)
         ctx.with_res = with_res
         ctx.act = _act_dtype(x)
@@ -499,22 +528,28 @@ class ResnetBlockFn(torch.autograd.Function):
     @staticmethod
     @_plain
     def backward(ctx, dout):
-        xr, y1, h1, y2, g1v, g2v, scale_c, shift_c, w1, w2, wres = ctx.saved_tensors
+        g1v, g2v, scale_c, shift_c, w1, w2, wres, *rows = ctx.saved_tensors
         b, cin, cout, f, h, w = ctx.dims
         frames, hw = b * f, h * w
+        if ctx.rows8:
+            from .block_hip import Rows8, rows8_wgrad
+            xr8, y18, h18, y28 = (Rows8(c, e, tuple(c.shape), torch.bfloat16) for c, e in zip(rows[::2], rows[1::2]))
+            xr, y1, h1, y2 = xr8.unpack, y18.unpack, h18.unpack, y28.unpack        # each widened where it is used
+        else:
+            xr, y1, h1, y2 = ((lambda r=r: r) for r in rows)
         do = to_rows(dout)
         # block2: SiLU / RMSNorm, then the conv
         # weight gradients only where asked for (a gradient with respect to the input alone - guidance at sampling time,
         # frozen weights - needs neither the transposes nor the contraction over pixels)
         need = ctx.needs_input_grad
-        dy2, dg2, db2, _, _ = rmsnorm_silu_bwd_rows(y2, do, g2v, None, None, b, f * hw)
+        dy2, dg2, db2, _, _ = rmsnorm_silu_bwd_rows(y2(), do, g2v, None, None, b, f * hw)
         dw2 = None
         if need[6]:
-            dw2 = conv3x3_wgrad(h1, dy2, frames, h, w)
+            dw2 = conv3x3_wgrad(h1(), dy2, frames, h, w)
         dh1 = conv_rows(dy2, param_pack(w2, True), None, frames, f, h, w)
         # block1
-        dy1, dg1, db1, dscale, dshift = rmsnorm_silu_bwd_rows(y1, dh1, g1v, scale_c, shift_c, b, f * hw)
-        dw1 = conv3x3_wgrad(xr, dy1, frames, h, w) if need[3] else None
+        dy1, dg1, db1, dscale, dshift = rmsnorm_silu_bwd_rows(y1(), dh1, g1v, scale_c, shift_c, b, f * hw)
+        dw1 = conv3x3_wgrad(xr(), dy1, frames, h, w) if need[3] else None
         # residual branch, then the input gradient: dgrad of conv1 + (res_conv's dgrad | the identity)
         if not ctx.with_res:
             dwres = dbres = dx_res = None
@@ -522,7 +557,9 @@ class ResnetBlockFn(torch.autograd.Function):
             dwres = dbres = None
             dx_res = do
         else:
-            dwres = rows_wgrad(xr, do).view(cout, cin, 1, 1, 1) if need[9] else None
+            dwres = None
+            if need[9]:
+                dwres = (rows8_wgrad(xr8, do) if ctx.rows8 else rows_wgrad(xr(), do)).view(cout, cin, 1, 1, 1)
             dbres = colsum_rows(do) if need[10] else None
             dx_res = conv_rows(do, param_pack(wres, True), None, frames, f, h, w)
         dx = conv_rows(dy1, param_pack(w1, True), None, frames, f, h, w, residual=dx_res)

@@ -239,6 +239,9 @@ class Trainer(object):
         # not a constructor argument (the reference's Trainer signature stays as it is): set the attribute, or the
         # environment variable VDMI_TRAIN_BACKEND, before train()
         self.train_backend = os.environ.get("VDMI_TRAIN_BACKEND", "torch-autograd")
+        # True: the ResnetBlocks on the HIP kernels keep their activations in 8 bits between forward and backward
+        # (train_hip.rows8_checkpoints): about half their memory, gradients that see the rows rounded
+        self.rows8_checkpoints = False
 
     @property
     def device(self):
@@ -326,11 +329,13 @@ class Trainer(object):
 
         # packed weight sets of the HIP layers: kept over the micro-steps of an accumulation, repacked (one launch) after
         # the optimizer step has moved the parameters' version counters
-        packs, store = _nullcontext, None
+        packs, store, keep = _nullcontext, None, _nullcontext
         if getattr(self.model.denoise_fn, "train_backend", None) in ("hip", "hip-resnet"):
             from . import train_hip
             store = train_hip.PackStore()
             packs = lambda: train_hip.fixed_weights(store)
+            if self.rows8_checkpoints:
+                keep = train_hip.rows8_checkpoints
 
         while self.step < self.train_num_steps:
             for i in range(self.gradient_accumulate_every):
@@ -338,7 +343,7 @@ class Trainer(object):
                 current_frames, prev_frames = batch['current'].to(dev), batch['prev'].to(dev)
                 last = i == self.gradient_accumulate_every - 1
                 sync = loss_mod.no_sync if (self.distributed and not last) else _nullcontext
-                with sync(), packs():
+                with sync(), packs(), keep():
                     with torch.autocast(dev.type, enabled=self.amp):
                         total_loss, diffusion_loss, vae_loss = loss_mod(current_frames, prev_frames, prob_focus_present,
                                                                         focus_present_mask)
