@@ -103,21 +103,39 @@ struct Split {
     // S[kt] <- whole S[kt] + (columns 32 kt .. of the image at tr)^T (the split rows)
     template <int KT>
     __device__ __forceinline__ void update(f32x16 (&S)[KT], float whole, const char* tr, int pitch) const {
+        if constexpr (Low<T>::THREE && KT > 1) {
+            // all into S: the products of different kt in turn (no chain of dependent ones)
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            const x8_t<T> k0 = tr_operand<T>(tr + 64 * kt, 8 * pitch), k1 = tr_operand<T>(tr + 64 * kt + 16 * pitch, 8 * pitch);
-            f32x16 add = mfma16(k0, e[0], zero16());
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) S[kt][r] *= whole;
-            S[kt] = mfma16(k0, h[0], S[kt]);
-            add = mfma16(k1, e[1], add);
-            S[kt] = mfma16(k1, h[1], S[kt]);
-            if (Low<T>::THREE) {
-                add = mfma16(k0, f[0], add);
-                S[kt] = mfma16(k1, f[1], S[kt]);
+                for (int r = 0; r < 16; ++r) S[kt][r] *= whole;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                x8_t<T> k[KT];
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) k[kt] = tr_operand<T>(tr + 64 * kt + 16 * s * pitch, 8 * pitch);
+#pragma unroll
+                for (int t = 0; t < 3; ++t)
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) S[kt] = mfma16(k[kt], t == 0 ? f[s] : t == 1 ? e[s] : h[s], S[kt]);
             }
+        } else {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) S[kt][r] += add[r] * (1.f / Low<T>::SCALE);
+            for (int kt = 0; kt < KT; ++kt) {
+                const x8_t<T> k0 = tr_operand<T>(tr + 64 * kt, 8 * pitch), k1 = tr_operand<T>(tr + 64 * kt + 16 * pitch, 8 * pitch);
+                f32x16 add = mfma16(k0, e[0], zero16());
+#pragma unroll
+                for (int r = 0; r < 16; ++r) S[kt][r] *= whole;
+                S[kt] = mfma16(k0, h[0], S[kt]);
+                add = mfma16(k1, e[1], add);
+                S[kt] = mfma16(k1, h[1], S[kt]);
+                if (Low<T>::THREE) {
+                    add = mfma16(k0, f[0], add);
+                    S[kt] = mfma16(k1, f[1], S[kt]);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) S[kt][r] += add[r] * (1.f / Low<T>::SCALE);
+            }
         }
     }
 };
@@ -133,12 +151,14 @@ struct Rows {
     __device__ __forceinline__ Rows(const void* p, const Strides& s, long long bb, long long ii, int head, int col0, int width)
         : base(static_cast<const char*>(p) + 2 * (bb * s.b + ii * s.i + head * s.h + col0)), pitch(2 * s.n),
           records((unsigned)(31 * 2 * s.n) + 2 * width) {}
-    __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile(int first) const {
-        return vdmi_rsrc(base + first * pitch, records);
+    // of a tile that has tokens; nothing is read where it has none
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile(int first, bool any = true) const {
+        return vdmi_rsrc(base + first * pitch, any ? records : 0u);
     }
     // offset of column byte `col` of token `row` of a tile of cnt tokens
     __device__ __forceinline__ unsigned at(int row, int cnt, bool reverse, int col) const {
-        return row < cnt ? (unsigned)(reverse ? cnt - 1 - row : row) * (unsigned)pitch + col : NOWHERE;
+        const unsigned off = (unsigned)(reverse ? cnt - 1 - row : row) * (unsigned)pitch + col;
+        return row < cnt ? off : NOWHERE;
     }
 };
 
@@ -211,14 +231,14 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
     };
     auto first_row = [&](int t0, int cnt) { return reverse ? at.len - t0 - cnt : t0; };
     auto load_kv = [&](int t0, int cnt) {
-        const auto rk = kr.tile(first_row(t0, cnt)), rv = vr.tile(first_row(t0, cnt));
+        const auto rk = kr.tile(first_row(t0, cnt), cnt > 0), rv = vr.tile(first_row(t0, cnt), cnt > 0);
 #pragma unroll
         for (int i = 0; i < KS; ++i) kreg[i] = load16<T>(rk, kofs[i]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) vreg[i] = load16<T>(rv, vofs[i]);
     };
     auto load_q = [&](int t0, int cnt) {
-        const auto rq = qr.tile(first_row(t0, cnt));
+        const auto rq = qr.tile(first_row(t0, cnt), cnt > 0);
 #pragma unroll
         for (int i = 0; i < KS; ++i) q[i] = load16<T>(rq, qofs + 32 * i);
     };
@@ -229,7 +249,7 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
     if (cnt > 0) {
         offsets(cnt);
         load_kv(at.t_begin, cnt);
-        if (!STATE_ONLY) load_q(at.t_begin, cnt);
+        if constexpr (!STATE_ONLY) load_q(at.t_begin, cnt);
     }
     const float l2 = log2_decay(a.log_decay, at.head);
     const long long state0 = (at.seq * a.heads + at.head) * (long long)(D * D);
@@ -276,19 +296,25 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
     token_decays(32);
     float whole = __builtin_amdgcn_exp2f(l2 * 32.f);
 
+    // the rest of a tile's work is one basic block (what the last tile needs comes first, the next tile's rows are asked for
+    // whether there is one or not): its phases depend on each other in chains that only overlap if they are scheduled together
     for (int t0 = at.t_begin; t0 < at.t_end; t0 += 32) {
         cnt = min(32, at.t_end - t0);
-        const int next = min(32, at.t_end - t0 - 32);
+        const int next = max(min(32, at.t_end - t0 - 32), 0);
+        if (cnt < 32) {
+            token_decays(cnt);
+            whole = __builtin_amdgcn_exp2f(l2 * (float)cnt);
+        }
+        if (next < 32) offsets(next);
 #pragma unroll
         for (int i = 0; i < KS; ++i) *reinterpret_cast<x8*>(kimg + (lane / (D / 8) + RS * i) * KP + 16 * (lane % (D / 8))) = kreg[i];
 #pragma unroll
         for (int i = 0; i < 2; ++i) *reinterpret_cast<x8*>(vimg + (16 * i + (lane >> 2)) * VP + 16 * (lane & 3)) = vreg[i];
         wave_lds_order();
-        if (next > 0) {
-            if (next < 32) offsets(next);
-            load_kv(t0 + 32, next);
-        }
+        load_kv(t0 + 32, next);
+        __builtin_amdgcn_sched_barrier(0);          // not later: a tile's work is what covers them
         const x8 v0 = tr_operand<T>(vtr, 8 * VP), v1 = tr_operand<T>(vtr + 16 * VP, 8 * VP);
+        const Split<T> sv(v0, v1, uw, half);
         if (!STATE_ONLY) {
             f32x16 st = zero16(), o = zero16();
 #pragma unroll
@@ -297,7 +323,8 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
                 st = mfma16(kf, q[ks], st);
                 o = mfma16(acc_operand<T>(S[ks >> 1], ks & 1), q[ks], o);
             }
-            if (next > 0) load_q(t0 + 32, next);
+            load_q(t0 + 32, next);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 st[r] = weigh(st[r], dw[r]);
@@ -317,12 +344,6 @@ __global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a
                 store16<T>(ro, orow.at(row, cnt, reverse, 16 * (lane & 3)), *reinterpret_cast<const x8*>(vimg + row * VP + 16 * (lane & 3)));
             }
         }
-        if (cnt < 32) {
-            token_decays(cnt);
-            whole = __builtin_amdgcn_exp2f(l2 * (float)cnt);
-            wave_lds_order();
-        }
-        const Split<T> sv(v0, v1, uw, half);
         sv.update(S, whole, ktr, KP);
         wave_lds_order();               // the images and weights are read: the next tile may come
     }
@@ -373,7 +394,7 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
         vofs = vr.at(l31, cnt, true, 16 * half);
     };
     auto load_qg = [&](int t0, int cnt) {
-        const auto rq = qr.tile(at.len - t0 - cnt), rg = gr.tile(at.len - t0 - cnt);
+        const auto rq = qr.tile(at.len - t0 - cnt, cnt > 0), rg = gr.tile(at.len - t0 - cnt, cnt > 0);
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
             qreg[i] = load16<T>(rq, qofs[i]);
@@ -381,7 +402,7 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
         }
     };
     auto load_kv = [&](int t0, int cnt) {
-        const auto rk = kr.tile(at.len - t0 - cnt), rv = vr.tile(at.len - t0 - cnt);
+        const auto rk = kr.tile(at.len - t0 - cnt, cnt > 0), rv = vr.tile(at.len - t0 - cnt, cnt > 0);
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
             k[i] = load16<T>(rk, kofs + 32 * i);
@@ -431,17 +452,20 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
 
     for (int t0 = at.t_begin; t0 < at.t_end; t0 += 32) {
         cnt = min(32, at.t_end - t0);
-        const int next = min(32, at.t_end - t0 - 32);
+        const int next = max(min(32, at.t_end - t0 - 32), 0);
+        if (cnt < 32) {
+            token_decays(cnt);
+            whole = __builtin_amdgcn_exp2f(l2 * (float)cnt);
+        }
+        if (next < 32) offsets(next);
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
             *reinterpret_cast<x8*>(qimg + (lane / (D / 8) + RS * i) * KP + 16 * (lane % (D / 8))) = qreg[i];
             *reinterpret_cast<x8*>(gimg + (lane / (D / 8) + RS * i) * KP + 16 * (lane % (D / 8))) = greg[i];
         }
         wave_lds_order();
-        if (next > 0) {
-            if (next < 32) offsets(next);
-            load_qg(t0 + 32, next);
-        }
+        load_qg(t0 + 32, next);
+        __builtin_amdgcn_sched_barrier(0);
         // [query x key]: q k and do v;  [column x key]: R k and R^T v
         f32x16 p = zero16(), dp = zero16(), ov = zero16(), ok = zero16();
 #pragma unroll
@@ -453,7 +477,8 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
             ov = mfma16(acc_operand<T>(R[ks >> 1], ks & 1), k[ks], ov);
             ok = mfma16(acc_operand<T>(Rt[ks >> 1], ks & 1), v[ks], ok);
         }
-        if (next > 0) load_kv(t0 + 32, next);
+        load_kv(t0 + 32, next);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             p[r] = weigh(p[r], dw[r]);
@@ -467,11 +492,6 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
         ok = mfma16(q0, acc_operand<T>(dp, 0), ok);
         ov = mfma16(g1, acc_operand<T>(p, 1), ov);
         ok = mfma16(q1, acc_operand<T>(dp, 1), ok);
-        if (cnt < 32) {
-            token_decays(cnt);
-            whole = __builtin_amdgcn_exp2f(l2 * (float)cnt);
-            wave_lds_order();
-        }
         {
             const Split<T> sg(g0, g1, uw, half);
             sg.update(R, whole, qtr, KP);
