@@ -253,6 +253,53 @@ def test_no_rows():
     assert B.norm_before(x).shape == x.shape and B.norm_after(x, x).shape == x.shape
 
 
+@gpu
+def test_parameters_of_calls_without_rows():
+    from video_diffusion_amd import block_hip as B
+    x = torch.zeros(2, 0, 64, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    p = [torch.randn(64, device=DEV, requires_grad=True) for _ in range(5)]
+    for res, used in ((B.norm_between(x, x, *p), p), (B.norm_between(x, x, *p)[:1], p[:2]), ([B.norm_before(x, *p[:3])], p[:3])):
+        assert not any(g.any() for g in torch.autograd.grad([r.sum() for r in res], used))
+
+
+@gpu
+def test_many_samples():
+    """More samples than one grid dimension of 16 bits holds, each with its own parameters."""
+    p, ups = make((70001, 1, 8), torch.bfloat16, 6)
+    check("many", p, ups, alpha=0.9, post_kind="layer")
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """5.1e9 elements: the first and last rows against the same rows by themselves."""
+    from video_diffusion_amd import block_hip as B
+    rows, c = 620000, 8192
+    w = 1 + 0.3 * torch.randn(c, device=DEV)
+    x = torch.zeros(rows, c, device=DEV, dtype=torch.bfloat16)
+    ends = torch.randn(64, c, device=DEV).to(torch.bfloat16)
+    x[:32], x[-32:] = ends[:32], ends[32:]
+    y = B.norm_before(x, w)
+    assert torch.equal(torch.cat((y[:32], y[-32:])), B.norm_before(ends, w))
+    assert not y[32:40].any()
+    del y
+    x.requires_grad_()
+    ends.requires_grad_()
+    dy = torch.zeros_like(x)
+    dy[:32], dy[-32:] = 1.5, -0.5
+    (dx,) = torch.autograd.grad(B.norm_before(x, w), x, dy)
+    (want,) = torch.autograd.grad(B.norm_before(ends, w), ends, torch.cat((dy[:32], dy[-32:])))
+    assert torch.equal(torch.cat((dx[:32], dx[-32:])), want)
+
+
+@gpu
+def test_no_second_derivative():
+    from video_diffusion_amd import block_hip as B
+    x = torch.randn(2, 5, 64, device=DEV, requires_grad=True)
+    (g,) = torch.autograd.grad(B.norm_before(x).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
 def _args(**kw):
     a = _lib.BlockNormArgs()
     a.c, a.rows, a.rows_per_sample, a.eps, a.alpha = 64, 20, 10, 1e-5, 1.0
@@ -288,8 +335,6 @@ def test_entry_points_refuse_bad_arguments():
     assert need() > 0 and bwd(workspace=256, workspace_bytes=need() - 1) == E_ARG
     assert bwd(workspace=264, workspace_bytes=need()) == E_ALIGN
     assert need(dweight=None) == 0                                      # no parameter's gradient: no sums
-    many = dict(rows=70000, rows_per_sample=1)
-    assert bwd(**many, workspace=256, workspace_bytes=need(**many)) == E_SHAPE
 
 
 @gpu
@@ -304,6 +349,7 @@ def test_python_entry_points_refuse():
                     (lambda: B.norm_before(x, eps=-1), "eps"), (lambda: B.norm_after(x, x[:, :2]), "alike"),
                     (lambda: B.norm_after(x, x.float()), "alike"), (lambda: B.norm_after(x, x, alpha=float("nan")), "alpha"),
                     (lambda: B.norm_before(x[0, 0]), "rows are"), (lambda: B.norm_before(torch.zeros(2, 9000, device=DEV)), "8192"),
+                    (lambda: B.norm_after(x, None), "missing"), (lambda: B.norm_between(x, None), "missing"),
                     (lambda: B.norm_before(x, w.cpu()), "no CPU path")]:
         with pytest.raises(VdmiError, match=what):
             f()

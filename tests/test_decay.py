@@ -410,6 +410,42 @@ def test_no_tokens_and_no_sequences():
     assert B.decay_attention_step(q[:, 0], q[:, 0], q[:, 0], decay, s).shape == (0, 2, 32)
 
 
+@gpu
+def test_state_of_a_call_without_tokens():
+    from video_diffusion_amd import block_hip as B
+    q = torch.zeros(3, 0, 2, 32, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    s0 = torch.randn(3, 2, 32, 32, device=DEV, requires_grad=True)
+    dq, ds = torch.autograd.grad(B.decay_attention(q, q, q, torch.zeros(2, device=DEV), initial_state=s0).sum(), (q, s0))
+    assert dq.shape == q.shape and not ds.any()
+
+
+@gpu
+def test_a_state_kept_for_the_backward_and_stepped():
+    """decay_attention_step writes the state: a backward that kept it raises."""
+    from video_diffusion_amd import block_hip as B
+    q = torch.randn(1, 3, 2, 32, device=DEV).to(torch.bfloat16).requires_grad_()
+    dec, s = torch.full((2,), -0.1, device=DEV), torch.zeros(1, 2, 32, 32, device=DEV)
+    o = B.decay_attention(q, q, q, dec, initial_state=s)
+    with torch.no_grad():
+        B.decay_attention_step(q[:, 0], q[:, 0], q[:, 0], dec, s)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+    with torch.inference_mode():
+        s = torch.zeros(1, 2, 32, 32, device=DEV)
+        B.decay_attention_step(q[:, 0], q[:, 0], q[:, 0], dec, s)
+        assert s.any()
+
+
+@gpu
+def test_no_second_derivative():
+    from video_diffusion_amd import block_hip as B
+    q = torch.randn(1, 40, 2, 32, device=DEV).to(torch.bfloat16).requires_grad_()
+    o = B.decay_attention(q, q, q, torch.full((2,), -0.1, device=DEV))
+    (g,) = torch.autograd.grad(o.float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.float().sum().backward()
+
+
 def _args(**kw):
     a = _lib.DecayArgs()
     a.dtype, a.b, a.inner, a.n, a.heads, a.d, a.scale, a.log_decay = 0, 2, 3, 10, 2, 32, 0.2, 16
@@ -448,6 +484,10 @@ def test_entry_points_refuse_bad_arguments():
     assert fwd(**long) == E_ARG and fwd(**long, workspace=256, workspace_bytes=need - 1) == E_ARG
     assert bwd(**long, workspace=256, workspace_bytes=need - 1, fwd_workspace=256) == E_ARG
     assert bwd(**long, workspace=256, workspace_bytes=need) == E_ARG            # the forward's states
+    full = dict(**long, workspace_bytes=need)
+    assert fwd(**full, workspace=264) == E_ALIGN and bwd(**full, workspace=264, fwd_workspace=256) == E_ALIGN
+    assert bwd(**full, workspace=256, fwd_workspace=260) == E_ALIGN
+    assert bwd(state_in=264) == E_ALIGN
     for f, r in ((fwd, "q_n"), (fwd, "o_n"), (bwd, "v_n"), (bwd, "dk_n")):
         assert f(**{r: (1 << 25) + 8}) == E_SHAPE and f(**{r: -8}) == E_SHAPE
     assert lib.vdmi_decay_attn_workspace_bytes(C.byref(_args(d=48))) == 0

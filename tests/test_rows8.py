@@ -196,6 +196,35 @@ def test_graph_and_streams():
         assert all(torch.equal(a, b) for a, b in zip(outs, run()))
 
 
+@gpu
+def test_offsets_beyond_32_bits():
+    """5.1e9 elements: the first and last rows against the same rows by themselves."""
+    from video_diffusion_amd import block_hip as B
+    rows, c = 620000, 8192
+    x = torch.zeros(rows, c, device=DEV, dtype=torch.bfloat16)
+    ends = sample(64, c, torch.bfloat16, 4)
+    x[:32], x[-32:] = ends[:32], ends[32:]
+    kept, want = B.pack_rows8(x), B.pack_rows8(ends)
+    del x
+    at = lambda t: torch.cat((t[:32], t[-32:]))
+    assert torch.equal(at(kept.codes), want.codes) and torch.equal(at(kept.exps), want.exps)
+    assert torch.equal(at(kept.unpack()), want.unpack())
+    dy = torch.zeros(rows, 32, device=DEV, dtype=torch.bfloat16)
+    dy[:32] = 1
+    dy[-32:] = torch.randn(32, 32, device=DEV).to(torch.bfloat16)
+    dw = B.rows8_wgrad(kept, dy)
+    assert rel_err(dw, at(dy).double().t() @ want.unpack(torch.float32).double()) < 1e-5
+
+
+@gpu
+def test_no_second_derivative():
+    from video_diffusion_amd import block_hip as B
+    x = torch.randn(5, 64, device=DEV).to(torch.bfloat16).requires_grad_()
+    (g,) = torch.autograd.grad(B.linear_rows8(x, torch.randn(32, 64, device=DEV)).float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.float().sum().backward()
+
+
 def test_entry_points_refuse_bad_arguments():
     lib = _lib.lib()
     E_ARG, E_SHAPE, E_ALIGN = -1, -2, -3

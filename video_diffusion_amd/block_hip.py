@@ -19,6 +19,7 @@ import ctypes as C
 import functools
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import VdmiError, check
@@ -30,6 +31,7 @@ _I64x8 = C.c_int64 * 8
 
 
 _current_device, _raw_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
+_increment_version = torch.autograd.graph.increment_version
 
 
 def _stream_of(t: torch.Tensor) -> int:
@@ -64,6 +66,14 @@ def _ptr(t):
 
 def _wants_grad(*ts) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def _linked(empty: torch.Tensor, *params) -> torch.Tensor:
+    """A result of no elements as one of the parameters too: their gradients are zeros, not absent."""
+    for p in params:
+        if p is not None and _wants_grad(p):
+            empty = empty + p.sum().to(empty.dtype)
+    return empty
 
 
 # ---------------------------------------------------------------------------------------------------------------------
@@ -157,6 +167,7 @@ class DecayAttnFn(torch.autograd.Function):
         return o, last
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do, dlast):
         if do is None and dlast is None:
             return (None,) * 8
@@ -217,7 +228,7 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengt
         lengths = lengths.contiguous()
     if q.numel() == 0:
         # no sequences, or sequences of no tokens: the state stays
-        o = q * k * v
+        o = _linked(q * k * v, initial_state)
         if not return_state:
             return o
         return o, (torch.zeros(*lead, heads, d, d, device=q.device) if initial_state is None else initial_state.clone())
@@ -265,6 +276,8 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
         qh = kh = vh = d
     strides = _I64x8(qb, qh, kb, kh, vb, vh, heads * d, d)
     _decay_step(q, k, v, o, strides, log_decay.contiguous(), state, scale)
+    if not state.is_inference():
+        _increment_version((state,))            # written outside torch: a backward that kept it has to know
     return o
 
 
@@ -353,6 +366,7 @@ class BlockNormFn(torch.autograd.Function):
         return out, y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, dy):
         if dout is None and dy is None:
             return (None,) * 12
@@ -389,7 +403,8 @@ def _block_norm(x, h, post_weight, gate, weight, scale, shift, alpha, kind, post
     if not (0 <= eps < 1e30 and abs(alpha) < 3e38):
         raise VdmiError(f"eps is not negative and alpha finite (got {eps}, {alpha})")
     if x.numel() == 0:
-        return (None if h is None else x + h), (x * 1 if want_y else None)
+        out = x if h is None else _linked(x + h, post_weight, gate)
+        return (None if h is None else out), (_linked(out * 1, weight, scale, shift) if want_y else None)
     if _wants_grad(x, h, post_weight, gate, weight, scale, shift):
         return BlockNormFn.apply(x, h, post_weight, gate, weight, scale, shift, alpha, kind, post_kind, eps, want_y)
     return _norm_forward(*_norm_operands(x, h, post_weight, gate, weight, scale, shift), x.shape, alpha, kind, post_kind, eps, want_y)
@@ -405,6 +420,8 @@ def norm_before(x, weight=None, scale=None, shift=None, *, kind="rms", eps=1e-5)
 def norm_after(x, h, weight=None, gate=None, *, alpha=1.0, kind="rms", eps=1e-5):
     """alpha x + gate * P(h) * weight: a block's output h behind its norm (kind "rms" or "layer"; None: h as it is) and
     gate (float32 [c] or [samples, c]) added to the residual x.  Differentiable in x, h and the parameters."""
+    if h is None:
+        raise VdmiError("h, the block's output, is missing")
     return _block_norm(x, h, weight, gate, None, None, None, alpha, "rms", kind, eps, False)[0]
 
 
@@ -412,6 +429,8 @@ def norm_between(x, h, post_weight=None, gate=None, weight=None, scale=None, shi
                  post_kind="rms", eps=1e-5):
     """From one block to the next in one pass: out = norm_after(x, h, post_weight, gate) and y = norm_before of it with
     weight, scale, shift (of the sum before it is rounded to x's dtype).  Returns (out, y)."""
+    if h is None:
+        raise VdmiError("h, the block's output, is missing")
     return _block_norm(x, h, post_weight, gate, weight, scale, shift, alpha, kind, post_kind, eps, True)
 
 
@@ -519,6 +538,7 @@ class LinearRows8Fn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     @_plain
     def backward(ctx, dy):
         weight, *kept = ctx.saved_tensors
@@ -551,8 +571,9 @@ def _linear_backward(dy, weight, kept, shape, need):
 
 def linear_rows8(x: torch.Tensor, weight: torch.Tensor, bias=None) -> torch.Tensor:
     """F.linear(x, weight, bias) on the library's row GEMMs for bfloat16 x [..., cin] and float32 weight [cout, cin]
-    (multiples of 32), whose input is kept for the weight gradient in 8 bits (about half of a bfloat16 copy).  Output and input gradient are exactly
-    those of the bfloat16 path; only the weight gradient sees the rounding to 8 bits.  Needs the bfloat16 build."""
+    (multiples of 32), whose input is kept for the weight gradient in 8 bits (about half of a bfloat16 copy).  Output and
+    input gradient are exactly those of the bfloat16 path; only the weight gradient sees the rounding to 8 bits.  Needs the
+    bfloat16 build."""
     _on_gpu(x, weight, bias)
     if _lib.PRECISION != "bf16":
         raise VdmiError("the training layers exchange bfloat16 rows: VDMI_PRECISION=f16 serves sampling only")

@@ -343,8 +343,8 @@ __device__ __forceinline__ void add64(float (&v)[3], float (*buf)[3][16], int pl
 
 __global__ __launch_bounds__(1024) void norm_sums_kernel(const SumArgs a) {
     __shared__ float buf[64][3][16];
-    const int lc = threadIdx.x & 15, pl = threadIdx.x >> 4, col = blockIdx.x * 16 + lc;
-    const long long sample = blockIdx.y;
+    const int lc = threadIdx.x & 15, pl = threadIdx.x >> 4, col = blockIdx.y * 16 + lc;
+    const long long sample = blockIdx.x;
     float v[3] = {0.f, 0.f, 0.f};
     if (col < a.c) {
         const float* p = a.part + sample * a.parts * 3 * (long long)a.c + col;
@@ -545,7 +545,6 @@ extern "C" int vdmi_block_norm_bwd(const vdmi_block_norm_args* a, vdmi_stream st
     vdmi_block_norm_args f = *a;
     f.out = f.y = nullptr;
     const NormPlan p = norm_plan(&f, true);
-    if (p.samples > 65535 && p.sums) return VDMI_E_SHAPE;
     if (p.bytes && (!f.workspace || f.workspace_bytes < (int64_t)p.bytes)) return VDMI_E_ARG;
     if (p.bytes && !aligned16(f.workspace)) return VDMI_E_ALIGN;
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -563,7 +562,7 @@ extern "C" int vdmi_block_norm_bwd(const vdmi_block_norm_args* a, vdmi_stream st
     s.dpw = f.dpost_weight; s.dgate = f.dgate; s.dw = f.dweight; s.dscale = f.dscale; s.dshift = f.dshift;
     s.c = f.c; s.parts = p.parts; s.samples = p.samples;
     const unsigned gx = (unsigned)((f.c + 15) / 16);
-    hipLaunchKernelGGL(norm_sums_kernel, dim3(gx, (unsigned)p.samples), dim3(1024), 0, st, s);
+    hipLaunchKernelGGL(norm_sums_kernel, dim3((unsigned)p.samples, gx), dim3(1024), 0, st, s);
     VDMI_LAUNCH_CHECK();
     const bool across = p.samples > 1 && (f.dweight || f.dpost_weight || (f.dscale && !f.scale_stride) ||
                                           (f.dshift && !f.shift_stride) || (f.dgate && !f.gate_stride));

@@ -999,6 +999,7 @@ extern "C" int vdmi_decay_attn_fwd(const vdmi_decay_args* a, vdmi_stream stream)
     const Plan p = plan(a, wants_states(a));
     if (p.is_short) return launch_short(a, p, false, st);
     if (p.bytes && (!a->workspace || a->workspace_bytes < (int64_t)p.bytes)) return VDMI_E_ARG;
+    if (p.bytes && !aligned16(a->workspace)) return VDMI_E_ALIGN;
     ScanArgs s = scan_args(a, p);
     role(s, a->q, a->k, a->v, a->o);
     s.s_in = a->state_in;
@@ -1018,6 +1019,8 @@ extern "C" int vdmi_decay_attn_bwd(const vdmi_decay_args* a, vdmi_stream stream)
     const Plan p = plan(a, wants_states(a));
     if (p.is_short) return launch_short(a, p, true, st);
     if (p.bytes && (!a->workspace || a->workspace_bytes < (int64_t)p.bytes || !a->fwd_workspace)) return VDMI_E_ARG;
+    // S^T is read 16 bytes at a time
+    if (!aligned16(a->state_in) || (p.bytes && (!aligned16(a->workspace) || !aligned16(a->fwd_workspace)))) return VDMI_E_ALIGN;
     // dq: forward in time over (do, v, k) with S^T; the states at the segments' starts are the forward's
     ScanArgs s = scan_args(a, p);
     s.seg = const_cast<float*>(static_cast<const float*>(a->fwd_workspace));
