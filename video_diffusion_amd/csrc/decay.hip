@@ -25,6 +25,8 @@
 // the state (reading k and v only), a second one runs along the segments, a third computes all outputs.
 #include "block_common.h"
 
+#include <algorithm>
+
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -202,7 +204,7 @@ __device__ __forceinline__ int tr_offset(int lane, int pitch) {
 }
 
 template <typename T, int D, bool STATE_ONLY>
-__global__ __launch_bounds__(DW * 64, 2) void decay_scan_kernel(const ScanArgs a) {
+__global__ __launch_bounds__(DW * 64, D == 128 && Low<T>::THREE && !STATE_ONLY ? 1 : 2) void decay_scan_kernel(const ScanArgs a) {
     typedef x8_t<T> x8;
     constexpr int KS = D / 16, KT = D / 32, KP = 2 * D + 16, RS = 512 / D;      // RS: rows that 64 16-byte pieces cover
     __shared__ __attribute__((aligned(16))) char kimg_all[DW][32 * KP];
@@ -369,6 +371,7 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
     __shared__ __attribute__((aligned(16))) char qimg_all[DW][32 * KP];
     __shared__ __attribute__((aligned(16))) char gimg_all[DW][32 * KP];
     __shared__ __attribute__((aligned(16))) float uw_all[DW][32];
+    __shared__ float fade_all[D == 128 && Low<T>::THREE ? DW : 1][64];
     const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     char* qimg = qimg_all[wave];
@@ -383,12 +386,17 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
     at.clear<T>(a.dv, a.dvs, lane);
 
     x8 qreg[KS], greg[KS], k[KS], v[KS];
-    unsigned qofs[KS], gofs[KS], kofs, vofs;
+    // 128 features of bfloat16 leave no registers for the loads' offsets and the pairs' decays: the former are computed
+    // again for every tile, the latter read from LDS.  (From scratch memory, where the compiler would put them, each one
+    // waits for every load in flight: 16384 tokens, 8 heads took 205 us in place of 85.)
+    constexpr bool KEEP = D < 128 || !Low<T>::THREE;
+    unsigned qofs[KEEP ? KS : 1], gofs[KEEP ? KS : 1], kofs, vofs;
+    auto row_at = [&](const Rows& r, int i, int cnt) { return r.at(lane / (D / 8) + RS * i, cnt, true, 16 * (lane % (D / 8))); };
     auto offsets = [&](int cnt) {
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            qofs[i] = qr.at(lane / (D / 8) + RS * i, cnt, true, 16 * (lane % (D / 8)));
-            gofs[i] = gr.at(lane / (D / 8) + RS * i, cnt, true, 16 * (lane % (D / 8)));
+        for (int i = 0; KEEP && i < KS; ++i) {
+            qofs[i] = row_at(qr, i, cnt);
+            gofs[i] = row_at(gr, i, cnt);
         }
         kofs = kr.at(l31, cnt, true, 16 * half);
         vofs = vr.at(l31, cnt, true, 16 * half);
@@ -397,8 +405,8 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
         const auto rq = qr.tile(at.len - t0 - cnt, cnt > 0), rg = gr.tile(at.len - t0 - cnt, cnt > 0);
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
-            qreg[i] = load16<T>(rq, qofs[i]);
-            greg[i] = load16<T>(rg, gofs[i]);
+            qreg[i] = load16<T>(rq, KEEP ? qofs[i] : row_at(qr, i, cnt));
+            greg[i] = load16<T>(rg, KEEP ? gofs[i] : row_at(gr, i, cnt));
         }
     };
     auto load_kv = [&](int t0, int cnt) {
@@ -436,12 +444,20 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
                 Rt[kt][r] = src[col * D + row] * mul;
             }
     }
-    float dw[16];                       // as in the scan; register = query, lane = key, both counted backward in time
+    // the decays of pairs as in the scan; register = query, lane = key, both counted backward in time.  In LDS by gap + 32
+    // where there are no registers for them
+    float dw[KEEP ? 16 : 1];
+    float* fade = fade_all[KEEP ? 0 : wave];
+    if constexpr (KEEP) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int gap = l31 - acc_row(r, half);
-        dw[r] = gap >= 0 ? a.m * __builtin_amdgcn_exp2f(l2 * (float)gap) : 0.f;
+        for (int r = 0; r < 16; ++r) {
+            const int gap = l31 - acc_row(r, half);
+            dw[r] = gap >= 0 ? a.m * __builtin_amdgcn_exp2f(l2 * (float)gap) : 0.f;
+        }
+    } else {
+        fade[lane] = lane < 32 ? 0.f : a.m * __builtin_amdgcn_exp2f(l2 * (float)(lane - 32));
     }
+    const float* fades = fade + 32 + l31 - 4 * half;
     const float ow = a.m * __builtin_amdgcn_exp2f(l2 * (float)l31);
     float* uw = uw_all[wave];
     auto token_decays = [&](int cnt) {
@@ -481,8 +497,9 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            p[r] = weigh(p[r], dw[r]);
-            dp[r] = weigh(dp[r], dw[r]);
+            const float w = KEEP ? dw[r] : fades[-acc_row(r, 0)];
+            p[r] = weigh(p[r], w);
+            dp[r] = weigh(dp[r], w);
             ov[r] *= ow;
             ok[r] *= ow;
         }
@@ -492,10 +509,13 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
         ok = mfma16(q0, acc_operand<T>(dp, 0), ok);
         ov = mfma16(g1, acc_operand<T>(p, 1), ov);
         ok = mfma16(q1, acc_operand<T>(dp, 1), ok);
+        const x8 rok[2] = {acc_operand<T>(ok, 0), acc_operand<T>(ok, 1)}, rov[2] = {acc_operand<T>(ov, 0), acc_operand<T>(ov, 1)};
+        if (!KEEP) __builtin_amdgcn_sched_barrier(0);
         {
             const Split<T> sg(g0, g1, uw, half);
             sg.update(R, whole, qtr, KP);
         }
+        if (!KEEP) __builtin_amdgcn_sched_barrier(0);
         {
             const Split<T> sq(q0, q1, uw, half);
             sq.update(Rt, whole, gtr, KP);
@@ -504,8 +524,8 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
         wave_lds_order();
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            *reinterpret_cast<x8*>(qimg + l31 * VP + 32 * s + 16 * half) = acc_operand<T>(ok, s);
-            *reinterpret_cast<x8*>(gimg + l31 * VP + 32 * s + 16 * half) = acc_operand<T>(ov, s);
+            *reinterpret_cast<x8*>(qimg + l31 * VP + 32 * s + 16 * half) = rok[s];
+            *reinterpret_cast<x8*>(gimg + l31 * VP + 32 * s + 16 * half) = rov[s];
         }
         wave_lds_order();
         const auto rk = dkr.tile(at.len - t0 - cnt), rv = dvr.tile(at.len - t0 - cnt);
@@ -843,9 +863,17 @@ int check_args(const vdmi_decay_args* a) {
     return VDMI_OK;
 }
 
-// How the time axis is cut: waves = sequences x heads x d / 32 column slices x segments.  The card holds 256 x 8 waves of
-// these kernels; a segment costs its state (4 d d bytes written and read twice) and a second read of k and v, so segments
-// are only cut until the card is filled and never shorter than 4 d tokens (state traffic under half of its rows').
+// How the time axis is cut: waves = sequences x heads x d / 32 column slices x segments.  A tile is 1 to 4 us of steps that
+// depend on each other, so few sequences are cut until every SIMD of the card has a wave (256 x 4 of them), down to one tile
+// per segment; the walk along the segments is serial: beyond 64 of them they are 128 tokens or longer.  Two or three
+// segments cost about what they save (k and v are read once more, the states written and read) unless they are long.
+// Measured, bfloat16, forward / backward in us (sequences x tokens x heads x features: segments):
+//     6 x 701 x 4 x 64:    1: 29/83    2: 31/61    4: 23/43    21: 19/30
+//     1 x 1000 x 8 x 128:  1: 64/185   2: 57/126   8: 25/50    31: 22/39
+//     2 x 8192 x 8 x 64:   1: 281/847  16: 45/88   32 (1024 waves): 34/62   64: 40/73
+//     1 x 4000 x 8 x 32:   32: 19/30   64: 20/27   125: 26/33
+//     32 x 500 x 8 x 64:   1: 25/67    2: 38/66        30 x 2048 x 8 x 64:  1: 101/253   2: 102/202
+//     62 x 2048 x 8 x 64:  1: 130/332  2: 184/394
 Plan plan(const vdmi_decay_args* a, bool states) {
     Plan p;
     p.nseq = (long long)a->b * a->inner;
@@ -856,9 +884,8 @@ Plan plan(const vdmi_decay_args* a, bool states) {
     p.bytes = 0;
     if (p.is_short) return p;
     const long long waves = p.nseq * a->heads * (a->d / 32);
-    long long want = 2048 / waves;
-    const long long most = a->n / (4 * a->d);
-    if (want > most) want = most;
+    long long want = std::min(1024 / waves, std::min<long long>(a->n / 32, std::max(64, a->n / 128)));
+    if (want < 4 && a->n < 4 * a->d * want) want = 1;
     if (want > 1) {
         p.seg_len = (int)(((a->n + want - 1) / want + 31) / 32 * 32);
         p.nseg = (a->n + p.seg_len - 1) / p.seg_len;
