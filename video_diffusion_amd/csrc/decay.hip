@@ -142,6 +142,34 @@ struct Split {
     }
 };
 
+// What lies in accumulator registers (weighted pairs, a state), contracted over them, as a sum of two 16-bit operands.  One
+// operand alone is rounded once more than a sum in float32 would be: sqrt(2) of its error over many terms, more in a result
+// of few.  So the sequences of one tile take two (as exact as float32 sums; 16 frames of 16384 sites in training 317 -> 330
+// us), longer ones do not (16384 tokens of 8 x 128 forward: 77 -> 85 us with the pairs alone in two).
+template <typename T>
+struct FineOperand {
+    x8_t<T> h[2], e[2];
+    __device__ __forceinline__ explicit FineOperand(const f32x16& p) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                h[s][j] = high_part<T>(p[8 * s + j]);
+                e[s][j] = (T)((p[8 * s + j] - (float)h[s][j]) * Low<T>::SCALE);
+            }
+    }
+    // o + (a0 | a1) times this
+    __device__ __forceinline__ f32x16 times(const x8_t<T>& a0, const x8_t<T>& a1, f32x16 o) const {
+        f32x16 add = mfma16(a0, e[0], zero16());
+        o = mfma16(a0, h[0], o);
+        add = mfma16(a1, e[1], add);
+        o = mfma16(a1, h[1], o);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[r] += add[r] * (1.f / Low<T>::SCALE);
+        return o;
+    }
+};
+
 // Rows of one head, 32 tokens at a time: a buffer resource per tile, based on the tile's first row in memory, and 32-bit
 // lane offsets that stay the same from tile to tile; rows past the tile's last token get an offset past the resource's
 // end, which loads as zero and is not stored.  The tokens run backwards in memory where REVERSE.
@@ -203,8 +231,13 @@ __device__ __forceinline__ int tr_offset(int lane, int pitch) {
     return (4 * (g16 >> 1) + tq) * pitch + (16 * (g16 & 1) + 4 * (((tp & 1) << 1) | (tp >> 1))) * 2;
 }
 
-template <typename T, int D, bool STATE_ONLY>
-__global__ __launch_bounds__(DW * 64, D == 128 && Low<T>::THREE && !STATE_ONLY ? 1 : 2) void decay_scan_kernel(const ScanArgs a) {
+// WHAT: the outputs; only the segments' states; the outputs of sequences of one tile (FineOperand)
+enum { OUTPUTS, STATES, ONE_TILE };
+
+template <typename T, int D, int WHAT>
+__global__ __launch_bounds__(DW * 64, D == 128 && (Low<T>::THREE || WHAT == ONE_TILE) && WHAT != STATES ? 1 : 2)
+void decay_scan_kernel(const ScanArgs a) {
+    constexpr bool STATE_ONLY = WHAT == STATES, FINE = WHAT == ONE_TILE;
     typedef x8_t<T> x8;
     constexpr int KS = D / 16, KT = D / 32, KP = 2 * D + 16, RS = 512 / D;      // RS: rows that 64 16-byte pieces cover
     __shared__ __attribute__((aligned(16))) char kimg_all[DW][32 * KP];
@@ -318,22 +351,33 @@ __global__ __launch_bounds__(DW * 64, D == 128 && Low<T>::THREE && !STATE_ONLY ?
         const x8 v0 = tr_operand<T>(vtr, 8 * VP), v1 = tr_operand<T>(vtr + 16 * VP, 8 * VP);
         const Split<T> sv(v0, v1, uw, half);
         if (!STATE_ONLY) {
-            f32x16 st = zero16(), o = zero16();
+            f32x16 st = zero16(), o = zero16(), low = zero16();
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const x8 kf = *reinterpret_cast<const x8*>(kimg + l31 * KP + 32 * ks + 16 * half);
                 st = mfma16(kf, q[ks], st);
-                o = mfma16(acc_operand<T>(S[ks >> 1], ks & 1), q[ks], o);
+                if constexpr (FINE) {
+                    const FineOperand<T> state(S[ks >> 1]);
+                    o = mfma16(state.h[ks & 1], q[ks], o);
+                    low = mfma16(state.e[ks & 1], q[ks], low);
+                } else {
+                    o = mfma16(acc_operand<T>(S[ks >> 1], ks & 1), q[ks], o);
+                }
             }
             load_q(t0 + 32, next);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 st[r] = weigh(st[r], dw[r]);
+                if (FINE) o[r] += low[r] * (1.f / Low<T>::SCALE);
                 o[r] *= ow;
             }
-            o = mfma16(v0, acc_operand<T>(st, 0), o);
-            o = mfma16(v1, acc_operand<T>(st, 1), o);
+            if constexpr (FINE) {
+                o = FineOperand<T>(st).times(v0, v1, o);
+            } else {
+                o = mfma16(v0, acc_operand<T>(st, 0), o);
+                o = mfma16(v1, acc_operand<T>(st, 1), o);
+            }
             // through LDS (the tile's v image is in registers by now) to 16-byte stores, four lanes on a row's 64 bytes
             wave_lds_order();
             *reinterpret_cast<x8*>(vimg + l31 * VP + 16 * half) = acc_operand<T>(o, 0);
@@ -364,14 +408,14 @@ __global__ __launch_bounds__(DW * 64, D == 128 && Low<T>::THREE && !STATE_ONLY ?
 // dk and dv in one walk backward in time: both read q, k, v and do, and what one of them needs of R = dS / m by columns the
 // other needs by rows.  A wave computes 32 columns of dv and the same 32 columns of dk and holds R[all dk][its columns of
 // dv] and R^T[all dv][its columns of dk].
-template <typename T, int D>
+template <typename T, int D, bool FINE>
 __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(const GradArgs a) {
     typedef x8_t<T> x8;
     constexpr int KS = D / 16, KT = D / 32, KP = 2 * D + 16, RS = 512 / D;
     __shared__ __attribute__((aligned(16))) char qimg_all[DW][32 * KP];
     __shared__ __attribute__((aligned(16))) char gimg_all[DW][32 * KP];
     __shared__ __attribute__((aligned(16))) float uw_all[DW][32];
-    __shared__ float fade_all[D == 128 && Low<T>::THREE ? DW : 1][64];
+    __shared__ float fade_all[D == 128 && (Low<T>::THREE || FINE) ? DW : 1][64];
     const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     char* qimg = qimg_all[wave];
@@ -389,7 +433,7 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
     // 128 features of bfloat16 leave no registers for the loads' offsets and the pairs' decays: the former are computed
     // again for every tile, the latter read from LDS.  (From scratch memory, where the compiler would put them, each one
     // waits for every load in flight: 16384 tokens, 8 heads took 205 us in place of 85.)
-    constexpr bool KEEP = D < 128 || !Low<T>::THREE;
+    constexpr bool KEEP = D < 128 || !(Low<T>::THREE || FINE);
     unsigned qofs[KEEP ? KS : 1], gofs[KEEP ? KS : 1], kofs, vofs;
     auto row_at = [&](const Rows& r, int i, int cnt) { return r.at(lane / (D / 8) + RS * i, cnt, true, 16 * (lane % (D / 8))); };
     auto offsets = [&](int cnt) {
@@ -483,15 +527,23 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
         load_qg(t0 + 32, next);
         __builtin_amdgcn_sched_barrier(0);
         // [query x key]: q k and do v;  [column x key]: R k and R^T v
-        f32x16 p = zero16(), dp = zero16(), ov = zero16(), ok = zero16();
+        f32x16 p = zero16(), dp = zero16(), ov = zero16(), ok = zero16(), lv = zero16(), lk = zero16();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const x8 qf = *reinterpret_cast<const x8*>(qimg + l31 * KP + 32 * ks + 16 * half);
             const x8 gf = *reinterpret_cast<const x8*>(gimg + l31 * KP + 32 * ks + 16 * half);
             p = mfma16(qf, k[ks], p);
             dp = mfma16(gf, v[ks], dp);
-            ov = mfma16(acc_operand<T>(R[ks >> 1], ks & 1), k[ks], ov);
-            ok = mfma16(acc_operand<T>(Rt[ks >> 1], ks & 1), v[ks], ok);
+            if constexpr (FINE) {
+                const FineOperand<T> r(R[ks >> 1]), rt(Rt[ks >> 1]);
+                ov = mfma16(r.h[ks & 1], k[ks], ov);
+                ok = mfma16(rt.h[ks & 1], v[ks], ok);
+                lv = mfma16(r.e[ks & 1], k[ks], lv);
+                lk = mfma16(rt.e[ks & 1], v[ks], lk);
+            } else {
+                ov = mfma16(acc_operand<T>(R[ks >> 1], ks & 1), k[ks], ov);
+                ok = mfma16(acc_operand<T>(Rt[ks >> 1], ks & 1), v[ks], ok);
+            }
         }
         load_kv(t0 + 32, next);
         __builtin_amdgcn_sched_barrier(0);
@@ -500,15 +552,24 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
             const float w = KEEP ? dw[r] : fades[-acc_row(r, 0)];
             p[r] = weigh(p[r], w);
             dp[r] = weigh(dp[r], w);
+            if (FINE) {
+                ov[r] += lv[r] * (1.f / Low<T>::SCALE);
+                ok[r] += lk[r] * (1.f / Low<T>::SCALE);
+            }
             ov[r] *= ow;
             ok[r] *= ow;
         }
         const x8 g0 = tr_operand<T>(gtr + 64 * at.slice, 8 * KP), g1 = tr_operand<T>(gtr + 64 * at.slice + 16 * KP, 8 * KP);
         const x8 q0 = tr_operand<T>(qtr + 64 * at.slice, 8 * KP), q1 = tr_operand<T>(qtr + 64 * at.slice + 16 * KP, 8 * KP);
-        ov = mfma16(g0, acc_operand<T>(p, 0), ov);
-        ok = mfma16(q0, acc_operand<T>(dp, 0), ok);
-        ov = mfma16(g1, acc_operand<T>(p, 1), ov);
-        ok = mfma16(q1, acc_operand<T>(dp, 1), ok);
+        if constexpr (FINE) {
+            ov = FineOperand<T>(p).times(g0, g1, ov);
+            ok = FineOperand<T>(dp).times(q0, q1, ok);
+        } else {
+            ov = mfma16(g0, acc_operand<T>(p, 0), ov);
+            ok = mfma16(q0, acc_operand<T>(dp, 0), ok);
+            ov = mfma16(g1, acc_operand<T>(p, 1), ov);
+            ok = mfma16(q1, acc_operand<T>(dp, 1), ok);
+        }
         const x8 rok[2] = {acc_operand<T>(ok, 0), acc_operand<T>(ok, 1)}, rov[2] = {acc_operand<T>(ov, 0), acc_operand<T>(ov, 1)};
         if (!KEEP) __builtin_amdgcn_sched_barrier(0);
         {
@@ -622,8 +683,8 @@ __device__ __forceinline__ bool finite(const x8_t<T> (&x)[N]) {
 
 // NH heads of D features side by side in memory are one row of W columns, moved as 16-byte pieces with all lanes of a row
 // next to each other and transposed to operands through LDS.  Measured over 16 frames of 16384 sites with 8 heads of 32
-// features (537 MB forward, 940 MB backward): 122 us and 197 us, 4.4 and 4.8 TB/s; one head at a time (64-byte rows) 127
-// and 234 us; every lane loading and storing its own token's row as operands (32 bytes of a row per instruction) 150 and 283.
+// features (537 MB forward, 940 MB backward): 123 us and 207 us, 4.4 and 4.5 TB/s; before the pairs were two operands
+// each 122 and 197 us, one head at a time (64-byte rows) 127 and 234; every lane loading and storing its own token's row as operands (32 bytes of a row per instruction) 150 and 283.
 constexpr int short_waves(int d, bool bwd) { return d == 128 && bwd ? 1 : 2; }
 
 template <typename T, int D, int NH, bool BWD>
@@ -724,13 +785,11 @@ __global__ __launch_bounds__((short_waves(D, BWD) * 64), D == 128 ? 1 : 2) void 
     };
     // (columns of an image)^T x pairs into the same columns of another one
     auto product = [&](const char* src, const f32x16& p, char* dst) {
-        const x8 p0 = acc_operand<T>(p, 0), p1 = acc_operand<T>(p, 1);
+        const FineOperand<T> pairs(p);
         f32x16 o[DT];
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            o[dt] = mfma16(tr_operand<T>(src + tr_off + 64 * dt, 8 * P), p0, zero16());
-            o[dt] = mfma16(tr_operand<T>(src + tr_off + 64 * dt + 16 * P, 8 * P), p1, o[dt]);
-        }
+        for (int dt = 0; dt < DT; ++dt)
+            o[dt] = pairs.times(tr_operand<T>(src + tr_off + 64 * dt, 8 * P), tr_operand<T>(src + tr_off + 64 * dt + 16 * P, 8 * P), zero16());
         wave_lds_order();
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
@@ -898,15 +957,15 @@ bool wants_states(const vdmi_decay_args* a) { return a->state_in || a->state_out
 
 Strides strides_of(const vdmi_rows4& r) { return Strides{r.b, r.i, r.n, r.h}; }
 
-template <bool STATE_ONLY>
+template <int WHAT>
 int launch_scan(const ScanArgs& s, const vdmi_decay_args* a, const Plan& p, hipStream_t st) {
     ScanArgs x = s;
-    const long long segs = STATE_ONLY && !x.s_out ? p.nseg - 1 : p.nseg;
+    const long long segs = WHAT == STATES && !x.s_out ? p.nseg - 1 : p.nseg;
     const long long tasks = p.nseq * a->heads * segs * (a->d / 32), wgs = (tasks + DW - 1) / DW;
     if (tasks > 0x7fffffffLL) return VDMI_E_SHAPE;
     x.tasks = (unsigned)tasks;
     const dim3 grid((unsigned)wgs), block(DW * 64);
-#define SCAN(T, D) hipLaunchKernelGGL((decay_scan_kernel<T, D, STATE_ONLY>), grid, block, 0, st, x)
+#define SCAN(T, D) hipLaunchKernelGGL((decay_scan_kernel<T, D, WHAT>), grid, block, 0, st, x)
 #define SCAN_D(T) do { if (a->d == 32) SCAN(T, 32); else if (a->d == 64) SCAN(T, 64); else SCAN(T, 128); } while (0)
     if (a->dtype == VDMI_DT_BF16) SCAN_D(__bf16); else SCAN_D(_Float16);
 #undef SCAN_D
@@ -915,10 +974,14 @@ int launch_scan(const ScanArgs& s, const vdmi_decay_args* a, const Plan& p, hipS
     return VDMI_OK;
 }
 
+int outputs(const ScanArgs& s, const vdmi_decay_args* a, const Plan& p, hipStream_t st) {
+    return a->n <= 32 ? launch_scan<ONE_TILE>(s, a, p, st) : launch_scan<OUTPUTS>(s, a, p, st);
+}
+
 // sums of the segments and the states at their starts (nothing to do for one segment)
 int segment_states(ScanArgs s, const vdmi_decay_args* a, const Plan& p, hipStream_t st) {
     if (p.nseg == 1) return VDMI_OK;
-    const int r = launch_scan<true>(s, a, p, st);
+    const int r = launch_scan<STATES>(s, a, p, st);
     if (r != VDMI_OK) return r;
     hipLaunchKernelGGL(decay_segments_kernel, dim3((unsigned)(p.nseq * a->heads), (unsigned)(a->d * a->d / 256)), dim3(256), 0, st,
                        s, a->d * a->d);
@@ -1000,10 +1063,11 @@ int launch_grad(const vdmi_decay_args* a, const Plan& p, hipStream_t st) {
     if (tasks > 0x7fffffffLL) return VDMI_E_SHAPE;
     g.tasks = (unsigned)tasks;
     const dim3 grid((unsigned)wgs), block(DW * 64);
-#define GRAD_D(T) do { if (a->d == 32) hipLaunchKernelGGL((decay_grad_kernel<T, 32>), grid, block, 0, st, g); \
-                       else if (a->d == 64) hipLaunchKernelGGL((decay_grad_kernel<T, 64>), grid, block, 0, st, g); \
-                       else hipLaunchKernelGGL((decay_grad_kernel<T, 128>), grid, block, 0, st, g); } while (0)
+#define GRAD(T, D) do { if (a->n <= 32) hipLaunchKernelGGL((decay_grad_kernel<T, D, true>), grid, block, 0, st, g); \
+                        else hipLaunchKernelGGL((decay_grad_kernel<T, D, false>), grid, block, 0, st, g); } while (0)
+#define GRAD_D(T) do { if (a->d == 32) GRAD(T, 32); else if (a->d == 64) GRAD(T, 64); else GRAD(T, 128); } while (0)
     if (a->dtype == VDMI_DT_BF16) GRAD_D(__bf16); else GRAD_D(_Float16);
+#undef GRAD
 #undef GRAD_D
     VDMI_LAUNCH_CHECK();
     return VDMI_OK;
@@ -1033,7 +1097,7 @@ extern "C" int vdmi_decay_attn_fwd(const vdmi_decay_args* a, vdmi_stream stream)
     s.s_out = a->state_out;
     s.e_out = 1;
     const int r = segment_states(s, a, p, st);
-    return r != VDMI_OK ? r : launch_scan<false>(s, a, p, st);
+    return r != VDMI_OK ? r : outputs(s, a, p, st);
 }
 
 extern "C" int vdmi_decay_attn_bwd(const vdmi_decay_args* a, vdmi_stream stream) {
@@ -1055,7 +1119,7 @@ extern "C" int vdmi_decay_attn_bwd(const vdmi_decay_args* a, vdmi_stream stream)
     s.e_out = 1;
     s.rs = 1;
     role(s, a->dout, a->v, a->k, a->dq);
-    int r = launch_scan<false>(s, a, p, st);
+    int r = outputs(s, a, p, st);
     if (r != VDMI_OK) return r;
     // dv and dk: backward in time; R = dS / m collects lambda^(i+1) q_i do_i^T
     if (p.nseg > 1) {
