@@ -57,104 +57,74 @@ struct RowSum {                         // sums over the L lanes of a row; L == 
     }
 };
 
-// column of element e of piece p: eight consecutive ones (16-byte loads), or one per lane where the rows' pitch, address
-// or width does not allow that
-template <bool VEC, int L>
-__device__ __forceinline__ int column(int p, int e, int l) { return VEC ? (p * L + l) * 8 + e : (p * 8 + e) * L + l; }
+// column of element e of piece p: eight consecutive ones of a row, loaded and stored 16 bytes at a time at any alignment of
+// the elements.  TAIL: the columns are no multiple of eight, and the row's last piece goes element by element.
+template <int L>
+__device__ __forceinline__ int column(int p, int e, int l) { return (p * L + l) * 8 + e; }
 
-template <typename T, bool VEC, int L, int P>
-__device__ __forceinline__ void load_row(float (&v)[P * 8], const void* base, long long row, long long ld, int c, int l) {
-    const T* r = static_cast<const T*>(base) + row * ld;
+template <typename T, bool TAIL, int L, int P>
+__device__ __forceinline__ void load_row(float (&v)[P * 8], const T* r, float absent, int c, int l) {
+    constexpr int W = 16 / sizeof(T);
+    typedef T wide __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+    T x[P * 8];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-        if constexpr (VEC) {
-            const int col = column<true, L>(p, 0, l);
-            if constexpr (sizeof(T) == 4) {
-                f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
-                if (col < c) {
-                    a = *reinterpret_cast<const f32x4*>(r + col);
-                    b = *reinterpret_cast<const f32x4*>(r + col + 4);
-                }
+        const int col = column<L>(p, 0, l);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { v[8 * p + e] = a[e]; v[8 * p + 4 + e] = b[e]; }
-            } else {
-                typedef __attribute__((ext_vector_type(8))) T t8;
-                t8 a;
+        for (int e = 0; e < 8; ++e) x[8 * p + e] = (T)absent;
+        if (TAIL ? col + 8 <= c : col < c) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) a[e] = (T)0.f;
-                if (col < c) a = *reinterpret_cast<const t8*>(r + col);
+            for (int i = 0; i < 8 / W; ++i) {
+                const wide a = *reinterpret_cast<const wide*>(r + col + W * i);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[8 * p + e] = (float)a[e];
+                for (int e = 0; e < W; ++e) x[8 * p + W * i + e] = a[e];
             }
-        } else {
+        } else if (TAIL) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int col = column<false, L>(p, e, l);
-                v[8 * p + e] = col < c ? (float)r[col] : 0.f;
+            for (int e = 0; e < 7; ++e)
+                if (col + e < c) x[8 * p + e] = r[col + e];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < P * 8; ++i) v[i] = (float)x[i];
+}
+
+template <typename T, bool TAIL, int L, int P>
+__device__ __forceinline__ void store_row(const float (&v)[P * 8], T* r, int c, int l) {
+    constexpr int W = 16 / sizeof(T);
+    typedef T wide __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int col = column<L>(p, 0, l);
+        if (TAIL ? col + 8 <= c : col < c) {
+#pragma unroll
+            for (int i = 0; i < 8 / W; ++i) {
+                wide a;
+#pragma unroll
+                for (int e = 0; e < W; ++e) a[e] = (T)v[8 * p + W * i + e];
+                *reinterpret_cast<wide*>(r + col + W * i) = a;
             }
+        } else if (TAIL) {
+#pragma unroll
+            for (int e = 0; e < 7; ++e)
+                if (col + e < c) r[col + e] = (T)v[8 * p + e];
         }
     }
 }
 
-template <typename T, bool VEC, int L, int P>
-__device__ __forceinline__ void store_row(const float (&v)[P * 8], void* base, long long row, long long ld, int c, int l) {
-    T* r = static_cast<T*>(base) + row * ld;
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-        if constexpr (VEC) {
-            const int col = column<true, L>(p, 0, l);
-            if (col >= c) continue;
-            if constexpr (sizeof(T) == 4) {
-                f32x4 a, b;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) { a[e] = v[8 * p + e]; b[e] = v[8 * p + 4 + e]; }
-                *reinterpret_cast<f32x4*>(r + col) = a;
-                *reinterpret_cast<f32x4*>(r + col + 4) = b;
-            } else {
-                typedef __attribute__((ext_vector_type(8))) T t8;
-                t8 a;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) a[e] = (T)v[8 * p + e];
-                *reinterpret_cast<t8*>(r + col) = a;
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int col = column<false, L>(p, e, l);
-                if (col < c) r[col] = (T)v[8 * p + e];
-            }
-        }
-    }
-}
-
-// the lane's columns of a parameter row (any element alignment), `absent` where there is none
-template <bool VEC, int L, int P>
+// the lane's columns of a parameter row, `absent` where there is none
+template <bool TAIL, int L, int P>
 __device__ __forceinline__ void load_params(float (&v)[P * 8], const float* src, float absent, int c, int l) {
-    typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+    if (src) {
+        load_row<float, TAIL, L, P>(v, src, absent, c, l);
+    } else {
 #pragma unroll
-    for (int i = 0; i < P * 8; ++i) v[i] = absent;
-    if (!src) return;
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-        if constexpr (VEC) {
-            const int col = column<true, L>(p, 0, l);
-            if (col < c) {
-                const f4u x = *reinterpret_cast<const f4u*>(src + col), y = *reinterpret_cast<const f4u*>(src + col + 4);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) { v[8 * p + e] = x[e]; v[8 * p + 4 + e] = y[e]; }
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int col = column<false, L>(p, e, l);
-                if (col < c) v[8 * p + e] = src[col];
-            }
-        }
+        for (int i = 0; i < P * 8; ++i) v[i] = absent;
     }
 }
 
 // v -> its norm in place; returns the factor
-template <bool VEC, int L, int P>
+template <int L, int P>
 __device__ __forceinline__ float normalise(float (&v)[P * 8], RowSum<L>& sum, int kind, int c, float inv_c, float eps, int l) {
     if (kind == 1) {
         float s = 0.f, z = 0.f;
@@ -163,7 +133,7 @@ __device__ __forceinline__ float normalise(float (&v)[P * 8], RowSum<L>& sum, in
         sum.two(s, z);
         const float mean = s * inv_c;
 #pragma unroll
-        for (int i = 0; i < P * 8; ++i) v[i] = column<VEC, L>(i >> 3, i & 7, l) < c ? v[i] - mean : 0.f;
+        for (int i = 0; i < P * 8; ++i) v[i] = column<L>(i >> 3, i & 7, l) < c ? v[i] - mean : 0.f;
     }
     float s = 0.f, z = 0.f;
 #pragma unroll
@@ -176,7 +146,7 @@ __device__ __forceinline__ float normalise(float (&v)[P * 8], RowSum<L>& sum, in
 }
 
 // g (gradient of a norm's result n) -> f (g - mean g - n mean(g n)); the plain mean for the layer norm
-template <bool VEC, int L, int P>
+template <int L, int P>
 __device__ __forceinline__ void norm_gradient(float (&g)[P * 8], const float (&n)[P * 8], float f, RowSum<L>& sum, int kind, int c,
                                               float inv_c, int l) {
     float s = 0.f, t = 0.f;
@@ -186,10 +156,10 @@ __device__ __forceinline__ void norm_gradient(float (&g)[P * 8], const float (&n
     s = kind == 1 ? s * inv_c : 0.f;
     t *= inv_c;
 #pragma unroll
-    for (int i = 0; i < P * 8; ++i) g[i] = column<VEC, L>(i >> 3, i & 7, l) < c ? f * (g[i] - s - n[i] * t) : 0.f;
+    for (int i = 0; i < P * 8; ++i) g[i] = column<L>(i >> 3, i & 7, l) < c ? f * (g[i] - s - n[i] * t) : 0.f;
 }
 
-template <typename T, bool VEC, int L, int P, bool BWD>
+template <typename T, bool TAIL, int L, int P, bool BWD>
 __global__ __launch_bounds__(256) void block_norm_kernel(const NormArgs a) {
     constexpr int N = P * 8, ROWS = 256 / L;
     __shared__ float slots[2][2][4];
@@ -203,21 +173,21 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const NormArgs a) {
     const float inv_c = 1.f / (float)c;
     // per column: a = weight (1 + scale), gate * post_weight, shift
     float wa[N], pg[N], sh[BWD ? 1 : N];
-    load_params<VEC, L, P>(wa, a.w, 1.f, c, l);
-    load_params<VEC, L, P>(pg, a.pw, 1.f, c, l);
+    load_params<TAIL, L, P>(wa, a.w, 1.f, c, l);
+    load_params<TAIL, L, P>(pg, a.pw, 1.f, c, l);
     if (a.scale) {
         float t[N];
-        load_params<VEC, L, P>(t, a.scale + sample * a.scale_bs, 0.f, c, l);
+        load_params<TAIL, L, P>(t, a.scale + sample * a.scale_bs, 0.f, c, l);
 #pragma unroll
         for (int i = 0; i < N; ++i) wa[i] *= 1.f + t[i];
     }
     if (a.gate) {
         float t[N];
-        load_params<VEC, L, P>(t, a.gate + sample * a.gate_bs, 0.f, c, l);
+        load_params<TAIL, L, P>(t, a.gate + sample * a.gate_bs, 0.f, c, l);
 #pragma unroll
         for (int i = 0; i < N; ++i) pg[i] *= t[i];
     }
-    if constexpr (!BWD) load_params<VEC, L, P>(sh, a.shift ? a.shift + sample * a.shift_bs : nullptr, 0.f, c, l);
+    if constexpr (!BWD) load_params<TAIL, L, P>(sh, a.shift ? a.shift + sample * a.shift_bs : nullptr, 0.f, c, l);
     float s1[BWD ? N : 1], s2[BWD ? N : 1], s3[BWD ? N : 1];
     if constexpr (BWD) {
 #pragma unroll
@@ -229,47 +199,47 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const NormArgs a) {
         if (r >= last) continue;        // L <= 64: lanes of other rows are not involved in this one's sums
         const long long row = sample * a.rows_per_sample + r;
         float v[N], h[N];
-        load_row<T, VEC, L, P>(v, a.x, row, a.ldx, c, l);
-        if (a.h) load_row<T, VEC, L, P>(h, a.h, row, a.ldh, c, l);
+        load_row<T, TAIL, L, P>(v, static_cast<const T*>(a.x) + row * a.ldx, 0.f, c, l);
+        if (a.h) load_row<T, TAIL, L, P>(h, static_cast<const T*>(a.h) + row * a.ldh, 0.f, c, l);
         float fh = 1.f;
         if constexpr (!BWD) {
             if (a.h) {
-                if (a.pkind >= 0) normalise<VEC, L, P>(h, sum, a.pkind, c, inv_c, a.eps, l);
+                if (a.pkind >= 0) normalise<L, P>(h, sum, a.pkind, c, inv_c, a.eps, l);
 #pragma unroll
                 for (int i = 0; i < N; ++i) v[i] = a.alpha * v[i] + pg[i] * h[i];
-                store_row<T, VEC, L, P>(v, a.out, row, a.ldo, c, l);
+                store_row<T, TAIL, L, P>(v, static_cast<T*>(a.out) + row * a.ldo, c, l);
             }
             if (a.y) {
-                normalise<VEC, L, P>(v, sum, a.kind, c, inv_c, a.eps, l);
+                normalise<L, P>(v, sum, a.kind, c, inv_c, a.eps, l);
 #pragma unroll
                 for (int i = 0; i < N; ++i) v[i] = v[i] * wa[i] + sh[i];
-                store_row<T, VEC, L, P>(v, a.y, row, a.ldy, c, l);
+                store_row<T, TAIL, L, P>(v, static_cast<T*>(a.y) + row * a.ldy, c, l);
             }
         } else {
             float ds[N], g[N];
-            if (a.dout) load_row<T, VEC, L, P>(ds, a.dout, row, a.lddo, c, l);
-            if (a.dy) load_row<T, VEC, L, P>(g, a.dy, row, a.lddy, c, l);
+            if (a.dout) load_row<T, TAIL, L, P>(ds, static_cast<const T*>(a.dout) + row * a.lddo, 0.f, c, l);
+            if (a.dy) load_row<T, TAIL, L, P>(g, static_cast<const T*>(a.dy) + row * a.lddy, 0.f, c, l);
             if (a.h) {
-                if (a.pkind >= 0) fh = normalise<VEC, L, P>(h, sum, a.pkind, c, inv_c, a.eps, l);
+                if (a.pkind >= 0) fh = normalise<L, P>(h, sum, a.pkind, c, inv_c, a.eps, l);
 #pragma unroll
                 for (int i = 0; i < N; ++i) v[i] = a.alpha * v[i] + pg[i] * h[i];
             }
             if (a.dy) {
-                const float f = normalise<VEC, L, P>(v, sum, a.kind, c, inv_c, a.eps, l);
+                const float f = normalise<L, P>(v, sum, a.kind, c, inv_c, a.eps, l);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     s1[i] += g[i] * v[i];
                     s2[i] += g[i];
                     g[i] *= wa[i];
                 }
-                norm_gradient<VEC, L, P>(g, v, f, sum, a.kind, c, inv_c, l);
+                norm_gradient<L, P>(g, v, f, sum, a.kind, c, inv_c, l);
 #pragma unroll
                 for (int i = 0; i < N; ++i) ds[i] = a.dout ? ds[i] + g[i] : g[i];
             }
             if (a.dx) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) v[i] = (a.h ? a.alpha : 1.f) * ds[i];
-                store_row<T, VEC, L, P>(v, a.dx, row, a.lddx, c, l);
+                store_row<T, TAIL, L, P>(v, static_cast<T*>(a.dx) + row * a.lddx, c, l);
             }
             if (a.h) {
 #pragma unroll
@@ -278,8 +248,8 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const NormArgs a) {
                     ds[i] *= pg[i];
                 }
                 if (a.dh) {
-                    if (a.pkind >= 0) norm_gradient<VEC, L, P>(ds, h, fh, sum, a.pkind, c, inv_c, l);
-                    store_row<T, VEC, L, P>(ds, a.dh, row, a.lddh, c, l);
+                    if (a.pkind >= 0) norm_gradient<L, P>(ds, h, fh, sum, a.pkind, c, inv_c, l);
+                    store_row<T, TAIL, L, P>(ds, static_cast<T*>(a.dh) + row * a.lddh, c, l);
                 }
             }
         }
@@ -293,7 +263,7 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const NormArgs a) {
                 if constexpr (ROWS == 1) {
 #pragma unroll
                     for (int i = 0; i < N; ++i) {
-                        const int col = column<VEC, L>(i >> 3, i & 7, l);
+                        const int col = column<L>(i >> 3, i & 7, l);
                         if (col < c) dst[(long long)k * c + col] = s[i];
                     }
                 } else {
@@ -302,7 +272,7 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const NormArgs a) {
                     for (int i = 0; i < N; ++i) cols[(group * N + i) * L + l] = s[i];
                     __syncthreads();
                     for (int q = threadIdx.x; q < L * N; q += 256) {
-                        const int i = q / L, col = column<VEC, L>(i >> 3, i & 7, q % L);
+                        const int i = q / L, col = column<L>(i >> 3, i & 7, q % L);
                         float t = 0.f;
                         for (int gr = 0; gr < ROWS; ++gr) t += cols[(gr * N + i) * L + q % L];
                         if (col < c) dst[(long long)k * c + col] = t;
@@ -395,21 +365,13 @@ __global__ __launch_bounds__(1024) void norm_sample_sums_kernel(const SumArgs a)
 
 // Lanes and pieces of a row: a wave or less holds up to 1024 columns, 16 per lane; wider rows spread over the workgroup
 // (3711 float32 rows of 2048 columns forward: 29 us, 4.2 TB/s; with a wave per row and 32 columns per lane 95 us).
-struct Shape { bool vec; int lanes, pieces; };
+struct Shape { bool tail; int lanes, pieces; };
 
 Shape shape_of(const vdmi_block_norm_args* a) {
     const int g = (a->c + 7) / 8;
     Shape s;
-    const int64_t pitches[8] = {a->ldx, a->h ? a->ldh : 0, a->out ? a->ldo : 0, a->y ? a->ldy : 0, a->dout ? a->lddo : 0,
-                                a->dy ? a->lddy : 0, a->dx ? a->lddx : 0, a->dh ? a->lddh : 0};
-    const void* ps[8] = {a->x, a->h, a->out, a->y, a->dout, a->dy, a->dx, a->dh};
-    s.vec = a->c % 8 == 0;
-    for (int i = 0; i < 8; ++i) s.vec = s.vec && pitches[i] % 8 == 0 && aligned16(ps[i]);
-    if (s.vec && g <= 8) s.lanes = 8;
-    else if (s.vec && g <= 16) s.lanes = 16;
-    else if (s.vec && g <= 32) s.lanes = 32;
-    else if (g <= (s.vec ? 128 : 64)) s.lanes = 64;
-    else s.lanes = 256;
+    s.tail = a->c % 8 != 0;
+    s.lanes = g <= 8 ? 8 : g <= 16 ? 16 : g <= 32 ? 32 : g <= 128 ? 64 : 256;
     s.pieces = (g + s.lanes - 1) / s.lanes;
     if (s.pieces == 3) s.pieces = 4;
     return s;
@@ -470,27 +432,18 @@ int check_norm(const vdmi_block_norm_args* a, bool bwd) {
 
 template <typename T, bool BWD>
 int launch_norm(const NormArgs& n, const Shape& s, unsigned grid, hipStream_t st) {
-#define NORM(V, L, P) hipLaunchKernelGGL((block_norm_kernel<T, V, L, P, BWD>), dim3(grid), dim3(256), 0, st, n)
-    if (s.vec) {
-        switch (s.lanes * 8 + s.pieces) {
-            case 8 * 8 + 1: NORM(true, 8, 1); break;
-            case 16 * 8 + 1: NORM(true, 16, 1); break;
-            case 32 * 8 + 1: NORM(true, 32, 1); break;
-            case 64 * 8 + 1: NORM(true, 64, 1); break;
-            case 64 * 8 + 2: NORM(true, 64, 2); break;
-            case 256 * 8 + 1: NORM(true, 256, 1); break;
-            case 256 * 8 + 2: NORM(true, 256, 2); break;
-            case 256 * 8 + 4: NORM(true, 256, 4); break;
-            default: return VDMI_E_SHAPE;
-        }
-    } else {
-        switch (s.lanes * 8 + s.pieces) {
-            case 64 * 8 + 1: NORM(false, 64, 1); break;
-            case 256 * 8 + 1: NORM(false, 256, 1); break;
-            case 256 * 8 + 2: NORM(false, 256, 2); break;
-            case 256 * 8 + 4: NORM(false, 256, 4); break;
-            default: return VDMI_E_SHAPE;
-        }
+#define NORM(L, P) do { if (s.tail) hipLaunchKernelGGL((block_norm_kernel<T, true, L, P, BWD>), dim3(grid), dim3(256), 0, st, n); \
+                        else hipLaunchKernelGGL((block_norm_kernel<T, false, L, P, BWD>), dim3(grid), dim3(256), 0, st, n); } while (0)
+    switch (s.lanes * 8 + s.pieces) {
+        case 8 * 8 + 1: NORM(8, 1); break;
+        case 16 * 8 + 1: NORM(16, 1); break;
+        case 32 * 8 + 1: NORM(32, 1); break;
+        case 64 * 8 + 1: NORM(64, 1); break;
+        case 64 * 8 + 2: NORM(64, 2); break;
+        case 256 * 8 + 1: NORM(256, 1); break;
+        case 256 * 8 + 2: NORM(256, 2); break;
+        case 256 * 8 + 4: NORM(256, 4); break;
+        default: return VDMI_E_SHAPE;
     }
 #undef NORM
     VDMI_LAUNCH_CHECK();
