@@ -711,10 +711,11 @@ int vdmi_decay_attn_step(const void* q, const void* k, const void* v, void* o, c
  * VDMI_NORM_RMS t / sqrt(mean t^2 + eps), VDMI_NORM_LAYER (t - mean) / sqrt(var + eps), post_kind also VDMI_NORM_NONE
  * (P(h) = h).  weight, post_weight: float [c] or NULL (ones).  gate (NULL: ones), scale, shift (NULL: zeros): float, one row
  * of c for all rows (stride 0) or one per sample of rows_per_sample consecutive rows (stride c).  Any pitch and element
- * alignment; multiples of 8 elements at 16-byte aligned addresses take the wide-load form.
+ * alignment.
  * Backward: from x, h and the gradients dout (of out, or of sum where h is NULL and it is used elsewhere) and dy, either
  * NULL for zeros, the gradients dx, dh and, summed over the rows in a fixed order, of the parameters (each NULL where not
- * wanted; dgate, dscale, dshift have the layout of gate, scale, shift; at most 65535 samples where any is wanted).
+ * wanted; dgate, dscale, dshift have the layout of gate, scale, shift).
+ * No output may overlap an input.
  * workspace: vdmi_block_norm_bwd_workspace_bytes() bytes, 16-byte aligned, contents irrelevant.
  * ------------------------------------------------------------------------------------------ */
 enum vdmi_norm_kind { VDMI_NORM_NONE = -1, VDMI_NORM_RMS = 0, VDMI_NORM_LAYER = 1 };
@@ -743,10 +744,11 @@ int vdmi_block_norm_bwd(const vdmi_block_norm_args* a, vdmi_stream stream);
  * Activation checkpoints in 8 bits (no counterpart in the reference, which keeps what autograd saves): rows [rows][c], c a
  * multiple of 8, as codes uint8 [rows][c] (e4m3: 4 exponent, 3 fraction bits, largest 448, no infinities) and exps uint8
  * [rows][ceil(c / 32)] (e + 127): x ~ code 2^e, e per row and 32 consecutive channels the least exponent whose 448 2^e holds
- * the group's largest finite magnitude, in -118 .. 119 (magnitudes beyond 448 2^119 become that); rounded to nearest even; infinities and NaN become NaN.
+ * the group's largest finite magnitude, in -118 .. 119 (magnitudes beyond 448 2^119 become that); rounded to nearest even;
+ * infinities and NaN become NaN.
  * vdmi_rows8_wgrad: weight gradient of a Linear whose input was kept, dw float [cout][cin] = sum_r dy[r][o] x[r][i], from
- * the codes and bf16 rows dy [rows][cout] (pitch lddy, at most VDMI_ROWS8_MAX_PITCH), and db float [cout] = sum_r dy[r][o] (NULL: not wanted); cin, cout
- * multiples of 8; workspace as stated by vdmi_rows8_wgrad_workspace_bytes().
+ * the codes and bf16 rows dy [rows][cout] (pitch lddy, at most VDMI_ROWS8_MAX_PITCH), and db float [cout] = sum_r dy[r][o]
+ * (NULL: not wanted); cin, cout multiples of 8; workspace as stated by vdmi_rows8_wgrad_workspace_bytes().
  * ------------------------------------------------------------------------------------------ */
 #define VDMI_ROWS8_MAX_PITCH (1LL << 23)
 int vdmi_rows8_pack(const void* x, int64_t ldx, void* codes, void* exps, int dtype, int64_t rows, int c, vdmi_stream stream);

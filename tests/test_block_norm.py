@@ -101,6 +101,14 @@ def test_widths(c, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("c", [2, 5, 7, 9, 15, 17, 63, 65, 127, 129, 255, 257, 511, 513, 1023, 1025, 2047, 2049, 4095, 4097, 8191])
+def test_odd_widths(c, dtype):
+    """Rows whose last piece overlaps the one before, or that are shorter than a piece."""
+    check(f"odd{c}.{dtype}", *make((2, 37, c), dtype, c + 1), alpha=0.7, kind="layer" if c > 8 else "rms", eps=0.5 if c < 8 else 1e-5)
+
+
+@gpu
 @pytest.mark.parametrize("kind", ["rms", "layer"])
 @pytest.mark.parametrize("post_kind", ["rms", "layer", None])
 @pytest.mark.parametrize("shape", [(1, 1, 64), (2, 1, 64), (5, 333, 64), (2, 3, 5, 7, 96), (4, 2500, 32), (7, 512)])

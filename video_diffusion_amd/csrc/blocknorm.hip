@@ -57,66 +57,84 @@ struct RowSum {                         // sums over the L lanes of a row; L == 
     }
 };
 
-// column of element e of piece p: eight consecutive ones of a row, loaded and stored 16 bytes at a time at any alignment of
-// the elements.  TAIL: the columns are no multiple of eight, and the row's last piece goes element by element.
-template <int L>
-__device__ __forceinline__ int column(int p, int e, int l) { return (p * L + l) * 8 + e; }
+// A lane's pieces of eight consecutive columns, loaded and stored 16 bytes at a time at any alignment of the elements.
+// TAIL: the columns are no multiple of eight; the row's last piece then begins eight columns before its end and holds some
+// columns twice.  Both copies are computed and stored alike, sums take those from own[] on.  (160000 bfloat16 rows of 301
+// columns, forward / backward: 113 / 189 us; the last piece element by element 157 / 362; the whole row so 189 / 440.)
+// Rows of less than eight columns begin before their start: they go element by element from own[] on.
+template <bool TAIL, int L, int P>
+struct Columns {
+    int c, start[P], own[P];
+    __device__ __forceinline__ Columns(int c, int l) : c(c) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int at = (p * L + l) * 8;
+            start[p] = TAIL ? min(at, c - 8) : at;
+            own[p] = at < c ? at - start[p] : 8;
+        }
+    }
+    __device__ __forceinline__ bool there(int p) const { return TAIL ? own[p] < 8 : start[p] < c; }
+    // of element i = 8 p + e
+    __device__ __forceinline__ bool mine(int i) const { return TAIL ? (i & 7) >= own[i >> 3] : there(i >> 3); }
+    // what element i adds to a sum (elements that are not there are zeros)
+    __device__ __forceinline__ float part(float v, int i) const { return !TAIL || mine(i) ? v : 0.f; }
+};
 
 template <typename T, bool TAIL, int L, int P>
-__device__ __forceinline__ void load_row(float (&v)[P * 8], const T* r, float absent, int c, int l) {
+__device__ __forceinline__ void load_row(float (&v)[P * 8], const T* r, float absent, const Columns<TAIL, L, P>& at) {
     constexpr int W = 16 / sizeof(T);
     typedef T wide __attribute__((ext_vector_type(W), aligned(sizeof(T))));
     T x[P * 8];
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-        const int col = column<L>(p, 0, l);
+    for (int i = 0; i < P * 8; ++i) x[i] = (T)absent;
+    if (!TAIL || at.c >= 8) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[8 * p + e] = (T)absent;
-        if (TAIL ? col + 8 <= c : col < c) {
+        for (int p = 0; p < P; ++p)
+            if (at.there(p)) {
 #pragma unroll
-            for (int i = 0; i < 8 / W; ++i) {
-                const wide a = *reinterpret_cast<const wide*>(r + col + W * i);
+                for (int i = 0; i < 8 / W; ++i) {
+                    const wide a = *reinterpret_cast<const wide*>(r + at.start[p] + W * i);
 #pragma unroll
-                for (int e = 0; e < W; ++e) x[8 * p + W * i + e] = a[e];
+                    for (int e = 0; e < W; ++e) x[8 * p + W * i + e] = a[e];
+                }
             }
-        } else if (TAIL) {
+    } else {
 #pragma unroll
-            for (int e = 0; e < 7; ++e)
-                if (col + e < c) x[8 * p + e] = r[col + e];
-        }
+        for (int e = 1; e < 8; ++e)
+            if (at.mine(e)) x[e] = r[at.start[0] + e];
     }
 #pragma unroll
     for (int i = 0; i < P * 8; ++i) v[i] = (float)x[i];
 }
 
 template <typename T, bool TAIL, int L, int P>
-__device__ __forceinline__ void store_row(const float (&v)[P * 8], T* r, int c, int l) {
+__device__ __forceinline__ void store_row(const float (&v)[P * 8], T* r, const Columns<TAIL, L, P>& at) {
     constexpr int W = 16 / sizeof(T);
     typedef T wide __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+    if (!TAIL || at.c >= 8) {
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-        const int col = column<L>(p, 0, l);
-        if (TAIL ? col + 8 <= c : col < c) {
+        for (int p = 0; p < P; ++p)
+            if (at.there(p)) {
 #pragma unroll
-            for (int i = 0; i < 8 / W; ++i) {
-                wide a;
+                for (int i = 0; i < 8 / W; ++i) {
+                    wide a;
 #pragma unroll
-                for (int e = 0; e < W; ++e) a[e] = (T)v[8 * p + W * i + e];
-                *reinterpret_cast<wide*>(r + col + W * i) = a;
+                    for (int e = 0; e < W; ++e) a[e] = (T)v[8 * p + W * i + e];
+                    *reinterpret_cast<wide*>(r + at.start[p] + W * i) = a;
+                }
             }
-        } else if (TAIL) {
+    } else {
 #pragma unroll
-            for (int e = 0; e < 7; ++e)
-                if (col + e < c) r[col + e] = (T)v[8 * p + e];
-        }
+        for (int e = 1; e < 8; ++e)
+            if (at.mine(e)) r[at.start[0] + e] = (T)v[e];
     }
 }
 
 // the lane's columns of a parameter row, `absent` where there is none
 template <bool TAIL, int L, int P>
-__device__ __forceinline__ void load_params(float (&v)[P * 8], const float* src, float absent, int c, int l) {
+__device__ __forceinline__ void load_params(float (&v)[P * 8], const float* src, float absent, const Columns<TAIL, L, P>& at) {
     if (src) {
-        load_row<float, TAIL, L, P>(v, src, absent, c, l);
+        load_row<float, TAIL, L, P>(v, src, absent, at);
     } else {
 #pragma unroll
         for (int i = 0; i < P * 8; ++i) v[i] = absent;
@@ -124,20 +142,21 @@ __device__ __forceinline__ void load_params(float (&v)[P * 8], const float* src,
 }
 
 // v -> its norm in place; returns the factor
-template <int L, int P>
-__device__ __forceinline__ float normalise(float (&v)[P * 8], RowSum<L>& sum, int kind, int c, float inv_c, float eps, int l) {
+template <bool TAIL, int L, int P>
+__device__ __forceinline__ float normalise(float (&v)[P * 8], RowSum<L>& sum, int kind, float inv_c, float eps,
+                                           const Columns<TAIL, L, P>& at) {
     if (kind == 1) {
         float s = 0.f, z = 0.f;
 #pragma unroll
-        for (int i = 0; i < P * 8; ++i) s += v[i];
+        for (int i = 0; i < P * 8; ++i) s += at.part(v[i], i);
         sum.two(s, z);
         const float mean = s * inv_c;
 #pragma unroll
-        for (int i = 0; i < P * 8; ++i) v[i] = column<L>(i >> 3, i & 7, l) < c ? v[i] - mean : 0.f;
+        for (int i = 0; i < P * 8; ++i) v[i] = at.there(i >> 3) ? v[i] - mean : 0.f;
     }
     float s = 0.f, z = 0.f;
 #pragma unroll
-    for (int i = 0; i < P * 8; ++i) s += v[i] * v[i];
+    for (int i = 0; i < P * 8; ++i) s += at.part(v[i] * v[i], i);
     sum.two(s, z);
     const float f = 1.f / __builtin_sqrtf(s * inv_c + eps);
 #pragma unroll
@@ -146,21 +165,21 @@ __device__ __forceinline__ float normalise(float (&v)[P * 8], RowSum<L>& sum, in
 }
 
 // g (gradient of a norm's result n) -> f (g - mean g - n mean(g n)); the plain mean for the layer norm
-template <int L, int P>
-__device__ __forceinline__ void norm_gradient(float (&g)[P * 8], const float (&n)[P * 8], float f, RowSum<L>& sum, int kind, int c,
-                                              float inv_c, int l) {
+template <bool TAIL, int L, int P>
+__device__ __forceinline__ void norm_gradient(float (&g)[P * 8], const float (&n)[P * 8], float f, RowSum<L>& sum, int kind,
+                                              float inv_c, const Columns<TAIL, L, P>& at) {
     float s = 0.f, t = 0.f;
 #pragma unroll
-    for (int i = 0; i < P * 8; ++i) { s += g[i]; t += g[i] * n[i]; }
+    for (int i = 0; i < P * 8; ++i) { s += at.part(g[i], i); t += at.part(g[i] * n[i], i); }
     sum.two(s, t);
     s = kind == 1 ? s * inv_c : 0.f;
     t *= inv_c;
 #pragma unroll
-    for (int i = 0; i < P * 8; ++i) g[i] = column<L>(i >> 3, i & 7, l) < c ? f * (g[i] - s - n[i] * t) : 0.f;
+    for (int i = 0; i < P * 8; ++i) g[i] = at.there(i >> 3) ? f * (g[i] - s - n[i] * t) : 0.f;
 }
 
 template <typename T, bool TAIL, int L, int P, bool BWD>
-__global__ __launch_bounds__(256) void block_norm_kernel(const NormArgs a) {
+__global__ __launch_bounds__(256, P == 1 ? 4 : 1) void block_norm_kernel(const NormArgs a) {
     constexpr int N = P * 8, ROWS = 256 / L;
     __shared__ float slots[2][2][4];
     __shared__ float cols[BWD && ROWS > 1 ? ROWS * L * N : 1];
@@ -171,23 +190,24 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const NormArgs a) {
     const long long first = (long long)part * a.rows_per_wg;
     const long long last = min(first + a.rows_per_wg, a.rows_per_sample);
     const float inv_c = 1.f / (float)c;
+    const Columns<TAIL, L, P> at(c, l);
     // per column: a = weight (1 + scale), gate * post_weight, shift
     float wa[N], pg[N], sh[BWD ? 1 : N];
-    load_params<TAIL, L, P>(wa, a.w, 1.f, c, l);
-    load_params<TAIL, L, P>(pg, a.pw, 1.f, c, l);
+    load_params<TAIL, L, P>(wa, a.w, 1.f, at);
+    load_params<TAIL, L, P>(pg, a.pw, 1.f, at);
     if (a.scale) {
         float t[N];
-        load_params<TAIL, L, P>(t, a.scale + sample * a.scale_bs, 0.f, c, l);
+        load_params<TAIL, L, P>(t, a.scale + sample * a.scale_bs, 0.f, at);
 #pragma unroll
         for (int i = 0; i < N; ++i) wa[i] *= 1.f + t[i];
     }
     if (a.gate) {
         float t[N];
-        load_params<TAIL, L, P>(t, a.gate + sample * a.gate_bs, 0.f, c, l);
+        load_params<TAIL, L, P>(t, a.gate + sample * a.gate_bs, 0.f, at);
 #pragma unroll
         for (int i = 0; i < N; ++i) pg[i] *= t[i];
     }
-    if constexpr (!BWD) load_params<TAIL, L, P>(sh, a.shift ? a.shift + sample * a.shift_bs : nullptr, 0.f, c, l);
+    if constexpr (!BWD) load_params<TAIL, L, P>(sh, a.shift ? a.shift + sample * a.shift_bs : nullptr, 0.f, at);
     float s1[BWD ? N : 1], s2[BWD ? N : 1], s3[BWD ? N : 1];
     if constexpr (BWD) {
 #pragma unroll
@@ -199,47 +219,47 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const NormArgs a) {
         if (r >= last) continue;        // L <= 64: lanes of other rows are not involved in this one's sums
         const long long row = sample * a.rows_per_sample + r;
         float v[N], h[N];
-        load_row<T, TAIL, L, P>(v, static_cast<const T*>(a.x) + row * a.ldx, 0.f, c, l);
-        if (a.h) load_row<T, TAIL, L, P>(h, static_cast<const T*>(a.h) + row * a.ldh, 0.f, c, l);
+        load_row<T, TAIL, L, P>(v, static_cast<const T*>(a.x) + row * a.ldx, 0.f, at);
+        if (a.h) load_row<T, TAIL, L, P>(h, static_cast<const T*>(a.h) + row * a.ldh, 0.f, at);
         float fh = 1.f;
         if constexpr (!BWD) {
             if (a.h) {
-                if (a.pkind >= 0) normalise<L, P>(h, sum, a.pkind, c, inv_c, a.eps, l);
+                if (a.pkind >= 0) normalise<TAIL, L, P>(h, sum, a.pkind, inv_c, a.eps, at);
 #pragma unroll
                 for (int i = 0; i < N; ++i) v[i] = a.alpha * v[i] + pg[i] * h[i];
-                store_row<T, TAIL, L, P>(v, static_cast<T*>(a.out) + row * a.ldo, c, l);
+                store_row<T, TAIL, L, P>(v, static_cast<T*>(a.out) + row * a.ldo, at);
             }
             if (a.y) {
-                normalise<L, P>(v, sum, a.kind, c, inv_c, a.eps, l);
+                normalise<TAIL, L, P>(v, sum, a.kind, inv_c, a.eps, at);
 #pragma unroll
                 for (int i = 0; i < N; ++i) v[i] = v[i] * wa[i] + sh[i];
-                store_row<T, TAIL, L, P>(v, static_cast<T*>(a.y) + row * a.ldy, c, l);
+                store_row<T, TAIL, L, P>(v, static_cast<T*>(a.y) + row * a.ldy, at);
             }
         } else {
             float ds[N], g[N];
-            if (a.dout) load_row<T, TAIL, L, P>(ds, static_cast<const T*>(a.dout) + row * a.lddo, 0.f, c, l);
-            if (a.dy) load_row<T, TAIL, L, P>(g, static_cast<const T*>(a.dy) + row * a.lddy, 0.f, c, l);
+            if (a.dout) load_row<T, TAIL, L, P>(ds, static_cast<const T*>(a.dout) + row * a.lddo, 0.f, at);
+            if (a.dy) load_row<T, TAIL, L, P>(g, static_cast<const T*>(a.dy) + row * a.lddy, 0.f, at);
             if (a.h) {
-                if (a.pkind >= 0) fh = normalise<L, P>(h, sum, a.pkind, c, inv_c, a.eps, l);
+                if (a.pkind >= 0) fh = normalise<TAIL, L, P>(h, sum, a.pkind, inv_c, a.eps, at);
 #pragma unroll
                 for (int i = 0; i < N; ++i) v[i] = a.alpha * v[i] + pg[i] * h[i];
             }
             if (a.dy) {
-                const float f = normalise<L, P>(v, sum, a.kind, c, inv_c, a.eps, l);
+                const float f = normalise<TAIL, L, P>(v, sum, a.kind, inv_c, a.eps, at);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     s1[i] += g[i] * v[i];
                     s2[i] += g[i];
                     g[i] *= wa[i];
                 }
-                norm_gradient<L, P>(g, v, f, sum, a.kind, c, inv_c, l);
+                norm_gradient<TAIL, L, P>(g, v, f, sum, a.kind, inv_c, at);
 #pragma unroll
                 for (int i = 0; i < N; ++i) ds[i] = a.dout ? ds[i] + g[i] : g[i];
             }
             if (a.dx) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) v[i] = (a.h ? a.alpha : 1.f) * ds[i];
-                store_row<T, TAIL, L, P>(v, static_cast<T*>(a.dx) + row * a.lddx, c, l);
+                store_row<T, TAIL, L, P>(v, static_cast<T*>(a.dx) + row * a.lddx, at);
             }
             if (a.h) {
 #pragma unroll
@@ -248,8 +268,8 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const NormArgs a) {
                     ds[i] *= pg[i];
                 }
                 if (a.dh) {
-                    if (a.pkind >= 0) norm_gradient<L, P>(ds, h, fh, sum, a.pkind, c, inv_c, l);
-                    store_row<T, TAIL, L, P>(ds, static_cast<T*>(a.dh) + row * a.lddh, c, l);
+                    if (a.pkind >= 0) norm_gradient<TAIL, L, P>(ds, h, fh, sum, a.pkind, inv_c, at);
+                    store_row<T, TAIL, L, P>(ds, static_cast<T*>(a.dh) + row * a.lddh, at);
                 }
             }
         }
@@ -262,17 +282,16 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const NormArgs a) {
                 const float* s = k == 0 ? s1 : k == 1 ? s2 : s3;
                 if constexpr (ROWS == 1) {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const int col = column<L>(i >> 3, i & 7, l);
-                        if (col < c) dst[(long long)k * c + col] = s[i];
-                    }
+                    for (int i = 0; i < N; ++i)
+                        if (at.mine(i)) dst[(long long)k * c + at.start[i >> 3] + (i & 7)] = s[i];
                 } else {
                     __syncthreads();
 #pragma unroll
-                    for (int i = 0; i < N; ++i) cols[(group * N + i) * L + l] = s[i];
+                    for (int i = 0; i < N; ++i)
+                        if (!TAIL || at.mine(i)) cols[(group * N + i - (TAIL ? at.own[i >> 3] : 0)) * L + l] = s[i];
                     __syncthreads();
                     for (int q = threadIdx.x; q < L * N; q += 256) {
-                        const int i = q / L, col = column<L>(i >> 3, i & 7, q % L);
+                        const int i = q / L, col = ((i >> 3) * L + q % L) * 8 + (i & 7);     // by the pieces' places
                         float t = 0.f;
                         for (int gr = 0; gr < ROWS; ++gr) t += cols[(gr * N + i) * L + q % L];
                         if (col < c) dst[(long long)k * c + col] = t;
@@ -364,7 +383,8 @@ __global__ __launch_bounds__(1024) void norm_sample_sums_kernel(const SumArgs a)
 }
 
 // Lanes and pieces of a row: a wave or less holds up to 1024 columns, 16 per lane; wider rows spread over the workgroup
-// (3711 float32 rows of 2048 columns forward: 29 us, 4.2 TB/s; with a wave per row and 32 columns per lane 95 us).
+// (3711 float32 rows of 2048 columns forward: 29 us, 4.2 TB/s; with a wave per row and 32 columns per lane 95 us).  Kernels
+// of one piece per lane stay within 128 registers, four waves on a SIMD (301 columns backward: 189 us, with three 289).
 struct Shape { bool tail; int lanes, pieces; };
 
 Shape shape_of(const vdmi_block_norm_args* a) {
