@@ -29,7 +29,6 @@ _DTYPES = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16, torch.float
 _FLOAT16S = (torch.bfloat16, torch.float16)
 _I64x8 = C.c_int64 * 8
 
-
 _current_device, _raw_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
 _increment_version = torch.autograd.graph.increment_version
 
@@ -47,6 +46,16 @@ def _there(fn):
             return fn(t, *args)
         with torch.cuda.device(t.device):
             return fn(t, *args)
+    return inner
+
+
+def _first_order(backward):
+    """backward(ctx, *grads) whose own derivative raises; what that takes is only set up where a graph of it is asked for."""
+    once = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def inner(ctx, *grads):
+        return (once if torch.is_grad_enabled() else backward)(ctx, *grads)
     return inner
 
 
@@ -167,7 +176,7 @@ class DecayAttnFn(torch.autograd.Function):
         return o, last
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, do, dlast):
         if do is None and dlast is None:
             return (None,) * 8
@@ -366,7 +375,7 @@ class BlockNormFn(torch.autograd.Function):
         return out, y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout, dy):
         if dout is None and dy is None:
             return (None,) * 12
@@ -538,7 +547,7 @@ class LinearRows8Fn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     @_plain
     def backward(ctx, dy):
         weight, *kept = ctx.saved_tensors
