@@ -11,7 +11,7 @@
 namespace {
 
 // ---- pack: a lane holds 8 channels, four lanes a group ------------------------------------------------------------
-// What bounds it: memory.
+// What bounds it: memory.  262144 bfloat16 rows of 256 channels (203 MB): 42 us, 4.8 TB/s; back 31 us, 6.6 TB/s.
 struct PackArgs {
     const void* x;
     unsigned char* codes;       // [rows][c]
@@ -126,8 +126,11 @@ __global__ __launch_bounds__(256) void rows8_unpack_kernel(const UnpackArgs a) {
 // and the fragments are read with ds_read_b64_tr_b16.  A workgroup owns 128 x 128 of dw for a share of the rows, four waves
 // 64 x 64 each; LDS rows are 320 bytes apart (the four rows x two column blocks of a half wave's read fall into different
 // banks).  Shares are added in a fixed order by a second launch.  The bias gradient sum_r dy comes from the staged pieces.
+// What bounds it: LDS - a wave reads 4 KB of fragments for four products of 32 cycles, what LDS gives four waves in that
+// time, and the staging comes on top.  131072 rows, 512 -> 1536 channels: 243 to 300 us (690 to 850 TFLOP/s) and 17 us for
+// the shares' sums; bfloat16 rows through vdmi_rows_wgrad 414, the library's product 709.  A 256 x 128 tile (128 x 64 per
+// wave, three quarters of the LDS reads, one workgroup per CU) took 341, one stage ahead in registers in place of two 392.
 constexpr int WK = 64, WT = 128, WPITCH = 320;
-constexpr double WSTAGE_US = 0.7;
 
 struct Wgrad8Args {
     const unsigned char* codes; const unsigned char* exps;
@@ -258,23 +261,40 @@ __global__ __launch_bounds__(256, 2) void rows8_wgrad_kernel(const Wgrad8Args a)
     }
 }
 
+// The shares' sums: 32 x four consecutive columns of dw per workgroup, eight threads on each with every eighth share, their
+// sums added in order; the workgroups behind those of dw do the same for 32 columns of db.
 __global__ __launch_bounds__(256) void rows8_reduce_kernel(const float* part, const float* bpart, float* dw, float* db, int splits,
-                                                           int to, int ti, int cout, int cin) {
-    const long long tile = (long long)WT * WT, all = tile * to * ti;
-    const long long q = (long long)blockIdx.x * 256 + threadIdx.x;          // four consecutive columns
-    if (q < all / 4) {
-        const long long e = q * 4, t = e / tile, in = e - t * tile;
-        const int o = (int)(t / ti) * WT + (int)(in / WT), i = (int)(t % ti) * WT + (int)(in % WT);
-        if (o < cout && i < cin) {              // cin is a multiple of 8: four columns are in or out together
-            f32x4 s = {0.f, 0.f, 0.f, 0.f};
-            for (int k = 0; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(part + k * all + e);
-            *reinterpret_cast<f32x4*>(dw + (long long)o * cin + i) = s;
+                                                           int to, int ti, int cout, int cin, unsigned dw_wgs) {
+    __shared__ f32x4 sums[8][32];
+    const int slot = threadIdx.x & 31, g = threadIdx.x >> 5;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (blockIdx.x < dw_wgs) {
+        const long long e = ((long long)blockIdx.x * 32 + slot) * 4;        // cin is a multiple of 8: within a row
+        const int o = (int)(e / cin), i = (int)(e - (long long)o * cin);
+        if (o < cout) {
+            const long long all = (long long)WT * WT * to * ti;
+            const float* p = part + ((long long)(o / WT) * ti + i / WT) * (WT * WT) + (o % WT) * WT + i % WT;
+#pragma unroll 4
+            for (int k = g; k < splits; k += 8) s += *reinterpret_cast<const f32x4*>(p + k * all);
         }
-    }
-    if (db && q < (long long)to * WT && q < cout) {
-        float s = 0.f;
-        for (int k = 0; k < splits; ++k) s += bpart[(long long)k * to * WT + q];
-        db[q] = s;
+        sums[g][slot] = s;
+        __syncthreads();
+        if (g == 0 && o < cout) {
+#pragma unroll
+            for (int j = 1; j < 8; ++j) s += sums[j][slot];
+            *reinterpret_cast<f32x4*>(dw + e) = s;
+        }
+    } else {
+        const long long q = (long long)(blockIdx.x - dw_wgs) * 32 + slot;
+        if (q < cout)
+            for (int k = g; k < splits; k += 8) s[0] += bpart[(long long)k * to * WT + q];
+        sums[g][slot] = s;
+        __syncthreads();
+        if (g == 0 && q < cout) {
+#pragma unroll
+            for (int j = 1; j < 8; ++j) s[0] += sums[j][slot][0];
+            db[q] = s[0];
+        }
     }
 }
 
@@ -285,20 +305,23 @@ int wgrad8_plan(int cin, int cout, int64_t rows, Wgrad8Plan* p) {
     p->to = (cout + WT - 1) / WT;
     p->ti = (cin + WT - 1) / WT;
     const long long tiles = (long long)p->to * p->ti, stages = (rows + WK - 1) / WK;
-    // Shares of the rows: 1, 2, 4 or a multiple of 8 (whole XCDs).  512 workgroups run at once (80 KB of LDS each); a stage
-    // takes WSTAGE of a microsecond, a share's partial sums 128 KB of traffic per tile.
+    // Shares of the rows: 1, 2, 4 or a multiple of 8 (whole XCDs).  512 workgroups run at once (80 KB of LDS each); a stage of
+    // 64 rows takes 0.76 us of a workgroup that has a CU to itself and 1.1 us of two on one CU; a share's partial sums are
+    // 128 KB of traffic per tile, at 4 TB/s.  Shares: measured us (with the second launch), rows x cin x cout
+    //     131072 x 512 x 1536:  8: 293   16: 292   32: 276   48: 288   64: 299        300 x 512 x 512:  1: 13   2: 12   4: 11
+    //     131072 x 256 x 256:   8: 203   32: 60   64: 39   128: 37        4096 x 1024 x 1024:  1: 59   2: 36   4: 27   8: 32
     long long splits = 1;
     double best = 1e30;
-    for (long long k = 1; k <= 128 && k <= stages; k += k < 2 ? 1 : k < 4 ? 2 : k < 8 ? 4 : 8) {
+    for (long long k = 1; k <= 256 && k <= stages; k += k < 2 ? 1 : k < 4 ? 2 : k < 8 ? 4 : 8) {
         const long long per = (stages + k - 1) / k;
         const long long rounds = k % 8 ? (tiles * k + 511) / 512 : (tiles * (k / 8) + 63) / 64;
-        const double us = rounds * per * WSTAGE_US + 128e3 * tiles * k / 4e6;
+        const double us = rounds * per * (tiles * k <= 256 ? 0.76 : 1.1) + 128e3 * tiles * k / 4e6;
         if (us < best) { best = us; splits = k; }
     }
     const long long per = (stages + splits - 1) / splits;
     p->per = per * WK;
     p->splits = (int)splits;            // the last ones may be empty: a multiple of 8 stays one
-    if (tiles * p->splits > 0x7fffffffLL) return VDMI_E_SHAPE;
+    if (tiles * p->splits > 0x7fffffffLL || (long long)cin * cout > (0x7fffffffLL - (1 << 20)) * 128) return VDMI_E_SHAPE;
     p->part = (size_t)tiles * p->splits * WT * WT * sizeof(float);
     p->bytes = p->part + (size_t)p->splits * p->to * WT * sizeof(float);
     return VDMI_OK;
@@ -371,9 +394,9 @@ extern "C" int vdmi_rows8_wgrad(const void* codes, const void* exps, const void*
     a.cin = cin; a.cout = cout; a.groups = (cin + 31) / 32; a.to = p.to; a.ti = p.ti; a.splits = p.splits;
     hipLaunchKernelGGL(rows8_wgrad_kernel, dim3((unsigned)(p.to * p.ti * p.splits)), dim3(256), lds, st, a);
     VDMI_LAUNCH_CHECK();
-    const long long quads = (long long)p.to * p.ti * WT * WT / 4;
-    hipLaunchKernelGGL(rows8_reduce_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, a.part, a.bpart, dw, db, p.splits,
-                       p.to, p.ti, cout, cin);
+    const long long dw_wgs = ((long long)cout * cin + 127) / 128;
+    hipLaunchKernelGGL(rows8_reduce_kernel, dim3((unsigned)(dw_wgs + (db ? (cout + 31) / 32 : 0))), dim3(256), 0, st, a.part, a.bpart,
+                       dw, db, p.splits, p.to, p.ti, cout, cin, (unsigned)dw_wgs);
     VDMI_LAUNCH_CHECK();
     return VDMI_OK;
 }
