@@ -162,18 +162,31 @@ def _decay_backward(q, k, v, state, log_decay, lengths, fwd_ws, scale, do, dlast
     return dq, dk, dv, dstate
 
 
+def _decay_operands(q, k, v, state):
+    """q, k, v [b, inner, n, heads, d] and the state as the kernels read them, of [b, n, heads, d] or the former."""
+    if q.dim() == 4:
+        q, k, v = q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1)
+        state = None if state is None else state.unsqueeze(1)
+    if state is not None:
+        state = state.contiguous()
+        if state.data_ptr() & 15:
+            state = state.clone()
+    return _row_operand(q), _row_operand(k), _row_operand(v), state
+
+
 class DecayAttnFn(torch.autograd.Function):
-    """o (and the state after the last token) of q, k, v [b, inner, n, heads, d] and a first state; constants log_decay,
+    """o (and the state after the last token) of q, k, v [b(, sites), n, heads, d] and a first state; constants log_decay,
     lengths, scale."""
 
     @staticmethod
     def forward(ctx, q, k, v, state, log_decay, lengths, scale, return_state):
-        q, k, v = _row_operand(q), _row_operand(k), _row_operand(v)
-        o, last, ws = _decay_forward(q, k, v, state, log_decay, lengths, scale, return_state)
-        ctx.save_for_backward(q, k, v, state, log_decay, lengths, ws)
+        ctx.sites = q.dim() == 5
+        ops = _decay_operands(q, k, v, state)
+        o, last, ws = _decay_forward(*ops, log_decay, lengths, scale, return_state)
+        ctx.save_for_backward(*ops, log_decay, lengths, ws)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
-        return o, last
+        return (o, last) if ctx.sites else (o.squeeze(1), None if last is None else last.squeeze(1))
 
     @staticmethod
     @_first_order
@@ -181,7 +194,12 @@ class DecayAttnFn(torch.autograd.Function):
         if do is None and dlast is None:
             return (None,) * 8
         need = ctx.needs_input_grad
-        dq, dk, dv, dstate = _decay_backward(*ctx.saved_tensors, ctx.scale, do, dlast, need[3])
+        if not (ctx.sites or do is None):
+            do = do.unsqueeze(1)
+        grads = _decay_backward(*ctx.saved_tensors, ctx.scale, do, dlast, need[3])
+        if not ctx.sites:
+            grads = [None if g is None else g.squeeze(1) for g in grads]
+        dq, dk, dv, dstate = grads
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dstate, None, None, None, None)
 
 
@@ -241,21 +259,14 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengt
         if not return_state:
             return o
         return o, (torch.zeros(*lead, heads, d, d, device=q.device) if initial_state is None else initial_state.clone())
-    if dims == 4:
-        q, k, v = q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1)
-    state = initial_state
-    if state is not None:
-        state = state.reshape(*q.shape[:2], heads, d, d).contiguous()
-        if state.data_ptr() & 15:
-            state = state.clone()
     log_decay = log_decay.contiguous()
-    if _wants_grad(q, k, v, state):
-        o, last = DecayAttnFn.apply(q, k, v, state, log_decay, lengths, scale, bool(return_state))
-    else:
-        o, last, _ = _decay_forward(_row_operand(q), _row_operand(k), _row_operand(v), state, log_decay, lengths, scale, return_state)
+    if _wants_grad(q, k, v, initial_state):
+        o, last = DecayAttnFn.apply(q, k, v, initial_state, log_decay, lengths, scale, bool(return_state))
+        return (o, last) if return_state else o
+    o, last, _ = _decay_forward(*_decay_operands(q, k, v, initial_state), log_decay, lengths, scale, return_state)
     if dims == 4:
-        o = o.squeeze(1)
-    return (o, last.view(*lead, heads, d, d)) if return_state else o
+        o, last = o.squeeze(1), None if last is None else last.squeeze(1)
+    return (o, last) if return_state else o
 
 
 def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
