@@ -50,3 +50,11 @@ def record(name, err, bar=None):
     """Remember a measured error (and the bar it was held to) under `name`; returns err."""
     PARITY_LOG[name] = {"rel_err": float(err), "bar": bar}
     return err
+
+
+def new_graph():
+    """A CUDAGraph once garbage is collected: while any graph captured in inference mode lives (the sampling loops' are),
+    torch refuses to begin a capture outside of it, because all graphs share their random state."""
+    import gc
+    gc.collect()
+    return torch.cuda.CUDAGraph()

@@ -10,7 +10,7 @@ once as the convolution's input, each v / sqrt(3): under 4 v / sqrt(3)."""
 import pytest
 import torch
 
-from tests.helpers import record, rel_err
+from tests.helpers import new_graph, record, rel_err
 
 gpu = pytest.mark.gpu
 DEV = "cuda:0"
@@ -133,7 +133,7 @@ def test_layer_in_a_graph():
     with torch.cuda.stream(side):
         run()
     torch.cuda.current_stream().wait_stream(side)
-    graph = torch.cuda.CUDAGraph()
+    graph = new_graph()
     with torch.cuda.graph(graph):
         outs = run()
     g = torch.Generator(device=DEV).manual_seed(3)

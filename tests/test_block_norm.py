@@ -10,7 +10,7 @@ import ctypes as C
 import pytest
 import torch
 
-from tests.helpers import record, rel_err
+from tests.helpers import new_graph, record, rel_err
 from video_diffusion_amd import _lib
 
 gpu = pytest.mark.gpu
@@ -240,7 +240,7 @@ def test_same_bits_streams_and_graph():
     with torch.cuda.stream(side):
         run()
     torch.cuda.synchronize()
-    graph = torch.cuda.CUDAGraph()
+    graph = new_graph()
     with torch.cuda.graph(graph):
         outs = run()
     g = torch.Generator(device=DEV).manual_seed(10)

@@ -11,7 +11,7 @@ import ctypes as C
 import pytest
 import torch
 
-from tests.helpers import record, rel_err
+from tests.helpers import new_graph, record, rel_err
 from video_diffusion_amd import _lib
 
 gpu = pytest.mark.gpu
@@ -346,7 +346,7 @@ def test_captured_and_replayed(n, state):
     with torch.cuda.stream(side):
         run()
     torch.cuda.current_stream().wait_stream(side)
-    graph = torch.cuda.CUDAGraph()
+    graph = new_graph()
     with torch.cuda.graph(graph):
         outs = run()
     g = torch.Generator(device=DEV).manual_seed(77)

@@ -8,7 +8,7 @@ import ctypes as C
 import pytest
 import torch
 
-from tests.helpers import record, rel_err
+from tests.helpers import new_graph, record, rel_err
 from video_diffusion_amd import _lib
 
 gpu = pytest.mark.gpu
@@ -185,7 +185,7 @@ def test_graph_and_streams():
             res.append(run())
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for r in res for a, b in zip(r, want))
-    graph = torch.cuda.CUDAGraph()
+    graph = new_graph()
     with torch.cuda.graph(graph):
         outs = run()
     for seed in range(3):
