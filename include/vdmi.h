@@ -664,7 +664,7 @@ void vdmi_sla_rows_mfma_enable(int on);
  * are constants.  A token that is not finite makes the outputs from it on not finite and may make earlier ones of its own
  * sequence so; other sequences are unaffected.
  * Sequences of up to 32 tokens without states share 32-row tiles (one launch forward, one backward).  Others are scanned;
- * few long ones in segments, which takes `workspace` (vdmi_decay_attn_workspace_bytes() bytes, 16-byte aligned, contents
+ * few of them in segments, which takes `workspace` (vdmi_decay_attn_workspace_bytes() bytes, 16-byte aligned, contents
  * irrelevant; as many for both directions, 0 where none is needed); the backward then also takes the forward call's
  * workspace as that call left it, in fwd_workspace.  Token strides (.n) from 0 to VDMI_DECAY_MAX_PITCH elements.
  * ------------------------------------------------------------------------------------------ */

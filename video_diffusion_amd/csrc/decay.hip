@@ -85,9 +85,30 @@ __device__ __forceinline__ float weigh(float p, float w) { return vdmi_mul_legac
 template <typename T> struct Low { static constexpr float SCALE = 1.f; static constexpr bool THREE = true; };
 template <> struct Low<_Float16> { static constexpr float SCALE = 2048.f; static constexpr bool THREE = false; };
 template <typename T>
-__device__ __forceinline__ T high_part(float x) { return (T)x; }
+__device__ __forceinline__ float above(float x) { return x; }
 template <>
-__device__ __forceinline__ _Float16 high_part<_Float16>(float x) { return (_Float16)(fabsf(x) < 0x1p-14f ? 0.f : x); }
+__device__ __forceinline__ float above<_Float16>(float x) { return fabsf(x) < 0x1p-14f ? 0.f : x; }
+
+// two values at a time: the conversions come in pairs
+template <typename T>
+struct Two {
+    typedef __attribute__((ext_vector_type(2))) T t2;
+    typedef __attribute__((ext_vector_type(2))) float f2;
+    // elements j, j + 1 of h = what T holds of a, b;  a, b become what is left, times SCALE
+    static __device__ __forceinline__ void take(x8_t<T>& h, int j, float& a, float& b) {
+        const t2 w = __builtin_convertvector((f2{above<T>(a), above<T>(b)}), t2);
+        const f2 back = __builtin_convertvector(w, f2);
+        h[j] = w[0];
+        h[j + 1] = w[1];
+        a = (a - back[0]) * Low<T>::SCALE;
+        b = (b - back[1]) * Low<T>::SCALE;
+    }
+    static __device__ __forceinline__ void round(x8_t<T>& h, int j, float a, float b) {
+        const t2 w = __builtin_convertvector((f2{a, b}), t2);
+        h[j] = w[0];
+        h[j + 1] = w[1];
+    }
+};
 
 template <typename T>
 struct Split {
@@ -98,12 +119,16 @@ struct Split {
         for (int s = 0; s < 2; ++s) {
             const f32x4 w0 = *reinterpret_cast<const f32x4*>(w + 16 * s + 4 * half), w1 = *reinterpret_cast<const f32x4*>(w + 16 * s + 8 + 4 * half);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = (float)(s ? v1 : v0)[j] * (j < 4 ? w0[j & 3] : w1[j & 3]);
-                h[s][j] = high_part<T>(x);
-                const float y = (x - (float)h[s][j]) * Low<T>::SCALE;
-                e[s][j] = (T)y;
-                if (Low<T>::THREE) f[s][j] = (T)(y - (float)e[s][j]);
+            for (int j = 0; j < 8; j += 2) {
+                float x = (float)(s ? v1 : v0)[j] * (j < 4 ? w0[j & 3] : w1[j & 3]);
+                float y = (float)(s ? v1 : v0)[j + 1] * (j < 4 ? w0[(j + 1) & 3] : w1[(j + 1) & 3]);
+                Two<T>::take(h[s], j, x, y);
+                if (Low<T>::THREE) {
+                    Two<T>::take(e[s], j, x, y);
+                    Two<T>::round(f[s], j, x, y);
+                } else {
+                    Two<T>::round(e[s], j, x, y);
+                }
             }
         }
     }
@@ -158,9 +183,10 @@ struct FineOperand {
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                h[s][j] = high_part<T>(p[8 * s + j]);
-                e[s][j] = (T)((p[8 * s + j] - (float)h[s][j]) * Low<T>::SCALE);
+            for (int j = 0; j < 8; j += 2) {
+                float x = p[8 * s + j], y = p[8 * s + j + 1];
+                Two<T>::take(h[s], j, x, y);
+                Two<T>::round(e[s], j, x, y);
             }
     }
     // o + (a0 | a1) times this
