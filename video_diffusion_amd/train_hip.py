@@ -514,7 +514,7 @@ class ResnetBlockFn(torch.autograd.Function):
         else:
             h2 = rmsnorm_silu_rows(y2, g2v, None, 0, f * hw)
             out = conv_rows(xr, param_pack(wres, False), bres.detach().float().contiguous(), frames, f, h, w, residual=h2)
-        ctx.rows8 = _ROWS8
+        ctx.rows8 = _ROWS8 and any(ctx.needs_input_grad)
         rows = (xr, y1, h1, y2)
         if ctx.rows8:
             from .block_hip import pack_rows8
