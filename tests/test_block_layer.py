@@ -244,3 +244,33 @@ def test_rows8_checkpoints_nest():
             assert T._ROWS8 is False
         assert T._ROWS8 is True
     assert T._ROWS8 is False
+
+
+@gpu
+def test_trainer_keeps_rows_in_8_bits(tmp_path, monkeypatch):
+    """Trainer.rows8_checkpoints: the blocks of every micro-step pack their rows, the first loss is the one without."""
+    from tests.test_training import _write_gifs
+    from video_diffusion_amd import GaussianDiffusion, Trainer, Unet3D, VAE, block_hip
+    folder = str(tmp_path / "gifs")
+    _write_gifs(folder, n=4, frames=6, size=36)
+    packs = []
+    real = block_hip.pack_rows8
+    monkeypatch.setattr(block_hip, "pack_rows8", lambda x: packs.append(tuple(x.shape)) or real(x))
+
+    def run(on):
+        packs.clear()
+        torch.manual_seed(0)
+        gd = GaussianDiffusion(Unet3D(dim=64, dim_mults=(1, 2), channels=4), VAE(channels=3, latent_dim=4, base_dim=64),
+                               image_size=32, num_frames=4, channels=3, timesteps=50).to(DEV)
+        tr = Trainer(gd, folder, num_prev_frames=2, train_batch_size=2, train_num_steps=2, gradient_accumulate_every=1,
+                     step_start_ema=0, update_ema_every=1, save_and_sample_every=10 ** 6, results_folder=str(tmp_path / f"r{on}"))
+        tr.train_backend = "hip"
+        tr.rows8_checkpoints = on
+        torch.manual_seed(1)
+        logs = []
+        tr.train(log_fn=logs.append)
+        return [l["loss"] for l in logs], len(packs)
+
+    (a, none), (b, some) = run(False), run(True)
+    assert none == 0 and some > 0 and some % 8 == 0          # four row sets a block, the same blocks in both steps
+    assert a[0] == b[0] and all(x == x and abs(x) < 1e30 for x in b)

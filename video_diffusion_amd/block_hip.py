@@ -241,7 +241,10 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengt
     [heads], at most 0, a constant.  scale: d^-0.5 by default.  initial_state: float32 [b(, sites), heads, d, d], S before
     the first token (zeros by default).  lengths: int32 [b(, sites)] - tokens from there on are padding: they are not read,
     their outputs and gradients are zeros.  return_state: also return S after the last token, for decay_attention_step or
-    the next piece of the sequence.  Returns o like q (in q's order of dimensions in memory), or (o, state)."""
+    the next piece of the sequence.  Returns o like q (in q's order of dimensions in memory), or (o, state).
+
+    Pairs scale * q_t k_j and states enter products as operands of q's dtype: in float16 they have to stay within 65504 (the
+    state that is returned is float32 throughout); decay_attention_step rounds neither."""
     dims = q.dim()
     if dims not in (4, 5):
         raise VdmiError(f"q is [b, n, heads, d] or [b, sites, n, heads, d] (got {dims} dimensions)")
