@@ -658,12 +658,13 @@ void vdmi_sla_rows_mfma_enable(int on);
  * dtype VDMI_DT_BF16 or VDMI_DT_F16 in either library build.
  * lengths: int32 [b*inner] or NULL - tokens from there on are not read, their rows of o (of dq, dk, dv) are zeros and
  * the state is the one after the last token.  state_in / state_out: float [b*inner][heads][d][d], the state before the
- * first and after the last token, either may be NULL (zeros / not wanted) and state_in may be state_out; state_in is 16-byte aligned.
+ * first and after the last token, either may be NULL (zeros / not wanted) and state_in may be state_out; state_in is
+ * 16-byte aligned.
  * Backward: from q, k, v, dout and dstate_in (gradient of the last state; NULL = zeros) the gradients dq, dk, dv and
  * dstate_out (of the first state; NULL = not wanted; state_in as in the forward, state_out unused).  log_decay and scale
  * are constants.  With halfs, m q_t k_j and the states' elements have to stay within 65504 (they are operands of products;
- * the state handed on is float throughout).  A token that is not finite makes the outputs from it on not finite and may make earlier ones of its own
- * sequence so; other sequences are unaffected.
+ * the state handed on is float throughout).  A token that is not finite makes the outputs from it on not finite and may
+ * make earlier ones of its own sequence so; other sequences are unaffected.
  * Sequences of up to 32 tokens without states share 32-row tiles (one launch forward, one backward).  Others are scanned;
  * few of them in segments, which takes `workspace` (vdmi_decay_attn_workspace_bytes() bytes, 16-byte aligned, contents
  * irrelevant; as many for both directions, 0 where none is needed); the backward then also takes the forward call's

@@ -25,9 +25,9 @@
 // (reading k and v only), a second one runs along the segments, a third computes all outputs.
 // Measured, 2 x 8192 tokens, 8 heads of 64 features, bfloat16 (16.8 MB a tensor): segments' sums 11.6 us (2.9 TB/s), along
 // the segments 6, outputs 18.6 (3.6 TB/s); backward dq 18.6, dk and dv 30.5 (3.9 TB/s) beside another walk for the segments.
-// 16384 tokens, 8 heads of 128, half: 26 + 8.4 + 42 us.  A wave has its SIMD almost to itself there and its tile is a chain
-// of dependent steps (products, weights, products, LDS, stores); twice the segments read and write twice the states and
-// gain nothing.
+// 16384 tokens, 8 heads of 128, half: 26 + 8.4 + 42 us.  There a wave has its SIMD to itself and bounds it by issuing: 61 % of
+// its cycles in the scan and 71 % in the gradients (conversions, weights and the state's decay 39 and 55 %), 20 % waiting.  Two
+// waves per SIMD hide that but take twice the segments, whose states cost as much.
 #include "block_common.h"
 
 #include <algorithm>
