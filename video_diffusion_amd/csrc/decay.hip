@@ -9,7 +9,7 @@
 //     dv : backward in time over (k, q, do) with R = dS / m, where R collects lambda^(i+1) q_i do_i^T
 //     dk : backward in time over (v, do, q), with R^T (one walk with dv);   the gradient of the first state is m R there
 //
-// What bounds it: memory.  A tile of one head takes 2 d (d + 32) products per token and tensor element moved - an order
+// What bounds it: memory, and the instructions of a tile where long sequences leave a wave alone on its SIMD.  A tile of one head takes 2 d (d + 32) products per token and tensor element moved - an order
 // under what the matrix cores do in the time the rows take - so the kernels are built to keep loads in flight: a wave
 // works alone on (sequence, head, segment, 32 columns of v), no barriers, its next tile's rows on their way while the
 // current tile is multiplied.  Layouts (v_mfma_f32_32x32x16: lane = row of A / column of B, 8 contraction values):
@@ -24,9 +24,9 @@
 // Few sequences: the time axis is cut into segments.  A first launch computes every segment's own contribution to the state
 // (reading k and v only), a second one runs along the segments, a third computes all outputs.
 // Measured, 2 x 8192 tokens, 8 heads of 64 features, bfloat16 (16.8 MB a tensor): segments' sums 11.6 us (2.9 TB/s), along
-// the segments 6, outputs 18.6 (3.6 TB/s); backward dq 18.6, dk and dv 30.5 (3.9 TB/s) beside another walk for the segments.
+// the segments 6, outputs 18.6 (3.6 TB/s); backward dq 18.6, dk and dv 25 (4.7 TB/s) beside another walk for the segments.
 // 16384 tokens, 8 heads of 128, half: 26 + 8.4 + 42 us.  There a wave has its SIMD to itself and bounds it by issuing: 61 % of
-// its cycles in the scan and 71 % in the gradients (conversions, weights and the state's decay 39 and 55 %), 20 % waiting.  Two
+// its cycles in the scan and 71 % in the gradients, 20 % waiting (2 x 8192 x 8 x 64).  Two
 // waves per SIMD hide that but take twice the segments, whose states cost as much.
 #include "block_common.h"
 
@@ -439,9 +439,11 @@ void decay_scan_kernel(const ScanArgs a) {
 // dk and dv in one walk backward in time: both read q, k, v and do, and what one of them needs of R = dS / m by columns the
 // other needs by rows.  A wave computes 32 columns of dv and the same 32 columns of dk and holds R[all dk][its columns of
 // dv] and R^T[all dv][its columns of dk].  Two walks, one for each, took 2 x 19 us and another pass over the segments where
-// this takes 30.5 (2 x 8192 tokens, 8 heads of 64).
+// this takes 25 (2 x 8192 tokens, 8 heads of 64).  With 64 features dv's half of a tile comes before dk's: that leaves 250
+// registers, none to move to and from the second file (both halves together 30.5 us; 32 x 500 x 8 x 64 39 and 32).  With 32 and
+// 128 features both halves at once are faster (16384 x 8 x 128, half: backward 137 and 144 us).
 template <typename T, int D, bool FINE>
-__global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(const GradArgs a) {
+__global__ __launch_bounds__(DW * 64, D <= 64 ? 2 : 1) void decay_grad_kernel(const GradArgs a) {
     typedef x8_t<T> x8;
     constexpr int KS = D / 16, KT = D / 32, KP = 2 * D + 16, RS = 512 / D;
     __shared__ __attribute__((aligned(16))) char qimg_all[DW][32 * KP];
@@ -465,7 +467,7 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
     // 128 features of bfloat16 leave no registers for the loads' offsets and the pairs' decays: the former are computed
     // again for every tile, the latter read from LDS.  (From scratch memory, where the compiler would put them, each one
     // waits for every load in flight: 16384 tokens, 8 heads took 205 us in place of 85.)
-    constexpr bool KEEP = D < 128 || !(Low<T>::THREE || FINE);
+    constexpr bool KEEP = D < 128 || !(Low<T>::THREE || FINE), HALVES = D == 64;
     unsigned qofs[KEEP ? KS : 1], gofs[KEEP ? KS : 1], kofs, vofs;
     auto row_at = [&](const Rows& r, int i, int cnt) { return r.at(lane / (D / 8) + RS * i, cnt, true, 16 * (lane % (D / 8))); };
     auto offsets = [&](int cnt) {
@@ -485,13 +487,20 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
             greg[i] = load16<T>(rg, KEEP ? gofs[i] : row_at(gr, i, cnt));
         }
     };
-    auto load_kv = [&](int t0, int cnt) {
-        const auto rk = kr.tile(at.len - t0 - cnt, cnt > 0), rv = vr.tile(at.len - t0 - cnt, cnt > 0);
+    auto load_k = [&](int t0, int cnt) {
+        const auto r = kr.tile(at.len - t0 - cnt, cnt > 0);
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            k[i] = load16<T>(rk, kofs + 32 * i);
-            v[i] = load16<T>(rv, vofs + 32 * i);
-        }
+        for (int i = 0; i < KS; ++i) k[i] = load16<T>(r, kofs + 32 * i);
+    };
+    auto load_v = [&](int t0, int cnt) {
+        const auto r = vr.tile(at.len - t0 - cnt, cnt > 0);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) v[i] = load16<T>(r, vofs + 32 * i);
+    };
+    auto pairs_times = [&](const f32x16& p, const x8& x0, const x8& x1, f32x16 o) {
+        if constexpr (FINE) return FineOperand<T>(p).times(x0, x1, o);
+        o = mfma16(x0, acc_operand<T>(p, 0), o);
+        return mfma16(x1, acc_operand<T>(p, 1), o);
     };
     const char* qtr = qimg + tr_offset(lane, KP);
     const char* gtr = gimg + tr_offset(lane, KP);
@@ -500,7 +509,8 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
     if (cnt > 0) {
         offsets(cnt);
         load_qg(at.t_begin, cnt);
-        load_kv(at.t_begin, cnt);
+        load_k(at.t_begin, cnt);
+        load_v(at.t_begin, cnt);
     }
     const float l2 = log2_decay(a.log_decay, at.head);
     const long long state0 = (at.seq * a.heads + at.head) * (long long)(D * D);
@@ -558,60 +568,76 @@ __global__ __launch_bounds__(DW * 64, D == 32 ? 2 : 1) void decay_grad_kernel(co
         wave_lds_order();
         load_qg(t0 + 32, next);
         __builtin_amdgcn_sched_barrier(0);
-        // [query x key]: q k and do v;  [column x key]: R k and R^T v
-        f32x16 p = zero16(), dp = zero16(), ov = zero16(), ok = zero16(), lv = zero16(), lk = zero16();
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const x8 qf = *reinterpret_cast<const x8*>(qimg + l31 * KP + 32 * ks + 16 * half);
-            const x8 gf = *reinterpret_cast<const x8*>(gimg + l31 * KP + 32 * ks + 16 * half);
-            p = mfma16(qf, k[ks], p);
-            dp = mfma16(gf, v[ks], dp);
+        // [query x key]: q k, do v;  [column x key]: R k, R^T v
+        auto products = [&](const char* img, const x8 (&x)[KS], const f32x16 (&r)[KT], int ks, f32x16& p, f32x16& o, f32x16& low) {
+            p = mfma16(*reinterpret_cast<const x8*>(img + l31 * KP + 32 * ks + 16 * half), x[ks], p);
             if constexpr (FINE) {
-                const FineOperand<T> r(R[ks >> 1]), rt(Rt[ks >> 1]);
-                ov = mfma16(r.h[ks & 1], k[ks], ov);
-                ok = mfma16(rt.h[ks & 1], v[ks], ok);
-                lv = mfma16(r.e[ks & 1], k[ks], lv);
-                lk = mfma16(rt.e[ks & 1], v[ks], lk);
+                const FineOperand<T> f(r[ks >> 1]);
+                o = mfma16(f.h[ks & 1], x[ks], o);
+                low = mfma16(f.e[ks & 1], x[ks], low);
             } else {
-                ov = mfma16(acc_operand<T>(R[ks >> 1], ks & 1), k[ks], ov);
-                ok = mfma16(acc_operand<T>(Rt[ks >> 1], ks & 1), v[ks], ok);
+                o = mfma16(acc_operand<T>(r[ks >> 1], ks & 1), x[ks], o);
             }
-        }
-        load_kv(t0 + 32, next);
-        __builtin_amdgcn_sched_barrier(0);
+        };
+        auto weights = [&](f32x16& p, f32x16& o, const f32x16& low) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float w = KEEP ? dw[r] : fades[-acc_row(r, 0)];
-            p[r] = weigh(p[r], w);
-            dp[r] = weigh(dp[r], w);
-            if (FINE) {
-                ov[r] += lv[r] * (1.f / Low<T>::SCALE);
-                ok[r] += lk[r] * (1.f / Low<T>::SCALE);
+            for (int r = 0; r < 16; ++r) {
+                p[r] = weigh(p[r], KEEP ? dw[r] : fades[-acc_row(r, 0)]);
+                if (FINE) o[r] += low[r] * (1.f / Low<T>::SCALE);
+                o[r] *= ow;
             }
-            ov[r] *= ow;
-            ok[r] *= ow;
-        }
-        const x8 g0 = tr_operand<T>(gtr + 64 * at.slice, 8 * KP), g1 = tr_operand<T>(gtr + 64 * at.slice + 16 * KP, 8 * KP);
-        const x8 q0 = tr_operand<T>(qtr + 64 * at.slice, 8 * KP), q1 = tr_operand<T>(qtr + 64 * at.slice + 16 * KP, 8 * KP);
-        if constexpr (FINE) {
-            ov = FineOperand<T>(p).times(g0, g1, ov);
-            ok = FineOperand<T>(dp).times(q0, q1, ok);
+        };
+        auto slice = [&](x8& x0, x8& x1, const char* tr) {
+            x0 = tr_operand<T>(tr + 64 * at.slice, 8 * KP);
+            x1 = tr_operand<T>(tr + 64 * at.slice + 16 * KP, 8 * KP);
+        };
+        f32x16 p = zero16(), dp = zero16(), ov = zero16(), ok = zero16(), lv = zero16(), lk = zero16();
+        x8 g0, g1, q0, q1, rok[2], rov[2];
+        if constexpr (HALVES) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) products(qimg, k, R, ks, p, ov, lv);
+            load_k(t0 + 32, next);
+            __builtin_amdgcn_sched_barrier(0);
+            weights(p, ov, lv);
+            slice(g0, g1, gtr);
+            ov = pairs_times(p, g0, g1, ov);
+            Split<T>(g0, g1, uw, half).update(R, whole, qtr, KP);
+            rov[0] = acc_operand<T>(ov, 0);
+            rov[1] = acc_operand<T>(ov, 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) products(gimg, v, Rt, ks, dp, ok, lk);
+            load_v(t0 + 32, next);
+            __builtin_amdgcn_sched_barrier(0);
+            weights(dp, ok, lk);
+            slice(q0, q1, qtr);
+            ok = pairs_times(dp, q0, q1, ok);
+            Split<T>(q0, q1, uw, half).update(Rt, whole, gtr, KP);
+            rok[0] = acc_operand<T>(ok, 0);
+            rok[1] = acc_operand<T>(ok, 1);
         } else {
-            ov = mfma16(g0, acc_operand<T>(p, 0), ov);
-            ok = mfma16(q0, acc_operand<T>(dp, 0), ok);
-            ov = mfma16(g1, acc_operand<T>(p, 1), ov);
-            ok = mfma16(q1, acc_operand<T>(dp, 1), ok);
-        }
-        const x8 rok[2] = {acc_operand<T>(ok, 0), acc_operand<T>(ok, 1)}, rov[2] = {acc_operand<T>(ov, 0), acc_operand<T>(ov, 1)};
-        if (!KEEP) __builtin_amdgcn_sched_barrier(0);
-        {
-            const Split<T> sg(g0, g1, uw, half);
-            sg.update(R, whole, qtr, KP);
-        }
-        if (!KEEP) __builtin_amdgcn_sched_barrier(0);
-        {
-            const Split<T> sq(q0, q1, uw, half);
-            sq.update(Rt, whole, gtr, KP);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                products(qimg, k, R, ks, p, ov, lv);
+                products(gimg, v, Rt, ks, dp, ok, lk);
+            }
+            load_k(t0 + 32, next);
+            load_v(t0 + 32, next);
+            __builtin_amdgcn_sched_barrier(0);
+            weights(p, ov, lv);
+            weights(dp, ok, lk);
+            slice(g0, g1, gtr);
+            slice(q0, q1, qtr);
+            ov = pairs_times(p, g0, g1, ov);
+            ok = pairs_times(dp, q0, q1, ok);
+            rok[0] = acc_operand<T>(ok, 0);
+            rok[1] = acc_operand<T>(ok, 1);
+            rov[0] = acc_operand<T>(ov, 0);
+            rov[1] = acc_operand<T>(ov, 1);
+            if (!KEEP) __builtin_amdgcn_sched_barrier(0);
+            Split<T>(g0, g1, uw, half).update(R, whole, qtr, KP);
+            if (!KEEP) __builtin_amdgcn_sched_barrier(0);
+            Split<T>(q0, q1, uw, half).update(Rt, whole, gtr, KP);
         }
         // the images are done with: results through them to 16-byte stores, four lanes on a row's 64 bytes
         wave_lds_order();
