@@ -9,10 +9,11 @@
 //     dv : backward in time over (k, q, do) with R = dS / m, where R collects lambda^(i+1) q_i do_i^T
 //     dk : backward in time over (v, do, q), with R^T (one walk with dv);   the gradient of the first state is m R there
 //
-// What bounds it: memory, and the instructions of a tile where long sequences leave a wave alone on its SIMD.  A tile of one head takes 2 d (d + 32) products per token and tensor element moved - an order
-// under what the matrix cores do in the time the rows take - so the kernels are built to keep loads in flight: a wave
-// works alone on (sequence, head, segment, 32 columns of v), no barriers, its next tile's rows on their way while the
-// current tile is multiplied.  Layouts (v_mfma_f32_32x32x16: lane = row of A / column of B, 8 contraction values):
+// What bounds it: memory, and the instructions of a tile where long sequences leave a wave alone on its SIMD.  A tile of one
+// head takes 2 d (d + 32) products per token and tensor element moved - an order under what the matrix cores do in the time
+// the rows take - so the kernels are built to keep loads in flight: a wave works alone on (sequence, head, segment, 32
+// columns of v), no barriers, its next tile's rows on their way while the current tile is multiplied.  Layouts
+// (v_mfma_f32_32x32x16: lane = row of A / column of B, 8 contraction values):
 //   * S^T[key x query] = K Q^T takes both rows as they lie; times the decays (a select: what a later token holds never
 //     reaches an earlier one's pairs) it is the B operand of O^T = V^T P^T without leaving the registers;
 //   * products that contract over tokens (V^T, K^T) read their transposed operand with ds_read_b64_tr_b16 from the tile's
