@@ -544,3 +544,28 @@ def test_python_entry_points_refuse_on_the_gpu():
     for call, what in bad:
         with pytest.raises(VdmiError, match=what):
             call()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("n,state", [(20, False), (20, True), (33, False), (300, True), (2500, False)])
+def test_results_are_rounded_once(n, state, d, dtype):
+    """What is stored is as near to the definition as its rounding allows, at any length: pairs and states enter their
+    products as two 16-bit operands (2^-17 of them lost in bfloat16, 2^-22 in half), under a hundredth of the result's own
+    rounding in the 2-norm; 1.05 leaves room for the float32 sums."""
+    from video_diffusion_amd import block_hip as B
+    q, k, v, do, decay, st, ds, _ = inputs(1, 1, n, 3, d, dtype, n + d, state=state)
+    flat = lambda t: None if t is None else t[0]
+    (o, last, *want), _ = reference(flat(q), flat(k), flat(v), decay, flat(st), None, d ** -0.5, flat(do), flat(ds))
+    ins = [t.detach().requires_grad_() for t in (q, k, v)]
+    if state:
+        got, gl = B.decay_attention(*ins, decay, initial_state=st, return_state=True)
+        grads = torch.autograd.grad((got, gl), ins, (do, ds))
+    else:
+        got = B.decay_attention(*ins, decay)
+        grads = torch.autograd.grad(got, ins, do)
+    for name, x, w in zip(("o", "dq", "dk", "dv"), (got.detach(), *grads), (o, *want)):
+        once = rel_err(w.to(dtype), w)
+        err = record(f"decay.once.n{n}.d{d}.{dtype}.{state}.{name}", rel_err(flat(x), w), 1.05 * once)
+        assert err < 1.05 * once, (name, err, once)

@@ -25,8 +25,8 @@
 // Few sequences: the time axis is cut into segments.  A first launch computes every segment's own contribution to the state
 // (reading k and v only), a second one runs along the segments, a third computes all outputs.
 // Measured, 2 x 8192 tokens, 8 heads of 64 features, bfloat16 (16.8 MB a tensor): segments' sums 11.6 us (2.9 TB/s), along
-// the segments 6, outputs 18.6 (3.6 TB/s); backward dq 18.6, dk and dv 25 (4.7 TB/s) beside another walk for the segments.
-// 16384 tokens, 8 heads of 128, half: 26 + 8.4 + 42 us.  There a wave has its SIMD to itself and bounds it by issuing: 61 % of
+// the segments 6, outputs 20 (3.4 TB/s); backward dq 20, dk and dv 31 (3.8 TB/s) beside another walk for the segments.
+// 16384 tokens, 8 heads of 128, half: 25 + 8.6 + 58 us.  There a wave has its SIMD to itself and bounds it by issuing: 61 % of
 // its cycles in the scan and 71 % in the gradients, 20 % waiting (2 x 8192 x 8 x 64).  Two
 // waves per SIMD hide that but take twice the segments, whose states cost as much.
 #include "block_common.h"
@@ -173,10 +173,10 @@ struct Split {
     }
 };
 
-// What lies in accumulator registers (weighted pairs, a state), contracted over them, as a sum of two 16-bit operands.  One
-// operand alone is rounded once more than a sum in float32 would be: sqrt(2) of its error over many terms, more in a result
-// of few.  So the sequences of one tile take two (as exact as float32 sums; 16 frames of 16384 sites in training 317 -> 330
-// us), longer ones do not (16384 tokens of 8 x 128 forward: 77 -> 85 us with the pairs alone in two).
+// What lies in accumulator registers (weighted pairs, a state), contracted over them, as a sum of two 16-bit operands: 2^-17
+// of a bfloat16 one is lost, 2^-22 of a half.  One operand alone would be rounded as coarsely as the result is: sqrt(2) of
+// its error in all (2.35e-3 in place of 1.66e-3 in bfloat16).  Kernel time with one and with two operands, forward and
+// backward: 2 x 8192 x 8 x 64 99 and 107 us, 16384 x 8 x 128 in half 238 and 300, 32 x 500 x 8 x 64 88 and 105.
 template <typename T>
 struct FineOperand {
     x8_t<T> h[2], e[2];
@@ -263,13 +263,13 @@ __device__ __forceinline__ int tr_offset(int lane, int pitch) {
     return (4 * (g16 >> 1) + tq) * pitch + (16 * (g16 & 1) + 4 * (((tp & 1) << 1) | (tp >> 1))) * 2;
 }
 
-// WHAT: the outputs; only the segments' states; the outputs of sequences of one tile (FineOperand)
-enum { OUTPUTS, STATES, ONE_TILE };
+// WHAT: the outputs; only the segments' states
+enum { OUTPUTS, STATES };
 
 template <typename T, int D, int WHAT>
-__global__ __launch_bounds__(DW * 64, D == 128 && (Low<T>::THREE || WHAT == ONE_TILE) && WHAT != STATES ? 1 : 2)
+__global__ __launch_bounds__(DW * 64, D == 128 && WHAT != STATES ? 1 : 2)
 void decay_scan_kernel(const ScanArgs a) {
-    constexpr bool STATE_ONLY = WHAT == STATES, FINE = WHAT == ONE_TILE;
+    constexpr bool STATE_ONLY = WHAT == STATES;
     typedef x8_t<T> x8;
     constexpr int KS = D / 16, KT = D / 32, KP = 2 * D + 16, RS = 512 / D;      // RS: rows that 64 16-byte pieces cover
     __shared__ __attribute__((aligned(16))) char kimg_all[DW][32 * KP];
@@ -388,28 +388,18 @@ void decay_scan_kernel(const ScanArgs a) {
             for (int ks = 0; ks < KS; ++ks) {
                 const x8 kf = *reinterpret_cast<const x8*>(kimg + l31 * KP + 32 * ks + 16 * half);
                 st = mfma16(kf, q[ks], st);
-                if constexpr (FINE) {
-                    const FineOperand<T> state(S[ks >> 1]);
-                    o = mfma16(state.h[ks & 1], q[ks], o);
-                    low = mfma16(state.e[ks & 1], q[ks], low);
-                } else {
-                    o = mfma16(acc_operand<T>(S[ks >> 1], ks & 1), q[ks], o);
-                }
+                const FineOperand<T> state(S[ks >> 1]);
+                o = mfma16(state.h[ks & 1], q[ks], o);
+                low = mfma16(state.e[ks & 1], q[ks], low);
             }
             load_q(t0 + 32, next);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 st[r] = weigh(st[r], dw[r]);
-                if (FINE) o[r] += low[r] * (1.f / Low<T>::SCALE);
-                o[r] *= ow;
+                o[r] = (o[r] + low[r] * (1.f / Low<T>::SCALE)) * ow;
             }
-            if constexpr (FINE) {
-                o = FineOperand<T>(st).times(v0, v1, o);
-            } else {
-                o = mfma16(v0, acc_operand<T>(st, 0), o);
-                o = mfma16(v1, acc_operand<T>(st, 1), o);
-            }
+            o = FineOperand<T>(st).times(v0, v1, o);
             // through LDS (the tile's v image is in registers by now) to 16-byte stores, four lanes on a row's 64 bytes
             wave_lds_order();
             *reinterpret_cast<x8*>(vimg + l31 * VP + 16 * half) = acc_operand<T>(o, 0);
@@ -443,14 +433,14 @@ void decay_scan_kernel(const ScanArgs a) {
 // this takes 25 (2 x 8192 tokens, 8 heads of 64).  With 64 features dv's half of a tile comes before dk's: that leaves 250
 // registers, none to move to and from the second file (both halves together 30.5 us; 32 x 500 x 8 x 64 39 and 32).  With 32 and
 // 128 features both halves at once are faster (16384 x 8 x 128, half: backward 137 and 144 us).
-template <typename T, int D, bool FINE>
+template <typename T, int D>
 __global__ __launch_bounds__(DW * 64, D <= 64 ? 2 : 1) void decay_grad_kernel(const GradArgs a) {
     typedef x8_t<T> x8;
     constexpr int KS = D / 16, KT = D / 32, KP = 2 * D + 16, RS = 512 / D;
     __shared__ __attribute__((aligned(16))) char qimg_all[DW][32 * KP];
     __shared__ __attribute__((aligned(16))) char gimg_all[DW][32 * KP];
     __shared__ __attribute__((aligned(16))) float uw_all[DW][32];
-    __shared__ float fade_all[D == 128 && (Low<T>::THREE || FINE) ? DW : 1][64];
+    __shared__ float fade_all[D == 128 || (D == 64 && !Low<T>::THREE) ? DW : 1][64];
     const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     char* qimg = qimg_all[wave];
@@ -465,10 +455,10 @@ __global__ __launch_bounds__(DW * 64, D <= 64 ? 2 : 1) void decay_grad_kernel(co
     at.clear<T>(a.dv, a.dvs, lane);
 
     x8 qreg[KS], greg[KS], k[KS], v[KS];
-    // 128 features of bfloat16 leave no registers for the loads' offsets and the pairs' decays: the former are computed
+    // 128 features leave no registers for the loads' offsets and the pairs' decays: the former are computed
     // again for every tile, the latter read from LDS.  (From scratch memory, where the compiler would put them, each one
     // waits for every load in flight: 16384 tokens, 8 heads took 205 us in place of 85.)
-    constexpr bool KEEP = D < 128 || !(Low<T>::THREE || FINE), HALVES = D == 64;
+    constexpr bool KEEP = D == 32 || (D == 64 && Low<T>::THREE), HALVES = D == 64;
     unsigned qofs[KEEP ? KS : 1], gofs[KEEP ? KS : 1], kofs, vofs;
     auto row_at = [&](const Rows& r, int i, int cnt) { return r.at(lane / (D / 8) + RS * i, cnt, true, 16 * (lane % (D / 8))); };
     auto offsets = [&](int cnt) {
@@ -497,11 +487,6 @@ __global__ __launch_bounds__(DW * 64, D <= 64 ? 2 : 1) void decay_grad_kernel(co
         const auto r = vr.tile(at.len - t0 - cnt, cnt > 0);
 #pragma unroll
         for (int i = 0; i < KS; ++i) v[i] = load16<T>(r, vofs + 32 * i);
-    };
-    auto pairs_times = [&](const f32x16& p, const x8& x0, const x8& x1, f32x16 o) {
-        if constexpr (FINE) return FineOperand<T>(p).times(x0, x1, o);
-        o = mfma16(x0, acc_operand<T>(p, 0), o);
-        return mfma16(x1, acc_operand<T>(p, 1), o);
     };
     const char* qtr = qimg + tr_offset(lane, KP);
     const char* gtr = gimg + tr_offset(lane, KP);
@@ -572,20 +557,15 @@ __global__ __launch_bounds__(DW * 64, D <= 64 ? 2 : 1) void decay_grad_kernel(co
         // [query x key]: q k, do v;  [column x key]: R k, R^T v
         auto products = [&](const char* img, const x8 (&x)[KS], const f32x16 (&r)[KT], int ks, f32x16& p, f32x16& o, f32x16& low) {
             p = mfma16(*reinterpret_cast<const x8*>(img + l31 * KP + 32 * ks + 16 * half), x[ks], p);
-            if constexpr (FINE) {
-                const FineOperand<T> f(r[ks >> 1]);
-                o = mfma16(f.h[ks & 1], x[ks], o);
-                low = mfma16(f.e[ks & 1], x[ks], low);
-            } else {
-                o = mfma16(acc_operand<T>(r[ks >> 1], ks & 1), x[ks], o);
-            }
+            const FineOperand<T> f(r[ks >> 1]);
+            o = mfma16(f.h[ks & 1], x[ks], o);
+            low = mfma16(f.e[ks & 1], x[ks], low);
         };
         auto weights = [&](f32x16& p, f32x16& o, const f32x16& low) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 p[r] = weigh(p[r], KEEP ? dw[r] : fades[-acc_row(r, 0)]);
-                if (FINE) o[r] += low[r] * (1.f / Low<T>::SCALE);
-                o[r] *= ow;
+                o[r] = (o[r] + low[r] * (1.f / Low<T>::SCALE)) * ow;
             }
         };
         auto slice = [&](x8& x0, x8& x1, const char* tr) {
@@ -601,7 +581,7 @@ __global__ __launch_bounds__(DW * 64, D <= 64 ? 2 : 1) void decay_grad_kernel(co
             __builtin_amdgcn_sched_barrier(0);
             weights(p, ov, lv);
             slice(g0, g1, gtr);
-            ov = pairs_times(p, g0, g1, ov);
+            ov = FineOperand<T>(p).times(g0, g1, ov);
             Split<T>(g0, g1, uw, half).update(R, whole, qtr, KP);
             rov[0] = acc_operand<T>(ov, 0);
             rov[1] = acc_operand<T>(ov, 1);
@@ -612,7 +592,7 @@ __global__ __launch_bounds__(DW * 64, D <= 64 ? 2 : 1) void decay_grad_kernel(co
             __builtin_amdgcn_sched_barrier(0);
             weights(dp, ok, lk);
             slice(q0, q1, qtr);
-            ok = pairs_times(dp, q0, q1, ok);
+            ok = FineOperand<T>(dp).times(q0, q1, ok);
             Split<T>(q0, q1, uw, half).update(Rt, whole, gtr, KP);
             rok[0] = acc_operand<T>(ok, 0);
             rok[1] = acc_operand<T>(ok, 1);
@@ -629,8 +609,8 @@ __global__ __launch_bounds__(DW * 64, D <= 64 ? 2 : 1) void decay_grad_kernel(co
             weights(dp, ok, lk);
             slice(g0, g1, gtr);
             slice(q0, q1, qtr);
-            ov = pairs_times(p, g0, g1, ov);
-            ok = pairs_times(dp, q0, q1, ok);
+            ov = FineOperand<T>(p).times(g0, g1, ov);
+            ok = FineOperand<T>(dp).times(q0, q1, ok);
             rok[0] = acc_operand<T>(ok, 0);
             rok[1] = acc_operand<T>(ok, 1);
             rov[0] = acc_operand<T>(ov, 0);
@@ -1036,10 +1016,6 @@ int launch_scan(const ScanArgs& s, const vdmi_decay_args* a, const Plan& p, hipS
     return VDMI_OK;
 }
 
-int outputs(const ScanArgs& s, const vdmi_decay_args* a, const Plan& p, hipStream_t st) {
-    return a->n <= 32 ? launch_scan<ONE_TILE>(s, a, p, st) : launch_scan<OUTPUTS>(s, a, p, st);
-}
-
 // sums of the segments and the states at their starts (nothing to do for one segment)
 int segment_states(ScanArgs s, const vdmi_decay_args* a, const Plan& p, hipStream_t st) {
     if (p.nseg == 1) return VDMI_OK;
@@ -1125,8 +1101,7 @@ int launch_grad(const vdmi_decay_args* a, const Plan& p, hipStream_t st) {
     if (tasks > 0x7fffffffLL) return VDMI_E_SHAPE;
     g.tasks = (unsigned)tasks;
     const dim3 grid((unsigned)wgs), block(DW * 64);
-#define GRAD(T, D) do { if (a->n <= 32) hipLaunchKernelGGL((decay_grad_kernel<T, D, true>), grid, block, 0, st, g); \
-                        else hipLaunchKernelGGL((decay_grad_kernel<T, D, false>), grid, block, 0, st, g); } while (0)
+#define GRAD(T, D) hipLaunchKernelGGL((decay_grad_kernel<T, D>), grid, block, 0, st, g)
 #define GRAD_D(T) do { if (a->d == 32) GRAD(T, 32); else if (a->d == 64) GRAD(T, 64); else GRAD(T, 128); } while (0)
     if (a->dtype == VDMI_DT_BF16) GRAD_D(__bf16); else GRAD_D(_Float16);
 #undef GRAD
@@ -1159,7 +1134,7 @@ extern "C" int vdmi_decay_attn_fwd(const vdmi_decay_args* a, vdmi_stream stream)
     s.s_out = a->state_out;
     s.e_out = 1;
     const int r = segment_states(s, a, p, st);
-    return r != VDMI_OK ? r : outputs(s, a, p, st);
+    return r != VDMI_OK ? r : launch_scan<OUTPUTS>(s, a, p, st);
 }
 
 extern "C" int vdmi_decay_attn_bwd(const vdmi_decay_args* a, vdmi_stream stream) {
@@ -1181,7 +1156,7 @@ extern "C" int vdmi_decay_attn_bwd(const vdmi_decay_args* a, vdmi_stream stream)
     s.e_out = 1;
     s.rs = 1;
     role(s, a->dout, a->v, a->k, a->dq);
-    int r = outputs(s, a, p, st);
+    int r = launch_scan<OUTPUTS>(s, a, p, st);
     if (r != VDMI_OK) return r;
     // dv and dk: backward in time; R = dS / m collects lambda^(i+1) q_i do_i^T
     if (p.nseg > 1) {
