@@ -569,3 +569,31 @@ def test_results_are_rounded_once(n, state, d, dtype):
         once = rel_err(w.to(dtype), w)
         err = record(f"decay.once.n{n}.d{d}.{dtype}.{state}.{name}", rel_err(flat(x), w), 1.05 * once)
         assert err < 1.05 * once, (name, err, once)
+
+
+@gpu
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("n", [6, 10, 17, 24, 31, 32])
+def test_a_neighbour_that_is_not_finite(n, ragged):
+    """Sequences of every length that leaves rows of a tile over: an infinity or NaN in the first token of one of them does
+    not reach the ones beside it, forward or backward."""
+    from video_diffusion_amd import block_hip as B
+    q, k, v, do, decay, *_ = inputs(2, 9, n, 2, 32, torch.bfloat16, n)
+    lengths = torch.full((2, 9), n, device=DEV, dtype=torch.int32) if ragged else None
+    clean = [t.clone() for t in (q, k, v, do)]
+
+    def run(q, k, v, do):
+        ins = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = B.decay_attention(*ins, decay, lengths=lengths)
+        return [o, *torch.autograd.grad(o, ins, do)]
+
+    want = run(*clean)
+    others = torch.ones(2, 9, dtype=torch.bool, device=DEV)
+    others[0, 3] = others[1, 8] = False
+    for which in range(4):
+        for value in (float("nan"), float("inf")):
+            bad = [t.clone() for t in clean]
+            bad[which][0, 3, 0] = value
+            bad[which][1, 8, 0, 1, 7] = value
+            for got, w in zip(run(*bad), want):
+                assert torch.equal(got[others], w[others])

@@ -690,7 +690,8 @@ __global__ __launch_bounds__(256) void decay_segments_kernel(const ScanArgs a, i
 // v and do (dP^T = V dO^T with lane = query for dq; P = Q K^T and dP = dO V^T with lane = key for dv and dk).  A wave
 // computes one (tile, head) and ends: enough of them share a SIMD to cover each other's loads.
 // A row that is not finite must not reach the other sequences of its tile (zero times infinity in the second product):
-// such a tile is computed once per sequence with the others' rows as zeros.
+// such a tile is computed once per sequence with the others' rows as zeros.  Rows that no sequence of the tile fills
+// (32 - n of them where n > 16) are zeros too.
 // ------------------------------------------------------------------------------------------------------------------
 struct Strides32 { unsigned b, i, n; };            // bytes
 
@@ -751,11 +752,11 @@ __global__ __launch_bounds__((short_waves(D, BWD) * 64), D == 128 ? 1 : 2) void 
         const unsigned row = RPI * i + lane / PR, slot = row * a.inv_n >> 16;
         tt[i] = row - slot * n;
         unsigned seq = tile * (unsigned)a.per_tile + slot;
-        mine[i] = slot < (unsigned)a.per_tile && seq < a.nseq;
+        mine[i] = slot < (unsigned)a.per_tile && seq < a.nseq;     // rows behind the tile's last sequence are nobody's
         seq = min(seq, a.nseq - 1);     // a row that is not there loads another one; nothing of it is stored
         bb[i] = a.shift < 0 ? seq : __umulhi(seq, a.magic) >> a.shift;
         ii[i] = seq - bb[i] * a.inner;
-        live[i] = !a.lengths || (int)tt[i] < a.lengths[seq];
+        live[i] = mine[i] && (!a.lengths || (int)tt[i] < a.lengths[seq]);
     }
     auto row_of = [&](const void* p, const Strides32& s, long long h, int i) {
         return const_cast<x8*>(reinterpret_cast<const x8*>(static_cast<const char*>(p) + 2 * head0 * h + (unsigned long long)bb[i] * s.b +
@@ -774,7 +775,7 @@ __global__ __launch_bounds__((short_waves(D, BWD) * 64), D == 128 ? 1 : 2) void 
             x[2][i] = *row_of(a.v, a.vs, a.vh, i);
             if constexpr (BWD) x[3][i] = *row_of(a.g, a.gs, a.gh, i);
         }
-        if (a.lengths || s_hi - s_lo < a.per_tile) {
+        if (a.lengths || s_hi - s_lo < a.per_tile || n * a.per_tile < 32) {
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 const int slot = (int)((RPI * i + lane / PR) * a.inv_n >> 16);
