@@ -597,3 +597,19 @@ def test_a_neighbour_that_is_not_finite(n, ragged):
             bad[which][1, 8, 0, 1, 7] = value
             for got, w in zip(run(*bad), want):
                 assert torch.equal(got[others], w[others])
+
+
+@gpu
+@pytest.mark.parametrize("n", [5, 12, 20, 32, 70])
+def test_padding_behind_a_token_that_is_not_finite(n):
+    """Outputs and gradients behind lengths are zeros whatever the tokens before them hold."""
+    from video_diffusion_amd import block_hip as B
+    q, k, v, do, decay, *_ = inputs(2, 3, n, 2, 32, torch.bfloat16, n)
+    lengths = torch.full((2, 3), n - 2, device=DEV, dtype=torch.int32)
+    for which in range(4):
+        bad = [t.clone() for t in (q, k, v, do)]
+        bad[which][:, :, 1] = float("nan")
+        ins = [t.detach().requires_grad_() for t in bad[:3]]
+        o = B.decay_attention(*ins, decay, lengths=lengths)
+        for x in (o.detach(), *torch.autograd.grad(o, ins, bad[3])):
+            assert torch.equal(x[:, :, n - 2:], torch.zeros_like(x[:, :, n - 2:]))

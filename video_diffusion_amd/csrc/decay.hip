@@ -798,7 +798,10 @@ __global__ __launch_bounds__((short_waves(D, BWD) * 64), D == 128 ? 1 : 2) void 
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int slot = (int)((RPI * i + lane / PR) * a.inv_n >> 16);
-            const x8 x = *reinterpret_cast<const x8*>(src + (RPI * i + lane / PR) * P + 16 * piece);
+            x8 x = *reinterpret_cast<const x8*>(src + (RPI * i + lane / PR) * P + 16 * piece);
+            // whatever the sequence's own tokens made of its padding.  (lengths are read again: live[] kept until here takes
+            // the registers of 3 % of the backward.)
+            if (a.lengths && (int)tt[i] >= a.lengths[min(tile * (unsigned)a.per_tile + slot, a.nseq - 1)]) x = zero8;
             if (mine[i] && slot >= s_lo && slot < s_hi) *row_of(dst, s, h, i) = x;
         }
     };
