@@ -613,3 +613,30 @@ def test_padding_behind_a_token_that_is_not_finite(n):
         o = B.decay_attention(*ins, decay, lengths=lengths)
         for x in (o.detach(), *torch.autograd.grad(o, ins, bad[3])):
             assert torch.equal(x[:, :, n - 2:], torch.zeros_like(x[:, :, n - 2:]))
+
+
+@gpu
+@pytest.mark.parametrize("qk,up", [(1e-2, 1e-4), (1.0, 1e-5), (1e-3, 1.0), (1e-4, 1e-6)])
+@pytest.mark.parametrize("n,d,state", [(9, 64, False), (24, 32, True), (33, 64, False), (300, 128, False), (3000, 64, True)])
+def test_small_halfs(n, d, state, qk, up):
+    """Halfs whose pairs, states or own values lie below the type's normal range count in full: every result is as near to
+    the definition as its rounding to half allows (1.05 of that, as for values near one)."""
+    from video_diffusion_amd import block_hip as B
+    q, k, v, do, decay, st, ds, _ = inputs(1, 1, n, 2, d, torch.float32, n + d, state=state)
+    q, k, v, do = (qk * q).half(), (qk * k).half(), v.half(), (up * do).half()
+    if state:
+        st, ds = qk * st, up * ds
+    flat = lambda t: None if t is None else t[0]
+    (o, last, dq, dk, dv, ds0), _ = reference(flat(q), flat(k), flat(v), decay, flat(st), None, d ** -0.5, flat(do), flat(ds))
+    ins = [t.detach().requires_grad_() for t in (q, k, v)]
+    if state:
+        got, gl = B.decay_attention(*ins, decay, initial_state=st, return_state=True)
+        grads = torch.autograd.grad((got, gl), ins, (do, ds))
+        assert rel_err(flat(gl), last) < 1e-5
+    else:
+        got = B.decay_attention(*ins, decay)
+        grads = torch.autograd.grad(got, ins, do)
+    for name, x, w in zip(("o", "dq", "dk", "dv"), (got.detach(), *grads), (o, dq, dk, dv)):
+        once = rel_err(w.half(), w)
+        err = record(f"decay.small.n{n}.d{d}.{qk}.{up}.{state}.{name}", rel_err(flat(x), w), 1.05 * once)
+        assert err < 1.05 * once, (name, err, once)

@@ -244,7 +244,8 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengt
     the next piece of the sequence.  Returns o like q (in q's order of dimensions in memory), or (o, state).
 
     Pairs scale * q_t k_j and states enter products as sums of two operands of q's dtype, so that results are rounded once,
-    when they are stored: in float16 they have to stay within 65504 (the state that is returned is float32 throughout).  A token that is not finite makes the
+    when they are stored: in float16 they have to stay within 65504, and 2^-36 of small ones is lost (the state that is
+    returned is float32 throughout).  A token that is not finite makes the
     outputs from it on not finite and may make up to 31 earlier ones of its own sequence so; other sequences and tokens
     behind lengths have no such effect."""
     dims = q.dim()

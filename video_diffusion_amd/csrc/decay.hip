@@ -81,14 +81,11 @@ extern "C" __device__ float vdmi_mul_legacy(float, float) __asm("llvm.amdgcn.fmu
 __device__ __forceinline__ float weigh(float p, float w) { return vdmi_mul_legacy(p, w); }
 
 // lambda^(..) v as a sum of 16-bit operands: three of bfloat16 (8 bits each), two halfs (11 bits each).
-// The matrix cores take subnormal half operands as zeros: the low halfs (2^-11 of the values at most) are multiplied up
-// by 2^11, and a value that is itself below the normal range goes into the low operand as a whole.  bfloat16 has float's range.
+// The low halfs (2^-11 of the values at most) are multiplied up by 2^11, so that what is lost of a value is 2^-22 of it or
+// 2^-36, where a sum of plain halfs ends at steps of 2^-24.  (The matrix cores take subnormal halfs as what they are: 2^-15,
+// 2^-20 and 2^-24 as either operand gave exact products.)  bfloat16 has float's range.
 template <typename T> struct Low { static constexpr float SCALE = 1.f; static constexpr bool THREE = true; };
 template <> struct Low<_Float16> { static constexpr float SCALE = 2048.f; static constexpr bool THREE = false; };
-template <typename T>
-__device__ __forceinline__ float above(float x) { return x; }
-template <>
-__device__ __forceinline__ float above<_Float16>(float x) { return fabsf(x) < 0x1p-14f ? 0.f : x; }
 
 // two values at a time: the conversions come in pairs
 template <typename T>
@@ -97,7 +94,7 @@ struct Two {
     typedef __attribute__((ext_vector_type(2))) float f2;
     // elements j, j + 1 of h = what T holds of a, b;  a, b become what is left, times SCALE
     static __device__ __forceinline__ void take(x8_t<T>& h, int j, float& a, float& b) {
-        const t2 w = __builtin_convertvector((f2{above<T>(a), above<T>(b)}), t2);
+        const t2 w = __builtin_convertvector((f2{a, b}), t2);
         const f2 back = __builtin_convertvector(w, f2);
         h[j] = w[0];
         h[j + 1] = w[1];
@@ -174,7 +171,7 @@ struct Split {
 };
 
 // What lies in accumulator registers (weighted pairs, a state), contracted over them, as a sum of two 16-bit operands: 2^-17
-// of a bfloat16 one is lost, 2^-22 of a half.  One operand alone would be rounded as coarsely as the result is: sqrt(2) of
+// of a bfloat16 one is lost, 2^-22 of a half (or 2^-36).  One operand alone would be rounded as coarsely as the result is: sqrt(2) of
 // its error in all (2.35e-3 in place of 1.66e-3 in bfloat16).  Kernel time with one and with two operands, forward and
 // backward: 2 x 8192 x 8 x 64 99 and 107 us, 16384 x 8 x 128 in half 238 and 300, 32 x 500 x 8 x 64 88 and 105.
 template <typename T>
