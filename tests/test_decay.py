@@ -640,3 +640,30 @@ def test_small_halfs(n, d, state, qk, up):
         once = rel_err(w.half(), w)
         err = record(f"decay.small.n{n}.d{d}.{qk}.{up}.{state}.{name}", rel_err(flat(x), w), 1.05 * once)
         assert err < 1.05 * once, (name, err, once)
+
+
+@gpu
+@pytest.mark.parametrize("n,state", [(9, False), (9, True), (70, False), (3000, True)])
+def test_a_decay_that_is_not_a_number(n, state):
+    """NaN in log_decay makes everything of its head NaN, and nothing of another head."""
+    from video_diffusion_amd import block_hip as B
+    q, k, v, do, decay, st, ds, _ = inputs(1, 1, n, 3, 32, torch.bfloat16, n, state=state)
+    bad = decay.clone()
+    bad[1] = float("nan")
+
+    def run(decay):
+        ins = [t.detach().requires_grad_() for t in (q, k, v)]
+        if not state:
+            o = B.decay_attention(*ins, decay)
+            return [o.detach(), *torch.autograd.grad(o, ins, do)], []
+        o, s = B.decay_attention(*ins, decay, initial_state=st, return_state=True)
+        step = s.detach()[:, 0].clone()
+        x = B.decay_attention_step(q[:, 0, 0], k[:, 0, 0], v[:, 0, 0], decay, step)
+        return [o.detach(), *torch.autograd.grad((o, s), ins, (do, ds))], [s.detach()[:, 0], step, x]
+
+    (rows, states), (rows0, states0) = run(bad), run(decay)
+    for x, w in zip(rows, rows0):
+        assert torch.isnan(x[..., 1, :]).all()
+        assert torch.equal(x[..., 0::2, :], w[..., 0::2, :])
+    for x, w in zip(states, states0):
+        assert torch.isnan(x[:, 1]).all() and torch.equal(x[:, 0::2], w[:, 0::2])

@@ -70,9 +70,10 @@ struct GradArgs {                       // dk and dv
 __device__ __forceinline__ int swap23(int l) { return (l & 0x13) | ((l & 4) << 1) | ((l & 8) >> 1); }
 __device__ __forceinline__ int acc_row(int reg, int half) { return (reg & 3) + 8 * (reg >> 2) + 4 * half; }
 
-// log2 lambda, bounded so that exponents of zero tokens stay zero (lambda^1 has underflowed long before -1e4)
+// log2 lambda, bounded so that exponents of zero tokens stay zero (lambda^1 has underflowed long before -1e4); NaN stays
 __device__ __forceinline__ float log2_decay(const float* log_decay, int head) {
-    return fmaxf(log_decay[head] * LOG2E, -1e4f);
+    const float l2 = log_decay[head] * LOG2E;
+    return l2 < -1e4f ? -1e4f : l2;
 }
 
 // p * w where w = 0 marks a pair that does not exist: zero whatever p is (0 * inf and 0 * NaN are 0).  v_mul_legacy_f32 as
