@@ -747,7 +747,7 @@ int vdmi_block_norm_bwd(const vdmi_block_norm_args* a, vdmi_stream stream);
  * multiple of 8, as codes uint8 [rows][c] (e4m3: 4 exponent, 3 fraction bits, largest 448, no infinities) and exps uint8
  * [rows][ceil(c / 32)] (e + 127): x ~ code 2^e, e per row and 32 consecutive channels the least exponent whose 448 2^e holds
  * the group's largest finite magnitude, in -118 .. 119 (magnitudes beyond 448 2^119 become that); rounded to nearest even;
- * infinities and NaN become NaN.
+ * infinities and NaN become NaN.  Unpacked to halfs, magnitudes beyond 65504 (the code next to the largest halfs) become that.
  * vdmi_rows8_wgrad: weight gradient of a Linear whose input was kept, dw float [cout][cin] = sum_r dy[r][o] x[r][i], from
  * the codes and bf16 rows dy [rows][cout] (pitch lddy, at most VDMI_ROWS8_MAX_PITCH), and db float [cout] = sum_r dy[r][o]
  * (NULL: not wanted); cin, cout multiples of 8; workspace as stated by vdmi_rows8_wgrad_workspace_bytes().

@@ -270,3 +270,20 @@ def test_python_entry_points_refuse():
                      "multiples of 32")]:
         with pytest.raises(VdmiError, match=what):
             f()
+
+
+@gpu
+def test_the_largest_halfs():
+    """Rows of finite halfs come back finite: what their codes stand for, at most 65504; infinities and NaN as NaN."""
+    from video_diffusion_amd import block_hip as B
+    x = torch.tensor([[65504.0, 63488.0, 63456.0, 61440.0, 3.0, 0.0, -1e-7, 448.0], [-65504.0, -63488.0, -63456.0, 57344.0, 2.0, 1.0, 0.5, 0.25],
+                      [float("inf"), 65504.0, float("nan"), -65504.0, 1.0, 2.0, 3.0, 4.0]], device=DEV).half()
+    kept = B.pack_rows8(x)
+    values = kept_values(x)[0]
+    assert float(values.abs().nan_to_num().max()) == 65536.0                # the code next to the largest half
+    assert torch.equal(torch.nan_to_num(kept.unpack(torch.float32).cpu().double(), nan=7e7), torch.nan_to_num(values, nan=7e7))
+    got, want = kept.unpack().cpu().double(), values.clamp(-65504, 65504)
+    assert torch.equal(torch.isnan(got), ~torch.isfinite(x.cpu()))
+    assert torch.equal(torch.nan_to_num(got, nan=0.0), torch.nan_to_num(want, nan=0.0))
+    fin = torch.isfinite(x.cpu())
+    assert ((got - x.cpu().double()).abs()[fin] <= (x.cpu().double().abs() * 2.0 ** -4).clamp(min=2.0 ** -2)[fin]).all()

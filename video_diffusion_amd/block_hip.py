@@ -473,7 +473,8 @@ class Rows8:
         self.codes, self.exps, self.shape, self.dtype = codes, exps, shape, dtype
 
     def unpack(self, dtype=None) -> torch.Tensor:
-        """The values the codes stand for, in the packed tensor's shape."""
+        """The values the codes stand for, in the packed tensor's shape; in float16 at most 65504, also where rows of another
+        type held more."""
         dtype = self.dtype if dtype is None else dtype
         if dtype not in _DTYPES:
             raise VdmiError(f"rows are bfloat16, float16 or float32 (got {dtype})")

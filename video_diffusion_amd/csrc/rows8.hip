@@ -3,7 +3,7 @@
 //   pack    e = the least exponent with max |x| <= 448 2^e over the group's finite values, in -118 .. 119 (so that every
 //           code times 2^e is a bfloat16);  code = e4m3(x 2^-e), round to nearest even: off by 2^-4 of the value at most
 //           (2^-10 2^e below 2^-6 2^e).  Infinities and NaN become NaN; magnitudes beyond 448 2^119 (2.9e38) become that.
-//   unpack  code 2^e
+//   unpack  code 2^e, to halfs at most 65504
 //   weight gradient of a Linear from the kept input: dw[o][i] = sum_r dy[r][o] code[r][i] 2^e, on the matrix cores, codes
 //           widened to bfloat16 (exactly) on their way into LDS - half the bytes of bfloat16 rows.
 #include "block_common.h"
@@ -108,6 +108,11 @@ __global__ __launch_bounds__(256) void rows8_unpack_kernel(const UnpackArgs a) {
     const uint2 w = *reinterpret_cast<const uint2*>(a.codes + idx * 8);
     float v[8];
     widen8(v, w, a.exps[row * a.groups + (p >> 2)]);
+    if constexpr (__is_same(T, _Float16)) {
+        // halfs from 63488 on have the code of 65536, which is not a half: what is finite stays finite
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fabsf(v[e]) > 65504.f ? copysignf(65504.f, v[e]) : v[e];
+    }
     T* dst = static_cast<T*>(a.x) + row * a.ldx + 8 * p;
     if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<f32x4*>(dst) = f32x4{v[0], v[1], v[2], v[3]};
