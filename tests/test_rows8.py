@@ -287,3 +287,20 @@ def test_the_largest_halfs():
     assert torch.equal(torch.nan_to_num(got, nan=0.0), torch.nan_to_num(want, nan=0.0))
     fin = torch.isfinite(x.cpu())
     assert ((got - x.cpu().double()).abs()[fin] <= (x.cpu().double().abs() * 2.0 ** -4).clamp(min=2.0 ** -2)[fin]).all()
+
+
+@gpu
+def test_what_is_lost_of_the_smallest_values():
+    """The documented bound: 2^-4 of a value, or under 2^-17 of its group's largest (2^-128 where that is below 224 2^-118)."""
+    from video_diffusion_amd import block_hip as B
+    x = torch.zeros(64, 32, dtype=torch.float64)
+    for r in range(64):
+        x[r, 0] = 224.0 * (1 + 2.0 ** -7) * 2.0 ** (r - 40)             # just above the border to the next exponent
+        x[r, 1:] = x[r, 0] * 2.0 ** -17.8 * torch.linspace(0.2, 1.2, 31, dtype=torch.float64)
+    x[:8] *= 2.0 ** -100
+    x = x.float()
+    got, want = B.pack_rows8(x.to(DEV)).unpack().cpu().double(), x.double()
+    top = want.abs().amax(1, keepdim=True)
+    off = (got - want).abs()
+    assert (off <= torch.maximum(want.abs() * 2.0 ** -4, torch.maximum(top * 2.0 ** -17, torch.tensor(2.0 ** -128)))).all()
+    assert (off > torch.maximum(want.abs() * 2.0 ** -4, top * 2.0 ** -18)).any()            # 2^-18 would not hold

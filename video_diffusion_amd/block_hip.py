@@ -528,8 +528,9 @@ def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
 
 def pack_rows8(x: torch.Tensor) -> Rows8:
     """x [..., c] (bfloat16, float16 or float32, c a multiple of 8) in 8 bits: e4m3 codes times the least power of two per
-    row and 32 channels that holds the largest magnitude.  Off by 2^-4 of a value at most (2^-18 of its group's largest for
-    the smallest ones); infinities and NaN come back as NaN, magnitudes beyond 448 * 2^119 as that."""
+    row and 32 channels that holds the largest magnitude.  Off by 2^-4 of a value at most or, for the smallest ones, under
+    2^-17 of their group's largest (2^-128 where that is below 224 * 2^-118); infinities and NaN come back as NaN, magnitudes
+    beyond 448 * 2^119 as that."""
     _on_gpu(x)
     if x.dtype not in _DTYPES:
         raise VdmiError(f"rows are bfloat16, float16 or float32 (got {x.dtype})")
