@@ -304,3 +304,20 @@ def test_what_is_lost_of_the_smallest_values():
     off = (got - want).abs()
     assert (off <= torch.maximum(want.abs() * 2.0 ** -4, torch.maximum(top * 2.0 ** -17, torch.tensor(2.0 ** -128)))).all()
     assert (off > torch.maximum(want.abs() * 2.0 ** -4, top * 2.0 ** -18)).any()            # 2^-18 would not hold
+
+
+@gpu
+@pytest.mark.parametrize("n", [64, 96])
+def test_a_weight_and_its_transpose_within_fixed_weights(n):
+    """One square parameter as w and as w.t(): the same memory and shape, two weight sets."""
+    from video_diffusion_amd import block_hip as B, train_hip as T
+    g = torch.Generator(device=DEV).manual_seed(n)
+    w = (torch.randn(n, n, generator=g, device=DEV) * n ** -0.5).requires_grad_()
+    x = torch.randn(50, n, generator=g, device=DEV).to(torch.bfloat16).requires_grad_()
+    dy = torch.randn(50, n, generator=g, device=DEV).to(torch.bfloat16)
+    want = [(y, *torch.autograd.grad(y, (x, w), dy)) for y in (B.linear_rows8(x, w), B.linear_rows8(x, w.t()))]
+    with T.fixed_weights(T.PackStore()):
+        got = [(y, *torch.autograd.grad(y, (x, w), dy)) for y in (B.linear_rows8(x, w), B.linear_rows8(x, w.t()))]
+    for a, b in zip(want, got):
+        assert all(torch.equal(s, t) for s, t in zip(a, b))
+    assert rel_err(got[1][0].detach(), x.detach().double() @ w.detach().double()) < 2 * 2.0 ** -8

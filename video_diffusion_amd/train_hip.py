@@ -151,8 +151,8 @@ class PhasePacks:
 
 class PackStore:
     """Packed weight sets that outlive a forward / backward, for a caller that knows when the weights change (the Trainer
-    around its optimizer step, a sampler whose weights are frozen).  A set is found again by the weight's memory and
-    shape and trusted while the version counters of the weight (and of its scale) stand where they stood when it was
+    around its optimizer step, a sampler whose weights are frozen).  A set is found again by the weight's memory,
+    shape and strides and trusted while the version counters of the weight (and of its scale) stand where they stood when it was
     packed.  In-place updates under no_grad (load_state_dict, the single-tensor and foreach optimizers) move them; a
     FUSED optimizer step (torch._fused_adam_) and writes through `.data` do not - whoever runs those calls invalidate()
     afterwards, as the Trainer does after every optimizer step.  refresh() repacks every set that went stale in ONE
@@ -205,13 +205,13 @@ class PackStore:
         return e.pack
 
     def get(self, weight: torch.Tensor, transposed: bool, tile_bn=None, in_scale=None, gather=None, shape=None) -> DevPack:
-        key = (weight.data_ptr(), tuple(weight.shape), bool(transposed), tile_bn,
+        key = (weight.data_ptr(), tuple(weight.shape), weight.stride(), bool(transposed), tile_bn,
                None if in_scale is None else in_scale.data_ptr(), None if gather is None else gather.data_ptr())
         return self._entry(key, weight, in_scale,
                            lambda: DevPack(weight, transposed, tile_bn, fill=False, gather=gather, shape=shape))
 
     def get_phases(self, weight: torch.Tensor, gathers, shape, tile_bn) -> PhasePacks:
-        key = (weight.data_ptr(), tuple(weight.shape), "phases", tile_bn, None, gathers[0].data_ptr())
+        key = (weight.data_ptr(), tuple(weight.shape), weight.stride(), "phases", tile_bn, None, gathers[0].data_ptr())
         return self._entry(key, weight, None, lambda: PhasePacks(weight, gathers, shape, tile_bn))
 
     def refresh(self):
