@@ -321,3 +321,28 @@ def test_a_weight_and_its_transpose_within_fixed_weights(n):
     for a, b in zip(want, got):
         assert all(torch.equal(s, t) for s, t in zip(a, b))
     assert rel_err(got[1][0].detach(), x.detach().double() @ w.detach().double()) < 2 * 2.0 ** -8
+
+
+@gpu
+@pytest.mark.parametrize("start", [1, 3, 8])
+def test_linear_of_rows_at_any_address(start):
+    """Input, weight, bias and gradient that begin `start` elements into their memory."""
+    from video_diffusion_amd import block_hip as B
+
+    def at(t):
+        m = torch.zeros(t.numel() + start, device=DEV, dtype=t.dtype)
+        m[start:] = t.reshape(-1)
+        return m[start:].view(t.shape)
+
+    g = torch.Generator(device=DEV).manual_seed(start)
+    x = torch.randn(5, 11, 64, generator=g, device=DEV).to(torch.bfloat16)
+    w, b = torch.randn(96, 64, generator=g, device=DEV) / 8, torch.randn(96, generator=g, device=DEV)
+    dy = torch.randn(5, 11, 96, generator=g, device=DEV).to(torch.bfloat16)
+
+    def run(*ts):
+        ins = [t.detach().requires_grad_() for t in ts[:3]]
+        y = B.linear_rows8(*ins)
+        return (y.detach(), *torch.autograd.grad(y, ins, ts[3]))
+
+    for a, e in zip(run(at(x), at(w), at(b), at(dy)), run(x, w, b, dy)):
+        assert torch.equal(a, e)

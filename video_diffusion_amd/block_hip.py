@@ -573,11 +573,17 @@ class LinearRows8Fn(torch.autograd.Function):
         return _linear_backward(dy, weight, kept, ctx.shape, ctx.needs_input_grad)
 
 
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy of it, contiguous and 16-byte aligned: what the row GEMMs read."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
+
+
 @_there
 def _linear(x, weight, bias, keep):
     from .train_hip import _linear_pack, conv_rows
-    xr = x.reshape(-1, x.shape[-1]).contiguous()
-    y = conv_rows(xr, _linear_pack(weight.detach(), False), None if bias is None else bias.detach().float().contiguous(),
+    xr = _dense(x.reshape(-1, x.shape[-1]))
+    y = conv_rows(xr, _linear_pack(weight.detach(), False), None if bias is None else _dense(bias.detach().float()),
                   1, 1, 1, xr.shape[0])
     return y.view(*x.shape[:-1], weight.shape[0]), pack_rows8(xr) if keep else None
 
@@ -586,7 +592,7 @@ def _linear(x, weight, bias, keep):
 def _linear_backward(dy, weight, kept, shape, need):
     from .train_hip import _linear_pack, conv_rows
     dx = dw = db = None
-    d = dy.to(torch.bfloat16).reshape(-1, dy.shape[-1]).contiguous()
+    d = _dense(dy.to(torch.bfloat16).reshape(-1, dy.shape[-1]))
     if need[0]:
         dx = conv_rows(d, _linear_pack(weight.detach(), True), None, 1, 1, 1, d.shape[0]).view(shape)
     if need[1]:
