@@ -346,3 +346,21 @@ def test_linear_of_rows_at_any_address(start):
 
     for a, e in zip(run(at(x), at(w), at(b), at(dy)), run(x, w, b, dy)):
         assert torch.equal(a, e)
+
+
+@gpu
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_nothing_is_packed_where_no_backward_can_follow(mode, monkeypatch):
+    """Parameters ask for gradients while a model samples, too."""
+    from video_diffusion_amd import block_hip as B
+    x = torch.randn(40, 64, device=DEV).to(torch.bfloat16)
+    w, b = (torch.randn(96, 64, device=DEV) / 8).requires_grad_(), torch.randn(96, device=DEV).requires_grad_()
+    packs = []
+    real = B.pack_rows8
+    monkeypatch.setattr(B, "pack_rows8", lambda t: packs.append(t.shape) or real(t))
+    want = B.linear_rows8(x, w, b)
+    assert len(packs) == 1 and want.requires_grad
+    with mode():
+        got = B.linear_rows8(x, w, b)
+    assert len(packs) == 1 and not got.requires_grad and torch.equal(got, want)
+    assert B.linear_rows8(x.requires_grad_(), w.detach()).requires_grad and len(packs) == 1

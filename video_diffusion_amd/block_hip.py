@@ -558,7 +558,6 @@ class LinearRows8Fn(torch.autograd.Function):
     """y = x weight^T + bias on the row GEMMs of train_hip.py; what is kept of x for the weight gradient is 8 bits wide."""
 
     @staticmethod
-    @_plain
     def forward(ctx, x, weight, bias):
         y, kept = _linear(x, weight, bias, ctx.needs_input_grad[1])
         ctx.save_for_backward(weight, *((kept.codes, kept.exps) if kept else ()))
@@ -579,6 +578,7 @@ def _dense(t: torch.Tensor) -> torch.Tensor:
     return t.clone() if t.data_ptr() & 15 else t
 
 
+@_plain
 @_there
 def _linear(x, weight, bias, keep):
     from .train_hip import _linear_pack, conv_rows
@@ -619,4 +619,6 @@ def linear_rows8(x: torch.Tensor, weight: torch.Tensor, bias=None) -> torch.Tens
         raise VdmiError(f"multiples of 32 channels (got {tuple(weight.shape)})")
     if x.numel() == 0:
         return torch.nn.functional.linear(x, weight.to(x.dtype), None if bias is None else bias.to(x.dtype))
+    if not _wants_grad(x, weight, bias):        # nothing to keep: needs_input_grad does not know of no_grad
+        return _linear(x, weight, bias, False)[0]
     return LinearRows8Fn.apply(x, weight, bias)
