@@ -274,3 +274,21 @@ def test_trainer_keeps_rows_in_8_bits(tmp_path, monkeypatch):
     (a, none), (b, some) = run(False), run(True)
     assert none == 0 and some > 0 and some % 8 == 0          # four row sets a block, the same blocks in both steps
     assert a[0] == b[0] and all(x == x and abs(x) < 1e30 for x in b)
+
+
+@gpu
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_a_block_packs_nothing_where_no_backward_can_follow(mode, monkeypatch):
+    """Sampling inside a rows8_checkpoints block, with parameters that ask for gradients."""
+    from video_diffusion_amd import block_hip, train_hip as T
+    rb = _block(64, 128)
+    x, temb = torch.randn(1, 64, 2, 8, 8, device=DEV).to(torch.bfloat16), torch.randn(1, 32, device=DEV)
+    packs = []
+    real = block_hip.pack_rows8
+    monkeypatch.setattr(block_hip, "pack_rows8", lambda t: packs.append(t.shape) or real(t))
+    with T.rows8_checkpoints():
+        want = T.resnet_block(rb, x, temb)
+        assert len(packs) == 4
+        with mode():
+            got = T.resnet_block(rb, x, temb)
+        assert len(packs) == 4 and torch.equal(got, want)

@@ -488,8 +488,9 @@ class ResnetBlockFn(torch.autograd.Function):
 
     @staticmethod
     @_plain
-    def forward(ctx, x, scale, shift, w1, b1, g1, w2, b2, g2, wres, bres, with_res=True):
+    def forward(ctx, x, scale, shift, w1, b1, g1, w2, b2, g2, wres, bres, with_res=True, rows8=False):
         # with_res = False: block2(block1(x)) alone, for callers that put a layer between the blocks and the residual
+        # rows8: keep the activations in 8 bits; the caller's choice, since no_grad does not show in needs_input_grad
         if not x.is_cuda:
             raise _lib.VdmiError("the hip-resnet training backend needs CUDA (HIP) tensors; there is no CPU path")
         b, cin, f, h, w = x.shape
@@ -514,7 +515,7 @@ class ResnetBlockFn(torch.autograd.Function):
         else:
             h2 = rmsnorm_silu_rows(y2, g2v, None, 0, f * hw)
             out = conv_rows(xr, param_pack(wres, False), bres.detach().float().contiguous(), frames, f, h, w, residual=h2)
-        ctx.rows8 = _ROWS8 and any(ctx.needs_input_grad)
+        ctx.rows8 = rows8 and any(ctx.needs_input_grad)
         rows = (xr, y1, h1, y2)
         if ctx.rows8:
             from .block_hip import pack_rows8
@@ -564,7 +565,7 @@ class ResnetBlockFn(torch.autograd.Function):
             dx_res = conv_rows(do, param_pack(wres, True), None, frames, f, h, w)
         dx = conv_rows(dy1, param_pack(w1, True), None, frames, f, h, w, residual=dx_res)
         return (from_rows(dx, b, f, h, w, ctx.act), dscale, dshift, dw1, db1, dg1.view(cout, 1, 1, 1), dw2, db2,
-                dg2.view(cout, 1, 1, 1), dwres, dbres, None)
+                dg2.view(cout, 1, 1, 1), dwres, dbres, None, None)
 
 
 class InitConvFn(torch.autograd.Function):
@@ -751,12 +752,13 @@ def resnet_block(rb, x: torch.Tensor, temb) -> torch.Tensor:
     args = (x, scale, shift, rb.block1.proj.weight, rb.block1.proj.bias, rb.block1.norm.gamma,
             rb.block2.proj.weight, rb.block2.proj.bias, rb.block2.norm.gamma)
     tconv = getattr(rb, "temporal_conv", None)
+    rows8 = _ROWS8 and torch.is_grad_enabled()
     if tconv is not None:
-        h = ResnetBlockFn.apply(*args, None, None, False)
+        h = ResnetBlockFn.apply(*args, None, None, False, rows8)
         if tconv.kernel_size[1:] == (1, 1) and tconv.kernel_size[0] % 2 == 1 and tconv.padding == (tconv.kernel_size[0] // 2, 0, 0):
             return TemporalConvResFn.apply(h, x, tconv.weight, tconv.bias, wres, bres)
         return torch_ops(lambda y, xin: tconv(y) + rc(xin), h, x)
-    return ResnetBlockFn.apply(*args, wres, bres)
+    return ResnetBlockFn.apply(*args, wres, bres, True, rows8)
 
 
 def supports(unet) -> bool:
