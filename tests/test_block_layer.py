@@ -292,3 +292,48 @@ def test_a_block_packs_nothing_where_no_backward_can_follow(mode, monkeypatch):
         with mode():
             got = T.resnet_block(rb, x, temb)
         assert len(packs) == 4 and torch.equal(got, want)
+
+
+def test_rows8_checkpoints_belong_to_their_thread():
+    """The switch holds for the forward of the thread that set it."""
+    import threading
+    from video_diffusion_amd import train_hip as T
+    seen, inside, done = [], threading.Event(), threading.Event()
+
+    def other():
+        inside.wait(10)
+        seen.append(T._ROWS8)
+        with T.rows8_checkpoints(False):
+            seen.append(T._ROWS8)
+        with T.rows8_checkpoints():
+            seen.append(T._ROWS8)
+            done.set()
+
+    t = threading.Thread(target=other)
+    t.start()
+    with T.rows8_checkpoints():
+        inside.set()
+        done.wait(10)
+        assert T._ROWS8 is True
+    t.join(10)
+    assert T._ROWS8 is False and seen == [False, False, True]
+
+
+@gpu
+def test_rows8_checkpoints_and_recomputation():
+    """torch.utils.checkpoint around a block: its context_fn sets the switch for the recomputation too, which runs during the
+    backward, outside the `with` of the forward; gradients are those without recomputation."""
+    from torch.utils.checkpoint import checkpoint
+    from video_diffusion_amd import train_hip as T
+    rb = _block(64, 64)
+    x = torch.randn(1, 64, 2, 16, 16, device=DEV).to(torch.bfloat16).requires_grad_()
+    temb = torch.randn(1, 32, device=DEV)
+    leaves = [x, *rb.parameters()]
+    with T.rows8_checkpoints():
+        want = T.resnet_block(rb, x, temb)
+    dout = torch.randn_like(want)
+    grads = torch.autograd.grad(want, leaves, dout)
+    got = checkpoint(lambda x: T.resnet_block(rb, x, temb), x, use_reentrant=False,
+                     context_fn=lambda: (T.rows8_checkpoints(), T.rows8_checkpoints()))
+    assert torch.equal(got, want)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, leaves, dout), grads))

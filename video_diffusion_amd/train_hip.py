@@ -18,6 +18,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import os
+import threading
 
 import torch
 import torch.nn.functional as F
@@ -458,7 +459,20 @@ def colsum_rows(x: torch.Tensor) -> torch.Tensor:
     return out
 
 
-_ROWS8 = False          # inside a rows8_checkpoints block
+class _Rows8Switch(threading.local):
+    """The rows8_checkpoints blocks that this thread is in, innermost last."""
+
+    def __init__(self):
+        self.blocks = [False]
+
+
+_rows8 = _Rows8Switch()
+
+
+def __getattr__(name):
+    if name == "_ROWS8":        # whether this thread is inside a rows8_checkpoints block
+        return _rows8.blocks[-1]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 class rows8_checkpoints:
@@ -466,19 +480,21 @@ class rows8_checkpoints:
     activations (its input, its hidden rows, both convolutions' outputs) as 8-bit codes with a power of two per 32 channels
     (block_hip.pack_rows8) instead of bf16 rows: about half the memory, for gradients that see those rows rounded to 3
     fraction bits.  Outputs are unchanged.  The backward widens a block's rows again when it gets there (the res_conv's
-    weight gradient reads the codes themselves)."""
+    weight gradient reads the codes themselves).
+
+    The block holds for the thread that entered it.  What torch.utils.checkpoint computes again it computes during the
+    backward, outside of it: there the block goes in as context_fn=lambda: (rows8_checkpoints(), rows8_checkpoints()), or
+    torch finds other tensors saved than in the forward and raises."""
 
     def __init__(self, on: bool = True):
         self.on = bool(on)
 
     def __enter__(self):
-        global _ROWS8
-        self.prev, _ROWS8 = _ROWS8, self.on
+        _rows8.blocks.append(self.on)
         return self
 
     def __exit__(self, *exc):
-        global _ROWS8
-        _ROWS8 = self.prev
+        _rows8.blocks.pop()
         return False
 
 
@@ -752,7 +768,7 @@ def resnet_block(rb, x: torch.Tensor, temb) -> torch.Tensor:
     args = (x, scale, shift, rb.block1.proj.weight, rb.block1.proj.bias, rb.block1.norm.gamma,
             rb.block2.proj.weight, rb.block2.proj.bias, rb.block2.norm.gamma)
     tconv = getattr(rb, "temporal_conv", None)
-    rows8 = _ROWS8 and torch.is_grad_enabled()
+    rows8 = _rows8.blocks[-1] and torch.is_grad_enabled()
     if tconv is not None:
         h = ResnetBlockFn.apply(*args, None, None, False, rows8)
         if tconv.kernel_size[1:] == (1, 1) and tconv.kernel_size[0] % 2 == 1 and tconv.padding == (tconv.kernel_size[0] // 2, 0, 0):
