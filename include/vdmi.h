@@ -661,7 +661,8 @@ void vdmi_sla_rows_mfma_enable(int on);
  * first and after the last token, either may be NULL (zeros / not wanted) and state_in may be state_out; state_in is
  * 16-byte aligned.
  * Backward: from q, k, v, dout and dstate_in (gradient of the last state; NULL = zeros) the gradients dq, dk, dv and
- * dstate_out (of the first state; NULL = not wanted; state_in as in the forward, state_out unused).  log_decay and scale
+ * dstate_out (of the first state; NULL = not wanted; state_in as in the forward, state_out unused).  dq.p NULL, or dk.p and
+ * dv.p NULL (then dstate_out too): not wanted.  log_decay and scale
  * are constants.  With halfs, m q_t k_j and the states' elements have to stay within 65504 (they are operands of products,
  * each as two halfs: 2^-36 of small ones is lost; the state handed on is float throughout).  A token that is not finite makes the outputs from it on not finite and may
  * make earlier ones of its own sequence so; other sequences are unaffected.

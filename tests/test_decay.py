@@ -667,3 +667,38 @@ def test_a_decay_that_is_not_a_number(n, state):
         assert torch.equal(x[..., 0::2, :], w[..., 0::2, :])
     for x, w in zip(states, states0):
         assert torch.isnan(x[:, 1]).all() and torch.equal(x[:, 0::2], w[:, 0::2])
+
+
+@gpu
+@pytest.mark.parametrize("wanted,n,state", [(w, n, n > 9) for n in (9, 45, 3000) for w in ("q", "k", "v", "s", "qs", "kv", "qk")
+                                            if n > 9 or "s" not in w])
+def test_only_the_gradients_that_are_asked_for(wanted, n, state, monkeypatch):
+    """They are those of a call that asks for all, and nothing else is computed."""
+    from video_diffusion_amd import block_hip as B
+    q, k, v, do, decay, st, ds, _ = inputs(1, 2, n, 2, 64, torch.bfloat16, n, state=state)
+    asked = []
+    real = _lib.lib().vdmi_decay_attn_bwd
+    monkeypatch.setattr(_lib.lib(), "vdmi_decay_attn_bwd",
+                        lambda a, s: asked.append((bool(a.dq.p), bool(a.dk.p), bool(a.dv.p), bool(a.dstate_out))) or real(a, s))
+
+    def run(names):
+        t = {"q": q, "k": k, "v": v, "s": st}
+        t = {i: x if x is None else x.detach().requires_grad_(i in names) for i, x in t.items()}
+        o, s = B.decay_attention(t["q"], t["k"], t["v"], decay, initial_state=t["s"], return_state=True)
+        return dict(zip(names, torch.autograd.grad((o, s), [t[i] for i in names], (do, torch.zeros_like(s) if ds is None else ds))))
+
+    full, got = run("qkvs" if state else "qkv"), run(wanted)
+    for i in wanted:
+        assert torch.equal(got[i], full[i])
+    both = wanted != "q"                     # one walk computes dk, dv and the state's gradient
+    assert asked[1] == ("q" in wanted, both, both, "s" in wanted)
+
+
+def test_gradients_that_nobody_wants():
+    """The library takes a null dq, or null dk and dv without the state's gradient; not one of dk and dv alone, nor none."""
+    lib = _lib.lib()
+    bwd = lambda **kw: lib.vdmi_decay_attn_bwd(C.byref(_args(**kw)), None)
+    none = dict(dk_p=None, dv_p=None)
+    assert bwd(dv_p=None) == -1 and bwd(dq_p=None, **none) == -1 and bwd(dstate_out=256, **none) == -1
+    # the rest is still checked, up to here without a launch
+    assert bwd(dq_p=None, dk_b=4) == -3 and bwd(dq_p=8, **none) == -3 and bwd(dq_p=None, v_p=None) == -1

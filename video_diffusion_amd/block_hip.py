@@ -119,7 +119,9 @@ def _empty_like_rows(t: torch.Tensor) -> torch.Tensor:
 _NO_ROWS = _lib.Rows4()
 
 
-def _rows4(t: torch.Tensor) -> "_lib.Rows4":
+def _rows4(t) -> "_lib.Rows4":
+    if t is None:
+        return _NO_ROWS
     s = t.stride()
     return _lib.Rows4(t.data_ptr(), s[0], s[1], s[2], s[3])
 
@@ -147,12 +149,14 @@ def _decay_forward(q, k, v, state, log_decay, lengths, scale, return_state):
 
 
 @_there
-def _decay_backward(q, k, v, state, log_decay, lengths, fwd_ws, scale, do, dlast, want_dstate):
+def _decay_backward(q, k, v, state, log_decay, lengths, fwd_ws, scale, do, dlast, need):
+    """The gradients that need (of q, k, v, the state) asks for; dk and dv come together."""
     do = torch.zeros_like(q) if do is None else _row_operand(do if do.dtype == q.dtype else do.to(q.dtype))
     if dlast is not None:
         dlast = dlast.to(torch.float32).contiguous()
-    dq, dk, dv = _empty_like_rows(q), _empty_like_rows(k), _empty_like_rows(v)
-    dstate = torch.empty_like(state) if want_dstate else None
+    dq = _empty_like_rows(q) if need[0] else None
+    dk, dv = (_empty_like_rows(k), _empty_like_rows(v)) if any(need[1:4]) else (None, None)
+    dstate = torch.empty_like(state) if need[3] else None
     b, inner, n, h, d = q.shape
     a = _lib.DecayArgs(_DTYPES[q.dtype], b, inner, n, h, d, scale, 0, _rows4(q), _rows4(k), _rows4(v), _NO_ROWS,
                        _rows4(do), _rows4(dq), _rows4(dk), _rows4(dv), log_decay.data_ptr(), _ptr(lengths), _ptr(state), None,
@@ -196,7 +200,7 @@ class DecayAttnFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         if not (ctx.sites or do is None):
             do = do.unsqueeze(1)
-        grads = _decay_backward(*ctx.saved_tensors, ctx.scale, do, dlast, need[3])
+        grads = _decay_backward(*ctx.saved_tensors, ctx.scale, do, dlast, need)
         if not ctx.sites:
             grads = [None if g is None else g.squeeze(1) for g in grads]
         dq, dk, dv, dstate = grads

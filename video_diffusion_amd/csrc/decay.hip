@@ -695,7 +695,7 @@ struct Strides32 { unsigned b, i, n; };            // bytes
 
 struct ShortArgs {
     const void* q; const void* k; const void* v; const void* g;        // g: gradient of o
-    void* o; void* dq; void* dk; void* dv;
+    void* o; void* dq; void* dk; void* dv;                             // dq null or dk and dv null: not wanted
     Strides32 qs, ks, vs, gs, os, dqs, dks, dvs;
     long long qh, kh, vh, gh, oh, dqh, dkh, dvh;                        // head strides, elements
     const float* log_decay;
@@ -853,18 +853,22 @@ __global__ __launch_bounds__((short_waves(D, BWD) * 64), D == 128 ? 1 : 2) void 
                 const f32x16 p = pairs(im[2] + c, im[3] + c, false);                    // [key x query]: v do
                 const f32x16 pv = pairs(im[0] + c, im[1] + c, true);                    // [query x key]: q k
                 const f32x16 pk = pairs(im[3] + c, im[2] + c, true);                    // do v
-                product(im[1] + c, p, im[2] + c);                                       // dq, where v was
-                product(im[3] + c, pv, im[3] + c);                                      // dv, where do was
-                product(im[0] + c, pk, im[0] + c);                                      // dk, where q was
+                if (a.dq) product(im[1] + c, p, im[2] + c);                             // dq, where v was
+                if (a.dk) {
+                    product(im[3] + c, pv, im[3] + c);                                  // dv, where do was
+                    product(im[0] + c, pk, im[0] + c);                                  // dk, where q was
+                }
             }
         }
         wave_lds_order();
         if constexpr (!BWD) {
             store(im[0], a.o, a.os, a.oh, s_lo, s_hi);
         } else {
-            store(im[2], a.dq, a.dqs, a.dqh, s_lo, s_hi);
-            store(im[3], a.dv, a.dvs, a.dvh, s_lo, s_hi);
-            store(im[0], a.dk, a.dks, a.dkh, s_lo, s_hi);
+            if (a.dq) store(im[2], a.dq, a.dqs, a.dqh, s_lo, s_hi);
+            if (a.dk) {
+                store(im[3], a.dv, a.dvs, a.dvh, s_lo, s_hi);
+                store(im[0], a.dk, a.dks, a.dkh, s_lo, s_hi);
+            }
         }
     };
     const bool fine = load(0, a.per_tile);
@@ -1142,8 +1146,10 @@ extern "C" int vdmi_decay_attn_fwd(const vdmi_decay_args* a, vdmi_stream stream)
 extern "C" int vdmi_decay_attn_bwd(const vdmi_decay_args* a, vdmi_stream stream) {
     const int ok = check_args(a);
     if (ok != VDMI_OK) return ok;
-    if (!a->dout.p || !a->dq.p || !a->dk.p || !a->dv.p) return VDMI_E_ARG;
-    if (!rows_ok(a->dout) || !rows_ok(a->dq) || !rows_ok(a->dk) || !rows_ok(a->dv)) return VDMI_E_ALIGN;
+    // dk and dv come from one walk, which also ends in the gradient of the first state
+    const bool want_q = a->dq.p, want_kv = a->dk.p;
+    if (!a->dout.p || !(want_q || want_kv) || !a->dk.p != !a->dv.p || (a->dstate_out && !want_kv)) return VDMI_E_ARG;
+    if (!rows_ok(a->dout) || (want_q && !rows_ok(a->dq)) || (want_kv && (!rows_ok(a->dk) || !rows_ok(a->dv)))) return VDMI_E_ALIGN;
     if (!pitch_ok(a->dout) || !pitch_ok(a->dq) || !pitch_ok(a->dk) || !pitch_ok(a->dv)) return VDMI_E_SHAPE;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const Plan p = plan(a, wants_states(a));
@@ -1151,18 +1157,20 @@ extern "C" int vdmi_decay_attn_bwd(const vdmi_decay_args* a, vdmi_stream stream)
     if (p.bytes && (!a->workspace || a->workspace_bytes < (int64_t)p.bytes || !a->fwd_workspace)) return VDMI_E_ARG;
     // S^T is read 16 bytes at a time
     if (!aligned16(a->state_in) || (p.bytes && (!aligned16(a->workspace) || !aligned16(a->fwd_workspace)))) return VDMI_E_ALIGN;
-    // dq: forward in time over (do, v, k) with S^T; the states at the segments' starts are the forward's
-    ScanArgs s = scan_args(a, p);
-    s.seg = const_cast<float*>(static_cast<const float*>(a->fwd_workspace));
-    s.s_in = a->state_in;
-    s.e_out = 1;
-    s.rs = 1;
-    role(s, a->dout, a->v, a->k, a->dq);
-    int r = launch_scan<OUTPUTS>(s, a, p, st);
-    if (r != VDMI_OK) return r;
+    if (want_q) {
+        // dq: forward in time over (do, v, k) with S^T; the states at the segments' starts are the forward's
+        ScanArgs s = scan_args(a, p);
+        s.seg = const_cast<float*>(static_cast<const float*>(a->fwd_workspace));
+        s.s_in = a->state_in;
+        s.e_out = 1;
+        s.rs = 1;
+        role(s, a->dout, a->v, a->k, a->dq);
+        const int r = launch_scan<OUTPUTS>(s, a, p, st);
+        if (r != VDMI_OK || !want_kv) return r;
+    }
     // dv and dk: backward in time; R = dS / m collects lambda^(i+1) q_i do_i^T
     if (p.nseg > 1) {
-        s = scan_args(a, p);
+        ScanArgs s = scan_args(a, p);
         s.reverse = 1;
         s.e_u = 1;
         s.s_in = a->dstate_in;
@@ -1170,7 +1178,8 @@ extern "C" int vdmi_decay_attn_bwd(const vdmi_decay_args* a, vdmi_stream stream)
         s.s_out = a->dstate_out;
         s.s_out_mul = a->scale;
         role(s, a->k, a->q, a->dout, a->dv);
-        if ((r = segment_states(s, a, p, st)) != VDMI_OK) return r;
+        const int r = segment_states(s, a, p, st);
+        if (r != VDMI_OK) return r;
     }
     return launch_grad(a, p, st);
 }
