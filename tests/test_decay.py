@@ -702,3 +702,15 @@ def test_gradients_that_nobody_wants():
     assert bwd(dv_p=None) == -1 and bwd(dq_p=None, **none) == -1 and bwd(dstate_out=256, **none) == -1
     # the rest is still checked, up to here without a launch
     assert bwd(dq_p=None, dk_b=4) == -3 and bwd(dq_p=8, **none) == -3 and bwd(dq_p=None, v_p=None) == -1
+
+
+def test_results_of_a_broadcast_operand_stay_within_the_kernels_pitch():
+    """A result lies in memory in its operand's order, but never with tokens further apart than the kernels take: sites that
+    share one row do not become the fastest dimension of 2^26 elements."""
+    from video_diffusion_amd import block_hip as B
+    for shape, strides in (((2, 1 << 19, 4, 2, 64), (1024, 0, 128, 64, 1)), ((2, 1 << 19, 4, 2, 64), (0, 0, 0, 0, 1)),
+                           ((1, 1 << 19, 4, 2, 64), (0, 64, 1 << 25, 1 << 27, 1))):
+        q = torch.empty(0, device="meta", dtype=torch.bfloat16).new_empty_strided(shape, strides)
+        t = B._empty_like_rows(q)
+        assert t.shape == q.shape and t.stride(2) <= _lib.DECAY_MAX_PITCH and t.stride(4) == 1
+        assert t.untyped_storage().nbytes() == 2 * q.numel()

@@ -103,17 +103,21 @@ def _row_operand(t: torch.Tensor) -> torch.Tensor:
 
 def _empty_like_rows(t: torch.Tensor) -> torch.Tensor:
     """An uninitialised dense tensor of t's shape whose dimensions lie in memory in t's order: the sites of a frame stay
-    next to each other where t is a permuted view of (batch, frame, site) rows.  Broadcast dimensions of t become real."""
+    next to each other where t is a permuted view of (batch, frame, site) rows.  Broadcast dimensions of t become real; where
+    that would part the tokens further than the kernels go, they lie next to each other instead."""
     (b, i, n, h, d), (sb, si, sn, sh, _) = t.shape, t.stride()
     if sb >= si >= sn >= sh:
         return torch.empty((b, i, n, h, d), device=t.device, dtype=t.dtype)
     if sb >= sn >= si >= sh:                    # (batch, frame, site) rows
-        return t.new_empty_strided((b, i, n, h, d), (n * i * h * d, h * d, i * h * d, d, 1))
-    strides, pitch = [0, 0, 0, 0, 1], d
-    for k in sorted(range(4), key=lambda k: (t.stride(k), -k)):
-        strides[k] = pitch
-        pitch *= t.shape[k]
-    return t.new_empty_strided(t.shape, strides)
+        strides = [n * i * h * d, h * d, i * h * d, d, 1]
+    else:
+        strides, pitch = [0, 0, 0, 0, 1], d
+        for k in sorted(range(4), key=lambda k: (t.stride(k), -k)):
+            strides[k] = pitch
+            pitch *= t.shape[k]
+    if strides[2] > _lib.DECAY_MAX_PITCH:
+        return torch.empty((b, i, n, h, d), device=t.device, dtype=t.dtype)
+    return t.new_empty_strided((b, i, n, h, d), strides)
 
 
 _NO_ROWS = _lib.Rows4()
