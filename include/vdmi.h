@@ -650,7 +650,8 @@ void vdmi_sla_rows_mfma_enable(int on);
 
 /* ------------------------------------------------------------------------------------------
  * Attention over time with a decay per head (no counterpart in the reference, whose temporal attention is a softmax over
- * all frames and keeps no state): per head, with lambda = exp(log_decay[head]), log_decay <= 0, and m = scale,
+ * all frames and keeps no state): per head, with lambda = exp(log_decay[head]), log_decay <= 0, and m = scale
+ * (2^-126 to 2^126 in magnitude),
  *     S_t = lambda S_(t-1) + k_t v_t^T   (d x d, float),      o_t = m q_t S_t.
  * Rows of heads by strides (in elements, multiples of 8, pointers 16-byte aligned, the d features of a head contiguous):
  * element (b, i, t, h) of a vdmi_rows4 starts at p + b*.b + i*.i + t*.n + h*.h, for b < b, i < inner, t < n, h < heads

@@ -714,3 +714,16 @@ def test_results_of_a_broadcast_operand_stay_within_the_kernels_pitch():
         t = B._empty_like_rows(q)
         assert t.shape == q.shape and t.stride(2) <= _lib.DECAY_MAX_PITCH and t.stride(4) == 1
         assert t.untyped_storage().nbytes() == 2 * q.numel()
+
+
+def test_scales_without_a_reciprocal_are_refused():
+    """The backward divides by the scale: one whose reciprocal is not a finite float32 is refused on the host."""
+    lib = _lib.lib()
+    for s in (1e-39, -1e-39, 1e-45, 3e38, -3e38):
+        assert lib.vdmi_decay_attn_fwd(C.byref(_args(scale=s)), None) == -1
+        assert lib.vdmi_decay_attn_bwd(C.byref(_args(scale=s)), None) == -1
+    from video_diffusion_amd import block_hip as B
+    for s in (1e-39, -1e-39, 1e-46, 3e38, float("inf"), float("nan"), 0.0):
+        with pytest.raises(_lib.VdmiError, match="scale"):
+            B._scale(s, 32)
+    assert B._scale(2.0 ** -126, 32) == 2.0 ** -126 and B._scale(-(2.0 ** 126), 32) == -(2.0 ** 126)

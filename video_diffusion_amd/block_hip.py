@@ -235,8 +235,8 @@ def _scale(scale, d):
     if scale is None:
         return d ** -0.5
     scale = float(scale)
-    if scale == 0 or not abs(scale) < 3e38:
-        raise VdmiError(f"scale is finite and not zero (got {scale})")
+    if not 2.0 ** -126 <= abs(scale) <= 2.0 ** 126:
+        raise VdmiError(f"scale is from 2^-126 to 2^126 in magnitude (got {scale})")
     return scale
 
 
@@ -246,7 +246,8 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengt
 
     q, k, v: bfloat16 or float16 [b, n, heads, d] or, for the sequences of many sites, [b, sites, n, heads, d]; any strides
     (views of qkv rows are read in place where their rows are 16-byte aligned).  d is 32, 64 or 128.  log_decay: float32
-    [heads], at most 0, a constant (a NaN makes its head NaN).  scale: d^-0.5 by default.  initial_state: float32 [b(, sites), heads, d, d], S before
+    [heads], at most 0, a constant (a NaN makes its head NaN).  scale: d^-0.5 by default, 2^-126 to 2^126 in
+    magnitude.  initial_state: float32 [b(, sites), heads, d, d], S before
     the first token (zeros by default).  lengths: int32 [b(, sites)] - tokens from there on are padding: they are not read,
     their outputs and gradients are zeros.  return_state: also return S after the last token, for decay_attention_step or
     the next piece of the sequence.  Returns o like q (in q's order of dimensions in memory), or (o, state).

@@ -957,10 +957,13 @@ bool pitch_ok(const vdmi_rows4& r) { return r.n >= 0 && r.n <= VDMI_DECAY_MAX_PI
 // the short-sequence kernel multiplies batch indexes with 32-bit byte strides
 bool strides32_ok(const vdmi_rows4& r) { return r.b >= 0 && r.i >= 0 && r.b < 0x7fffffffLL && r.i < 0x7fffffffLL; }
 
+// the backward divides by it: it and its reciprocal are normal numbers (zero, infinities and NaN are not)
+bool scale_ok(float m) { return fabsf(m) >= 0x1p-126f && fabsf(m) <= 0x1p126f; }
+
 int check_args(const vdmi_decay_args* a) {
     if (!a || !a->log_decay) return VDMI_E_ARG;
     if (a->dtype != VDMI_DT_BF16 && a->dtype != VDMI_DT_F16) return VDMI_E_ARG;
-    if (!(a->scale != 0.f) || !(a->scale - a->scale == 0.f)) return VDMI_E_ARG;       // zero, infinite, NaN
+    if (!scale_ok(a->scale)) return VDMI_E_ARG;
     if (a->b <= 0 || a->inner <= 0 || a->n <= 0 || a->heads <= 0 || a->heads > 65535) return VDMI_E_SHAPE;
     if (a->d != 32 && a->d != 64 && a->d != 128) return VDMI_E_SHAPE;
     if ((long long)a->b * a->inner > 0x7fffffffLL / a->heads || a->n > (1 << 30)) return VDMI_E_SHAPE;
@@ -1189,7 +1192,7 @@ extern "C" int vdmi_decay_attn_step(const void* q, const void* k, const void* v,
                                     vdmi_stream stream) {
     if (!q || !k || !v || !o || !strides || !log_decay || !state) return VDMI_E_ARG;
     if (dtype != VDMI_DT_BF16 && dtype != VDMI_DT_F16) return VDMI_E_ARG;
-    if (!(scale != 0.f) || !(scale - scale == 0.f)) return VDMI_E_ARG;
+    if (!scale_ok(scale)) return VDMI_E_ARG;
     if (seqs <= 0 || heads <= 0 || (d != 32 && d != 64 && d != 128) || seqs > 0x7fffffffLL / heads) return VDMI_E_SHAPE;
     if (!aligned16(state)) return VDMI_E_ALIGN;
     StepArgs s = {q, k, v, o, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7],
