@@ -753,6 +753,7 @@ int vdmi_block_norm_bwd(const vdmi_block_norm_args* a, vdmi_stream stream);
  * vdmi_rows8_wgrad: weight gradient of a Linear whose input was kept, dw float [cout][cin] = sum_r dy[r][o] x[r][i], from
  * the codes and bf16 rows dy [rows][cout] (pitch lddy, at most VDMI_ROWS8_MAX_PITCH), and db float [cout] = sum_r dy[r][o]
  * (NULL: not wanted); cin, cout multiples of 8; workspace as stated by vdmi_rows8_wgrad_workspace_bytes().
+ * Under 2^30 groups of 32 channels a call, and cin * cout up to 2^30.
  * ------------------------------------------------------------------------------------------ */
 #define VDMI_ROWS8_MAX_PITCH (1LL << 23)
 int vdmi_rows8_pack(const void* x, int64_t ldx, void* codes, void* exps, int dtype, int64_t rows, int c, vdmi_stream stream);

@@ -368,3 +368,30 @@ def test_no_cpu_path():
     from video_diffusion_amd._lib import VdmiError
     with pytest.raises(VdmiError, match="no CPU path"):
         B.norm_before(torch.zeros(2, 8))
+
+
+@gpu
+def test_more_samples_than_one_launch_takes():
+    """A launch has less than 2^32 threads: 2^24 workgroups of 256 and 2^22 of 1024 are more.  Samples at the borders of
+    launches against the same samples by themselves; the weight's gradient, which 64 threads add up one sample after the
+    other, is off by 2^-24 sqrt(n / 128) of it: 2.2e-5."""
+    from video_diffusion_amd import block_hip as B
+    n, c = (1 << 24) + 5, 8
+    g = torch.Generator(device=DEV).manual_seed(7)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=DEV)
+    p = {"x": rnd(n, c).to(torch.bfloat16), "h": rnd(n, c).to(torch.bfloat16), "post_weight": None, "gate": None, "weight": 1 + 0.3 * rnd(c),
+         "scale": 0.5 * rnd(n, c), "shift": rnd(n, c)}
+    dy = rnd(n, c).to(torch.bfloat16)
+
+    def run(rows):
+        lv = {k: v if v is None else (v if v.dim() == 1 else v[rows]).detach().requires_grad_() for k, v in p.items()}
+        out, y = B.norm_between(*(lv[k] for k in NAMES))
+        return out.detach(), y.detach(), *torch.autograd.grad(y, [lv[k] for k in ("x", "h", "scale", "shift", "weight")], dy[rows])
+
+    *got, dw = run(slice(None))
+    for at in (0, 1 << 21, 1 << 22, 1 << 23, 1 << 24):
+        rows = slice(max(at - 40, 0), at + 40)
+        for a, b in zip(got, run(rows)):
+            assert torch.equal(a[rows], b)
+    s1 = got[4].double() / p["weight"].double()                             # dscale = weight * sum dy n
+    assert record("norm.launches.dweight", rel_err(dw, ((1 + p["scale"].double()) * s1).sum(0)), 5e-5) < 5e-5

@@ -727,3 +727,15 @@ def test_scales_without_a_reciprocal_are_refused():
         with pytest.raises(_lib.VdmiError, match="scale"):
             B._scale(s, 32)
     assert B._scale(2.0 ** -126, 32) == 2.0 ** -126 and B._scale(-(2.0 ** 126), 32) == -(2.0 ** 126)
+
+
+def test_calls_beyond_one_launch_are_refused():
+    """2^32 threads, of operands that all sequences may share: refused on the host, before anything is launched."""
+    lib = _lib.lib()
+    rows = lambda: _lib.Rows4(256, 0, 0, 32, 32)
+    for n in (32, 40):
+        a = _args(b=1 << 15, inner=1 << 15, n=n, heads=1, d=128, q=rows(), k=rows(), v=rows(), o=rows(), dout=rows(), dq=rows(), dk=rows(),
+                  dv=rows())
+        assert lib.vdmi_decay_attn_fwd(C.byref(a), None) == -2 and lib.vdmi_decay_attn_bwd(C.byref(a), None) == -2
+    st = (C.c_int64 * 8)(*[0, 0] * 4)
+    assert lib.vdmi_decay_attn_step(16, 16, 16, 16, st, 16, 16, 0, 1 << 26, 1, 32, 0.2, None) == -2

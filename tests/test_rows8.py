@@ -364,3 +364,14 @@ def test_nothing_is_packed_where_no_backward_can_follow(mode, monkeypatch):
         got = B.linear_rows8(x, w, b)
     assert len(packs) == 1 and not got.requires_grad and torch.equal(got, want)
     assert B.linear_rows8(x.requires_grad_(), w.detach()).requires_grad and len(packs) == 1
+
+
+def test_calls_beyond_one_launch_are_refused():
+    """2^32 threads of eight channels each, or of the shares' sums: refused on the host."""
+    lib = _lib.lib()
+    assert lib.vdmi_rows8_pack(16, 64, 16, 16, 0, 1 << 29, 64, None) == -2
+    assert lib.vdmi_rows8_unpack(16, 16, 16, 64, 0, 1 << 29, 64, None) == -2
+    assert lib.vdmi_rows8_pack(16, 8, 16, 16, 0, 1 << 30, 8, None) == -2       # three of four threads of a group are idle
+    assert lib.vdmi_rows8_wgrad_workspace_bytes(1 << 16, 1 << 16, 64) == 0
+    assert lib.vdmi_rows8_wgrad(16, 16, 16, 1 << 16, 16, None, 1 << 16, 1 << 16, 64, 16, None) == -2
+    assert lib.vdmi_rows8_wgrad_workspace_bytes(1 << 15, 1 << 15, 64) > 0

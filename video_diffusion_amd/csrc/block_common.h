@@ -7,6 +7,9 @@
 #undef __builtin_amdgcn_mfma_f32_32x32x16_bf16
 #endif
 
+// a launch has less than 2^32 threads along x
+inline bool launch_fits(long long workgroups, int threads) { return workgroups <= 0xffffffffLL / threads; }
+
 template <typename T>
 struct Pack;
 template <>

@@ -19,6 +19,8 @@
 // a fixed order.
 #include "block_common.h"
 
+#include <algorithm>
+
 namespace {
 
 struct NormArgs {
@@ -27,7 +29,7 @@ struct NormArgs {
     long long ldx, ldh, ldo, ldy, lddo, lddy, lddx, lddh;
     const float* pw; const float* gate; const float* w; const float* scale; const float* shift;
     long long gate_bs, scale_bs, shift_bs;
-    long long rows_per_sample;
+    long long rows_per_sample, sample0; // sample0: the launch's first one
     float* part;                        // [sample][parts][3][c] or null
     int c, kind, pkind, parts, rows_per_wg;     // kinds: 0 rms, 1 layer, -1 none
     float eps, alpha;
@@ -187,8 +189,9 @@ __global__ __launch_bounds__(256, P == 1 ? 4 : 1) void block_norm_kernel(const N
     __shared__ float cols[BWD && ROWS > 1 ? ROWS * L * N : 1];
     RowSum<L> sum{slots};
     const int l = threadIdx.x % L, group = threadIdx.x / L, c = a.c;
-    const long long sample = blockIdx.x / a.parts;
-    const int part = (int)(blockIdx.x - sample * a.parts);
+    const unsigned there = blockIdx.x / a.parts;
+    const long long sample = a.sample0 + there;
+    const int part = (int)(blockIdx.x - there * a.parts);
     const long long first = (long long)part * a.rows_per_wg;
     const long long last = min(first + a.rows_per_wg, a.rows_per_sample);
     const float inv_c = 1.f / (float)c;
@@ -314,7 +317,7 @@ struct SumArgs {
     long long gate_bs, scale_bs, shift_bs;
     float* dpw; float* dgate; float* dw; float* dscale; float* dshift;
     int c, parts;
-    long long samples;
+    long long samples, sample0;         // sample0: the launch's first one
 };
 
 __device__ __forceinline__ void add64(float (&v)[3], float (*buf)[3][16], int pl, int col) {
@@ -335,7 +338,7 @@ __device__ __forceinline__ void add64(float (&v)[3], float (*buf)[3][16], int pl
 __global__ __launch_bounds__(1024) void norm_sums_kernel(const SumArgs a) {
     __shared__ float buf[64][3][16];
     const int lc = threadIdx.x & 15, pl = threadIdx.x >> 4, col = blockIdx.y * 16 + lc;
-    const long long sample = blockIdx.x;
+    const long long sample = a.sample0 + blockIdx.x;
     float v[3] = {0.f, 0.f, 0.f};
     if (col < a.c) {
         const float* p = a.part + sample * a.parts * 3 * (long long)a.c + col;
@@ -483,14 +486,21 @@ NormArgs norm_args(const vdmi_block_norm_args* a, const NormPlan& p) {
     return n;
 }
 
+// workgroups of one launch: 2^23 of 256 threads and 2^21 of 1024 stay below its 2^32 threads
+constexpr long long AT_ONCE = 1LL << 23;
+
 template <bool BWD>
-int run_norm(const vdmi_block_norm_args* a, const NormArgs& n, const NormPlan& p, hipStream_t st) {
-    const long long grid = p.samples * p.parts;
-    if (grid > 0x7fffffffLL) return VDMI_E_SHAPE;
+int run_norm(const vdmi_block_norm_args* a, NormArgs n, const NormPlan& p, hipStream_t st) {
     const Shape s = shape_of(a);
-    if (a->dtype == VDMI_DT_BF16) return launch_norm<__bf16, BWD>(n, s, (unsigned)grid, st);
-    if (a->dtype == VDMI_DT_F16) return launch_norm<_Float16, BWD>(n, s, (unsigned)grid, st);
-    return launch_norm<float, BWD>(n, s, (unsigned)grid, st);
+    const long long samples = std::max(AT_ONCE / p.parts, 1LL);         // parts: 2048 at most
+    for (n.sample0 = 0; n.sample0 < p.samples; n.sample0 += samples) {
+        const unsigned grid = (unsigned)(std::min(samples, p.samples - n.sample0) * p.parts);
+        const int r = a->dtype == VDMI_DT_BF16  ? launch_norm<__bf16, BWD>(n, s, grid, st)
+                      : a->dtype == VDMI_DT_F16 ? launch_norm<_Float16, BWD>(n, s, grid, st)
+                                                : launch_norm<float, BWD>(n, s, grid, st);
+        if (r != VDMI_OK) return r;
+    }
+    return VDMI_OK;
 }
 
 }   // namespace
@@ -537,8 +547,10 @@ extern "C" int vdmi_block_norm_bwd(const vdmi_block_norm_args* a, vdmi_stream st
     s.dpw = f.dpost_weight; s.dgate = f.dgate; s.dw = f.dweight; s.dscale = f.dscale; s.dshift = f.dshift;
     s.c = f.c; s.parts = p.parts; s.samples = p.samples;
     const unsigned gx = (unsigned)((f.c + 15) / 16);
-    hipLaunchKernelGGL(norm_sums_kernel, dim3((unsigned)p.samples, gx), dim3(1024), 0, st, s);
-    VDMI_LAUNCH_CHECK();
+    for (s.sample0 = 0; s.sample0 < p.samples; s.sample0 += AT_ONCE / 4) {
+        hipLaunchKernelGGL(norm_sums_kernel, dim3((unsigned)std::min(AT_ONCE / 4, p.samples - s.sample0), gx), dim3(1024), 0, st, s);
+        VDMI_LAUNCH_CHECK();
+    }
     const bool across = p.samples > 1 && (f.dweight || f.dpost_weight || (f.dscale && !f.scale_stride) ||
                                           (f.dshift && !f.shift_stride) || (f.dgate && !f.gate_stride));
     if (!across) return VDMI_OK;

@@ -1013,7 +1013,7 @@ int launch_scan(const ScanArgs& s, const vdmi_decay_args* a, const Plan& p, hipS
     ScanArgs x = s;
     const long long segs = WHAT == STATES && !x.s_out ? p.nseg - 1 : p.nseg;
     const long long tasks = p.nseq * a->heads * segs * (a->d / 32), wgs = (tasks + DW - 1) / DW;
-    if (tasks > 0x7fffffffLL) return VDMI_E_SHAPE;
+    if (!launch_fits(wgs, DW * 64)) return VDMI_E_SHAPE;
     x.tasks = (unsigned)tasks;
     const dim3 grid((unsigned)wgs), block(DW * 64);
 #define SCAN(T, D) hipLaunchKernelGGL((decay_scan_kernel<T, D, WHAT>), grid, block, 0, st, x)
@@ -1085,6 +1085,7 @@ int launch_short(const vdmi_decay_args* a, const Plan& p, bool bwd, hipStream_t 
     for (const vdmi_rows4* r : {&a->q, &a->k, &a->v, &a->o, &a->dout, &a->dq, &a->dk, &a->dv}) two = two && (!r->p || r->h == 32);
 #define SHORT(T, D, NH, B) do { constexpr int sw = short_waves(D, B); \
     const long long wgs = ((long long)s.tiles * (a->heads / NH) + sw - 1) / sw; \
+    if (!launch_fits(wgs, sw * 64)) return VDMI_E_SHAPE; \
     hipLaunchKernelGGL((decay_short_kernel<T, D, NH, B>), dim3((unsigned)wgs), dim3(sw * 64), 0, st, s); } while (0)
 #define SHORT_D(T, B) do { if (two) SHORT(T, 32, 2, B); else if (a->d == 32) SHORT(T, 32, 1, B); else if (a->d == 64) SHORT(T, 64, 1, B); \
                            else SHORT(T, 128, 1, B); } while (0)
@@ -1107,7 +1108,7 @@ int launch_grad(const vdmi_decay_args* a, const Plan& p, hipStream_t st) {
     g.inner = a->inner; g.n = a->n; g.heads = a->heads; g.nseg = p.nseg; g.seg_len = p.seg_len;
     g.m = a->scale;
     const long long tasks = p.nseq * a->heads * p.nseg * (a->d / 32), wgs = (tasks + DW - 1) / DW;
-    if (tasks > 0x7fffffffLL) return VDMI_E_SHAPE;
+    if (!launch_fits(wgs, DW * 64)) return VDMI_E_SHAPE;
     g.tasks = (unsigned)tasks;
     const dim3 grid((unsigned)wgs), block(DW * 64);
 #define GRAD(T, D) hipLaunchKernelGGL((decay_grad_kernel<T, D>), grid, block, 0, st, g)
@@ -1198,7 +1199,7 @@ extern "C" int vdmi_decay_attn_step(const void* q, const void* k, const void* v,
     StepArgs s = {q, k, v, o, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7],
                   log_decay, state, heads, scale, seqs * heads * (d / 32)};
     const long long wgs = (s.tasks + 3) / 4;
-    if (wgs > 0x7fffffffLL) return VDMI_E_SHAPE;
+    if (!launch_fits(wgs, 256)) return VDMI_E_SHAPE;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid((unsigned)wgs), block(256);
 #define STEP(T) do { if (d == 32) hipLaunchKernelGGL((decay_step_kernel<T, 32>), grid, block, 0, st, s); \

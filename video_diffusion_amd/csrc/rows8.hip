@@ -326,7 +326,8 @@ int wgrad8_plan(int cin, int cout, int64_t rows, Wgrad8Plan* p) {
     const long long per = (stages + splits - 1) / splits;
     p->per = per * WK;
     p->splits = (int)splits;            // the last ones may be empty: a multiple of 8 stays one
-    if (tiles * p->splits > 0x7fffffffLL || (long long)cin * cout > (0x7fffffffLL - (1 << 20)) * 128) return VDMI_E_SHAPE;
+    // the shares' sums: 128 elements of dw a workgroup, 32 of db
+    if (!launch_fits(tiles * p->splits, 256) || !launch_fits((long long)cin * cout / 128 + cout / 32 + 2, 256)) return VDMI_E_SHAPE;
     p->part = (size_t)tiles * p->splits * WT * WT * sizeof(float);
     p->bytes = p->part + (size_t)p->splits * p->to * WT * sizeof(float);
     return VDMI_OK;
@@ -337,7 +338,9 @@ std::atomic<uint64_t> g_wgrad8_lds{0};
 int check_rows8(const void* x, const void* codes, const void* exps, int dtype, int64_t rows, int c, int64_t ldx) {
     if (!x || !codes || !exps) return VDMI_E_ARG;
     if (dtype != VDMI_DT_BF16 && dtype != VDMI_DT_F16 && dtype != VDMI_DT_F32) return VDMI_E_ARG;
-    if (rows <= 0 || c <= 0 || c % 8 || c > (1 << 20) || ldx < c || ldx % 8 || rows > (0x7fffffffLL * 64) / ((c + 31) / 32)) return VDMI_E_SHAPE;
+    if (rows <= 0 || c <= 0 || c % 8 || c > (1 << 20) || ldx < c || ldx % 8) return VDMI_E_SHAPE;
+    // a thread takes eight channels, of the last group also those that are not there
+    if (rows > (1LL << 32) || !launch_fits((rows * ((c + 31) / 32) * 4 + 255) / 256, 256)) return VDMI_E_SHAPE;
     if (!aligned16(x) || (reinterpret_cast<uintptr_t>(codes) & 7u)) return VDMI_E_ALIGN;
     return VDMI_OK;
 }
