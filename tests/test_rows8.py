@@ -375,3 +375,37 @@ def test_calls_beyond_one_launch_are_refused():
     assert lib.vdmi_rows8_wgrad_workspace_bytes(1 << 16, 1 << 16, 64) == 0
     assert lib.vdmi_rows8_wgrad(16, 16, 16, 1 << 16, 16, None, 1 << 16, 1 << 16, 64, 16, None) == -2
     assert lib.vdmi_rows8_wgrad_workspace_bytes(1 << 15, 1 << 15, 64) > 0
+
+
+@gpu
+@pytest.mark.parametrize("rows,o", [(40, 64), (200000, 256), (300000, 32)])
+def test_bias_gradient_of_a_frozen_weight(rows, o):
+    """The bias gradient alone, eager and from a graph that is replayed with eager work in between."""
+    from video_diffusion_amd import block_hip as B
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    x, w = torch.randn(rows, 64, generator=g, device=DEV).to(torch.bfloat16), torch.randn(o, 64, generator=g, device=DEV) / 8
+    b = torch.randn(o, generator=g, device=DEV).requires_grad_()
+    dy = torch.randn(rows, o, generator=g, device=DEV).to(torch.bfloat16)
+
+    def run():
+        return torch.autograd.grad(B.linear_rows8(x, w, b), b, dy)[0]
+
+    def check(db):
+        slack = (db.double() - dy.double().sum(0)).abs() - 1e-6 * dy.double().abs().sum(0)
+        assert float(slack.max()) <= 0
+
+    check(run())
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = new_graph()
+    with torch.cuda.graph(graph):
+        db = run()
+    for _ in range(4):
+        dy.copy_(torch.randn(rows, o, generator=g, device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(db)
+        assert torch.equal(db, run())

@@ -599,7 +599,7 @@ def _linear(x, weight, bias, keep):
 
 @_there
 def _linear_backward(dy, weight, kept, shape, need):
-    from .train_hip import _linear_pack, conv_rows
+    from .train_hip import _linear_pack, colsum_rows, conv_rows
     dx = dw = db = None
     d = _dense(dy.to(torch.bfloat16).reshape(-1, dy.shape[-1]))
     if need[0]:
@@ -608,7 +608,7 @@ def _linear_backward(dy, weight, kept, shape, need):
         dw = rows8_wgrad(Rows8(*kept, shape, torch.bfloat16), d, bias=need[2])
         dw, db = dw if need[2] else (dw, None)
     elif need[2]:
-        db = d.float().sum(0)
+        db = colsum_rows(d)             # not torch's sum: what it clears is wrong from a graph's second replay on
     return dx, dw, db
 
 
