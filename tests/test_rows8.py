@@ -409,3 +409,14 @@ def test_bias_gradient_of_a_frozen_weight(rows, o):
         torch.cuda.synchronize()
         check(db)
         assert torch.equal(db, run())
+
+
+@gpu
+def test_tensors_without_dimensions_are_refused():
+    from video_diffusion_amd import block_hip as B
+    from video_diffusion_amd._lib import VdmiError
+    one = torch.zeros((), device=DEV, dtype=torch.bfloat16)
+    kept = B.pack_rows8(torch.zeros(1, 8, device=DEV, dtype=torch.bfloat16))
+    for f in (lambda: B.pack_rows8(one), lambda: B.rows8_wgrad(kept, one), lambda: B.linear_rows8(one, torch.zeros(32, 32, device=DEV))):
+        with pytest.raises(VdmiError, match=r"\(\)|no dimensions"):
+            f()

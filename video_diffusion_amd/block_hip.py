@@ -552,7 +552,9 @@ def rows8_wgrad(kept: Rows8, dy: torch.Tensor, bias: bool = False):
     """float32 [cout][cin] weight gradient of a Linear from its input kept in 8 bits and the gradient dy [..., cout] of its
     output (bfloat16 rows); with bias also the bias gradient: (dw, db)."""
     _on_gpu(kept.codes, dy)
-    rows, cin = kept.codes.shape
+    rows = kept.codes.shape[0]
+    if dy.dim() < 1:
+        raise VdmiError("dy is [..., cout] (got no dimensions)")
     cout = dy.shape[-1]
     if dy.dtype != torch.bfloat16:
         raise VdmiError(f"dy is bfloat16 (got {dy.dtype})")
@@ -622,7 +624,7 @@ def linear_rows8(x: torch.Tensor, weight: torch.Tensor, bias=None) -> torch.Tens
         raise VdmiError("the training layers exchange bfloat16 rows: VDMI_PRECISION=f16 serves sampling only")
     if not (x.dtype == torch.bfloat16 and weight.dtype == torch.float32 and weight.dim() == 2):
         raise VdmiError(f"x is bfloat16 and weight float32 [cout, cin] (got {x.dtype}, {weight.dtype} {tuple(weight.shape)})")
-    if x.shape[-1] != weight.shape[1] or (bias is not None and bias.shape != (weight.shape[0],)):
+    if x.dim() < 1 or x.shape[-1] != weight.shape[1] or (bias is not None and bias.shape != (weight.shape[0],)):
         raise VdmiError(f"x [..., cin], weight [cout, cin], bias [cout] (got {tuple(x.shape)}, {tuple(weight.shape)})")
     if weight.shape[0] % 32 or weight.shape[1] % 32:
         raise VdmiError(f"multiples of 32 channels (got {tuple(weight.shape)})")
