@@ -12,8 +12,8 @@
 // and backward (which computes it again from x and h: reading them costs what reading the stored sum would).
 //
 // What bounds it: memory (x, h, out, y once; backward x, h, dout, dy, dx, dh once).  262144 bfloat16 rows of 256 columns:
-// forward 102 us (537 MB, 5.3 TB/s), backward 175 us (805 MB, 4.6 TB/s) and 11 us for the column sums; 3711 float32 rows of
-// 2048: 27 us (4.5 TB/s) and 44 us (4.1 TB/s), sums 10 us.  L lanes hold a row in registers, P
+// forward 102 us (537 MB, 5.3 TB/s), backward 181 us (805 MB, 4.4 TB/s) and 10 us for the column sums; 3711 float32 rows of
+// 2048: 29 us (4.2 TB/s) and 42 us (4.3 TB/s), sums 10 us.  L lanes hold a row in registers, P
 // pieces of eight columns each; a workgroup stays in one sample, so the parameters are products in registers and the column
 // sums are kept there too, added over the workgroup's rows and written once; a second launch adds the workgroups' sums in
 // a fixed order.

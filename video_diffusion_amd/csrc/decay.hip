@@ -24,10 +24,10 @@
 //     on): lambda^(31-j) v_j is the sum of three bfloat16 operands or two halfs (under 2^-22 of it is lost).
 // Few sequences: the time axis is cut into segments.  A first launch computes every segment's own contribution to the state
 // (reading k and v only), a second one runs along the segments, a third computes all outputs.
-// Measured, 2 x 8192 tokens, 8 heads of 64 features, bfloat16 (16.8 MB a tensor): segments' sums 11.6 us (2.9 TB/s), along
-// the segments 6, outputs 20 (3.4 TB/s); backward dq 20, dk and dv 31 (3.8 TB/s) beside another walk for the segments.
-// 16384 tokens, 8 heads of 128, half: 25 + 8.6 + 58 us.  There a wave has its SIMD to itself and bounds it by issuing: 61 % of
-// its cycles in the scan and 71 % in the gradients, 20 % waiting (2 x 8192 x 8 x 64).  Two
+// Measured, 2 x 8192 tokens, 8 heads of 64 features, bfloat16 (16.8 MB a tensor): segments' sums 11.7 us (2.9 TB/s), along
+// the segments 6.5, outputs 20 (3.4 TB/s); backward dq 20, dk and dv 32 (3.7 TB/s) beside another walk for the segments.
+// 16384 tokens, 8 heads of 128, half: 24 + 8.4 + 54 us.  There a wave has its SIMD to itself and bounds it by issuing: 72 % of
+// its cycles in the outputs and 66 % in the gradients, 18 and 26 % waiting (2 x 8192 x 8 x 64: 60 and 59 %, 25 and 21 %).  Two
 // waves per SIMD hide that but take twice the segments, whose states cost as much.
 #include "block_common.h"
 
@@ -172,9 +172,9 @@ struct Split {
 };
 
 // What lies in accumulator registers (weighted pairs, a state), contracted over them, as a sum of two 16-bit operands: 2^-17
-// of a bfloat16 one is lost, 2^-22 of a half (or 2^-36).  One operand alone would be rounded as coarsely as the result is: sqrt(2) of
-// its error in all (2.35e-3 in place of 1.66e-3 in bfloat16).  Kernel time with one and with two operands, forward and
-// backward: 2 x 8192 x 8 x 64 99 and 107 us, 16384 x 8 x 128 in half 238 and 300, 32 x 500 x 8 x 64 88 and 105.
+// of a bfloat16 one is lost, 2^-22 of a half (or 2^-36).  One operand alone would be rounded as coarsely as the result is:
+// sqrt(2) of its error in all (2.35e-3 in place of 1.66e-3 in bfloat16).  Kernel time with one and with two operands, forward
+// and backward: 2 x 8192 x 8 x 64 99 and 107 us, 16384 x 8 x 128 in half 238 and 300, 32 x 500 x 8 x 64 88 and 105.
 template <typename T>
 struct FineOperand {
     x8_t<T> h[2], e[2];
@@ -427,10 +427,11 @@ void decay_scan_kernel(const ScanArgs a) {
 
 // dk and dv in one walk backward in time: both read q, k, v and do, and what one of them needs of R = dS / m by columns the
 // other needs by rows.  A wave computes 32 columns of dv and the same 32 columns of dk and holds R[all dk][its columns of
-// dv] and R^T[all dv][its columns of dk].  Two walks, one for each, took 2 x 19 us and another pass over the segments where
-// this takes 25 (2 x 8192 tokens, 8 heads of 64).  With 64 features dv's half of a tile comes before dk's: that leaves 250
-// registers, none to move to and from the second file (both halves together 30.5 us; 32 x 500 x 8 x 64 39 and 32).  With 32 and
-// 128 features both halves at once are faster (16384 x 8 x 128, half: backward 137 and 144 us).
+// dv] and R^T[all dv][its columns of dk].  Two walks, one for each, are two scans of 20 us and another pass over the segments
+// of 18 where this takes 32 (2 x 8192 tokens, 8 heads of 64).  With 64 features dv's half of a tile comes before dk's, which
+// fits the registers (whole backward, halves together and apart: 2 x 8192 x 8 x 64 79 and 66 us, in half 91 and 67; 32 x 500 x
+// 8 x 64 131 and 73).  With 32 and 128 features it makes no difference (8 x 4000 x 8 x 32: 50.6 and 51.0 us; 16384 x 8 x 128, in
+// bfloat16 160 both ways); halves together are the shorter chain there.
 template <typename T, int D>
 __global__ __launch_bounds__(DW * 64, D <= 64 ? 2 : 1) void decay_grad_kernel(const GradArgs a) {
     typedef x8_t<T> x8;
@@ -453,9 +454,9 @@ __global__ __launch_bounds__(DW * 64, D <= 64 ? 2 : 1) void decay_grad_kernel(co
     at.clear<T>(a.dv, a.dvs, lane);
 
     x8 qreg[KS], greg[KS], k[KS], v[KS];
-    // 128 features leave no registers for the loads' offsets and the pairs' decays: the former are computed
+    // 128 features, and 64 of halfs, leave no registers for the loads' offsets and the pairs' decays: the former are computed
     // again for every tile, the latter read from LDS.  (From scratch memory, where the compiler would put them, each one
-    // waits for every load in flight: 16384 tokens, 8 heads took 205 us in place of 85.)
+    // waits for every load in flight: 2 x 8192 x 8 x 64 in half, 49 us in place of 33.)
     constexpr bool KEEP = D == 32 || (D == 64 && Low<T>::THREE), HALVES = D == 64;
     unsigned qofs[KEEP ? KS : 1], gofs[KEEP ? KS : 1], kofs, vofs;
     auto row_at = [&](const Rows& r, int i, int cnt) { return r.at(lane / (D / 8) + RS * i, cnt, true, 16 * (lane % (D / 8))); };
@@ -722,7 +723,7 @@ __device__ __forceinline__ bool finite(const x8_t<T> (&x)[N]) {
 
 // NH heads of D features side by side in memory are one row of W columns, moved as 16-byte pieces with all lanes of a row
 // next to each other and transposed to operands through LDS.  Measured over 16 frames of 16384 sites with 8 heads of 32
-// features (537 MB forward, 940 MB backward): 123 us and 207 us, 4.4 and 4.5 TB/s; before the pairs were two operands
+// features (537 MB forward, 940 MB backward): 123 us and 211 us, 4.4 and 4.5 TB/s; before the pairs were two operands
 // each 122 and 197 us, one head at a time (64-byte rows) 127 and 234, every lane loading and storing its own token's row as
 // operands (32 bytes of a row per instruction) 150 and 283.
 constexpr int short_waves(int d, bool bwd) { return d == 128 && bwd ? 1 : 2; }
@@ -978,12 +979,12 @@ int check_args(const vdmi_decay_args* a) {
 // per segment; the walk along the segments is serial: beyond 64 of them they are 128 tokens or longer.  Two or three
 // segments cost about what they save (k and v are read once more, the states written and read) unless they are long.
 // Measured, bfloat16, forward / backward in us (sequences x tokens x heads x features: segments):
-//     6 x 701 x 4 x 64:    1: 29/83    2: 31/61    4: 23/43    21: 19/30
-//     1 x 1000 x 8 x 128:  1: 64/185   2: 57/126   8: 25/50    31: 22/39
-//     2 x 8192 x 8 x 64:   1: 281/847  16: 45/88   32 (1024 waves): 34/62   64: 40/73
-//     1 x 4000 x 8 x 32:   32: 19/30   64: 20/27   125: 26/33
-//     32 x 500 x 8 x 64:   1: 25/67    2: 38/66        30 x 2048 x 8 x 64:  1: 101/253   2: 102/202
-//     62 x 2048 x 8 x 64:  1: 130/332  2: 184/394
+//     6 x 701 x 4 x 64:    1: 34/93    2: 34/66    4: 24/45    21: 19/31
+//     1 x 1000 x 8 x 128:  1: 78/226   2: 65/146   8: 27/55    31: 22/41
+//     2 x 8192 x 8 x 64:   1: 333/958  16: 49/94   32 (1024 waves): 36/65   64: 40/66
+//     1 x 4000 x 8 x 32:   32: 20/31   64: 20/28   125: 26/33
+//     32 x 500 x 8 x 64:   1: 28/73    2: 40/68        30 x 2048 x 8 x 64:  1: 88/260   2: 99/199
+//     62 x 2048 x 8 x 64:  1: 129/322  2: 183/398      1 x 16384 x 8 x 128:  16: 121/280   32 (1024 waves): 78/160   64: 83/185
 Plan plan(const vdmi_decay_args* a, bool states) {
     Plan p;
     p.nseq = (long long)a->b * a->inner;

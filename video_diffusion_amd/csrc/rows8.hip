@@ -132,9 +132,11 @@ __global__ __launch_bounds__(256) void rows8_unpack_kernel(const UnpackArgs a) {
 // 64 x 64 each; LDS rows are 320 bytes apart (the four rows x two column blocks of a half wave's read fall into different
 // banks).  Shares are added in a fixed order by a second launch.  The bias gradient sum_r dy comes from the staged pieces.
 // What bounds it: LDS - a wave reads 4 KB of fragments for four products of 32 cycles, what LDS gives four waves in that
-// time, and the staging comes on top.  131072 rows, 512 -> 1536 channels: 243 to 300 us (690 to 850 TFLOP/s) and 17 us for
-// the shares' sums; bfloat16 rows through vdmi_rows_wgrad 414, the library's product 709.  A 256 x 128 tile (128 x 64 per
-// wave, three quarters of the LDS reads, one workgroup per CU) took 341, one stage ahead in registers in place of two 392.
+// time, and the staging comes on top.  131072 rows, 512 -> 1536 channels: 243 us (850 TFLOP/s) in the first launches of a run
+// and after some 150 of them, 330 to 354 in between (launches 8 to 15; 297 on average over 20) - the same launches on the same
+// data, so the card's answer to the load, not the kernel's - and 17 us for the shares' sums; bfloat16 rows through
+// vdmi_rows_wgrad 414, the library's product 709.  A 256 x 128 tile (128 x 64 per wave, three quarters of the LDS reads, one
+// workgroup per CU) took 341, one stage ahead in registers in place of two 392.
 constexpr int WK = 64, WT = 128, WPITCH = 320;
 
 struct Wgrad8Args {
