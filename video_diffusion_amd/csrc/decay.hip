@@ -176,7 +176,7 @@ struct Split {
 // sqrt(2) of its error in all (2.35e-3 in place of 1.66e-3 in bfloat16).  Kernel time with one and with two operands, forward
 // and backward: 2 x 8192 x 8 x 64 99 and 107 us, 16384 x 8 x 128 in half 238 and 300, 32 x 500 x 8 x 64 88 and 105.
 // A third bfloat16 operand takes 7 % more (16 frames of 16384 sites 326 and 349 us, 2 x 8192 x 8 x 64 107 and 114) and leaves the
-// error at 1.66e-3: what two lose moves a result across a border between two values in one of some hundred cases.
+// error at 1.66e-3: what two lose moves one result in some three thousand across a border between two values.
 template <typename T>
 struct FineOperand {
     x8_t<T> h[2], e[2];
