@@ -246,17 +246,16 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengt
 
     q, k, v: bfloat16 or float16 [b, n, heads, d] or, for the sequences of many sites, [b, sites, n, heads, d]; any strides
     (views of qkv rows are read in place where their rows are 16-byte aligned).  d is 32, 64 or 128.  log_decay: float32
-    [heads], at most 0, a constant (a NaN makes its head NaN).  scale: d^-0.5 by default, 2^-126 to 2^126 in
-    magnitude.  initial_state: float32 [b(, sites), heads, d, d], S before
-    the first token (zeros by default).  lengths: int32 [b(, sites)] - tokens from there on are padding: they are not read,
-    their outputs and gradients are zeros.  return_state: also return S after the last token, for decay_attention_step or
-    the next piece of the sequence.  Returns o like q (in q's order of dimensions in memory), or (o, state).
+    [heads], at most 0, a constant (a NaN makes its head NaN).  scale: d^-0.5 by default, 2^-126 to 2^126 in magnitude.
+    initial_state: float32 [b(, sites), heads, d, d], S before the first token (zeros by default).  lengths: int32
+    [b(, sites)] - tokens from there on are padding: they do not matter, their outputs and gradients are zeros.
+    return_state: also return S after the last token, for decay_attention_step or the next piece of the sequence.  Returns o
+    like q (in q's order of dimensions in memory unless that parts tokens by more than 2^25 elements), or (o, state).
 
     Pairs scale * q_t k_j and states enter products as sums of two operands of q's dtype, so that results are rounded once,
     when they are stored: in float16 they have to stay within 65504, and 2^-36 of small ones is lost (the state that is
-    returned is float32 throughout).  A token that is not finite makes the
-    outputs from it on not finite and may make up to 31 earlier ones of its own sequence so; other sequences and tokens
-    behind lengths have no such effect."""
+    returned is float32 throughout).  A token that is not finite makes the outputs from it on not finite and may make up to 31
+    earlier ones of its own sequence so; other sequences and tokens behind lengths have no such effect."""
     dims = q.dim()
     if dims not in (4, 5):
         raise VdmiError(f"q is [b, n, heads, d] or [b, sites, n, heads, d] (got {dims} dimensions)")
